@@ -31,13 +31,21 @@ extern "C" {
 #define ESP_DTYPE_BF16 1
 #define ESP_DTYPE_F32 2
 
+/* Types of 8-bit codes.  A row of numbers is held as codes and one fp32 scale; the value of a code is code * scale.
+ * amax = max(max|x|, 2^-100); int8: scale = amax/127, code = rint(x * fl32(127/amax)), ties to even; e4m3: scale = amax/448,
+ * code = e4m3(fl32(x * fl32(448/amax))).  A row with an infinity or a NaN gets codes 0 and scale NaN. */
+#define ESP_CODE_INT8 0
+#define ESP_CODE_E4M3 1
+
 const char* esp_strerror(int code);
 /* Text of the last CUDA error seen by this library on the calling thread ("" if none). */
 const char* esp_last_cuda_error(void);
 /* ABI version of this header (bumped on incompatible change).  Version 2: the peer-memory entry points take `value_base`.
  * Version 3: the kernels that dereference slot ids take the pool's row count; the self-test kernels left the library.
- * Version 4: esp_prefill_step_strided added (nothing removed or changed). */
-#define ESP_ABI_VERSION 4
+ * Version 4: esp_prefill_step_strided added (nothing removed or changed).
+ * Version 5: the 8-bit entry points (esp_kv_*_q8, esp_decode_stage1_q8, esp_add_rms_norm*, esp_silu_and_mul_q8,
+ * esp_quantize_rows, esp_dequantize_rows, esp_mm_w8a8) added (nothing removed or changed). */
+#define ESP_ABI_VERSION 5
 int esp_abi_version(void);
 
 /* ------------------------------------------------------------------------------------------------
@@ -377,6 +385,74 @@ int esp_rotary_emb(void* x, const void* cosv, const void* sinv, int64_t x_stride
  * longserve_cuda_kernels.silu_and_mul_inplace (entrypoints.cpp:40-51, silu_and_mul.cu:17-45). */
 int esp_silu_and_mul_inplace(void* io, int64_t tokens, int32_t ffn_inter_dim, int32_t dtype,
                              void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * 8-bit serving path.  No counterpart in the reference, whose pool, activations and weights are 16-bit.
+ *
+ * KV pool in 8 bits.  Per slot and head: head_dim codes and one fp32 scale (slots are handed out token by token, so the
+ * scale belongs to one token and head).  codes: strides in bytes, multiples of 16, base 16-byte aligned; scales: the heads of
+ * a slot are next to each other, `scales_row_stride` fp32 elements between slots.  head_dim a multiple of 16, at most 512
+ * (esp_decode_stage1_q8: 128).  Slot ids outside [0, pool_rows) are skipped and reported by esp_kv_device_status; unlike
+ * the 16-bit entry points pool_rows must be given.  A slot that `dest` names twice ends up with parts of both rows. */
+
+/* codes[dest[i]], scales[dest[i]] = quantised src[i]; dtype F16/BF16 of src. */
+int esp_kv_scatter_q8(const void* src, int64_t src_row_stride, int64_t src_head_stride, void* codes,
+                      int64_t codes_row_stride, int64_t codes_head_stride, float* scales,
+                      int64_t scales_row_stride, const void* dest, int32_t idx64, int64_t n, int32_t heads2,
+                      int32_t head_dim, int32_t dtype, int32_t code, int64_t pool_rows, void* stream);
+
+/* esp_kv_scatter_register whose pool is held in 8 bits (same keep-range and registration rules). */
+int esp_kv_scatter_register_q8(int32_t batch, const int32_t* new_len, const int32_t* range_begin,
+                               const int32_t* range_end, const int64_t* new_len_cumsum, const void* kv,
+                               int64_t kv_row_stride, int64_t kv_head_stride, const int32_t* kv_b_start_loc,
+                               const int32_t* cur_kv_cache_index, const void* mem_index, int32_t idx64,
+                               void* codes, int64_t codes_row_stride, int64_t codes_head_stride, float* scales,
+                               int64_t scales_row_stride, int32_t* req_to_token, int64_t req_to_token_stride,
+                               const int32_t* b_req_idx, int64_t num_used_mem_index, int32_t max_len_in_batch,
+                               int32_t should_register, int32_t heads2, int32_t head_dim, int32_t dtype,
+                               int32_t code, int64_t pool_rows, void* stream);
+
+/* out[i] = codes[src[i]] * scales[src[i]]; dtype F16/BF16/F32 of out.  An id outside the pool gives a row of zeros. */
+int esp_kv_gather_q8(void* out, int64_t out_row_stride, int64_t out_head_stride, const void* codes,
+                     int64_t codes_row_stride, int64_t codes_head_stride, const float* scales,
+                     int64_t scales_row_stride, const void* src, int32_t idx64, int64_t n, int32_t heads2,
+                     int32_t head_dim, int32_t dtype, int32_t code, int64_t pool_rows, void* stream);
+
+/* esp_decode_stage1 over a pool held in 8 bits; the partials go to esp_decode_merge like those of the 16-bit form.
+ * dtype F16/BF16 of q.  req_rows / req_cols: rows and width of req_to_tokens; a request whose row is outside the table or
+ * whose length is beyond its width gets empty partials, and a slot id outside the pool leaves its token out; both are reported
+ * by esp_decode_device_status as ESP_ERR_BAD_SLOT (out[2] = 1 with the row, or 0 with the slot id). */
+int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q, const void* k, const void* v,
+                         const float* k_scale, const float* v_scale, int64_t k_stride_t, int64_t k_stride_h,
+                         int64_t v_stride_t, int64_t v_stride_h, int64_t k_scale_stride_t,
+                         int64_t v_scale_stride_t, const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                         int32_t req_rows, int32_t req_cols, const int32_t* b_req_idx, const int32_t* b_seqlen,
+                         int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int32_t max_len_in_batch, int32_t seq_block_size, int32_t dtype, int32_t code,
+                         float sm_scale, int64_t pool_rows, void* stream);
+
+/* t = in + residual; residual <- t rounded; out = t * rsqrt(mean(t^2) + eps) * weight, of the unrounded t.  Contiguous
+ * [tokens, hidden], hidden a multiple of 8 and at most 65536; dtype F16/BF16; fp32 arithmetic. */
+int esp_add_rms_norm(void* out, void* residual, const void* in, const void* weight, int64_t tokens,
+                     int32_t hidden, float eps, int32_t dtype, void* stream);
+/* The same with int8 rows and one scale per token instead of `out`; residual NULL: the plain norm of `in`. */
+int esp_add_rms_norm_q8(int8_t* codes, float* scale, void* residual, const void* in, const void* weight,
+                        int64_t tokens, int32_t hidden, float eps, int32_t dtype, void* stream);
+/* int8 rows of silu(io[:, :F]) * io[:, F:2F]; io contiguous [tokens, 2F] and left as it was; F as `hidden` above. */
+int esp_silu_and_mul_q8(int8_t* codes, float* scale, const void* io, int64_t tokens, int32_t ffn_inter_dim,
+                        int32_t dtype, void* stream);
+/* int8 rows of x (rows x_row_stride elements apart, a multiple of 8), and the way back (contiguous; F16/BF16/F32). */
+int esp_quantize_rows(int8_t* codes, float* scale, const void* x, int64_t x_row_stride, int64_t rows,
+                      int32_t cols, int32_t dtype, void* stream);
+int esp_dequantize_rows(void* out, const int8_t* codes, const float* scale, int64_t rows, int32_t cols,
+                        int32_t dtype, void* stream);
+
+/* out[m, n] = (sum_k a[m, k] * w[n, k]) * a_scale[m] * w_scale[n]: int8 operands with K contiguous, exact 32-bit integer
+ * sums, one rounding to out_dtype (F16/BF16/F32).  Row strides in elements; k and the int8 row strides multiples of 16,
+ * k <= 131071 (the sums stay inside 32 bits). */
+int esp_mm_w8a8(void* out, int64_t out_row_stride, const int8_t* a, int64_t a_row_stride, const float* a_scale,
+                const int8_t* w, int64_t w_row_stride, const float* w_scale, int64_t m, int64_t n, int64_t k,
+                int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,11 +14,12 @@ ATTN_LIB = os.environ.get("ESP_ATTENTION_LIB") or os.path.join(HERE, "libesp_att
 RNCCL_LIB = os.path.join(HERE, "libesp_rnccl.so")
 
 ESP_DTYPE_F16, ESP_DTYPE_BF16, ESP_DTYPE_F32 = 0, 1, 2
+ESP_CODE_INT8, ESP_CODE_E4M3 = 0, 1
 
 _i32, _i64, _f32, _vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
 # name -> argtypes, exactly as declared in include/esp_attention.h
-ESP_ABI_VERSION = 4      # what esp_abi_version() of a matching library returns (see include/esp_attention.h)
+ESP_ABI_VERSION = 5      # what esp_abi_version() of a matching library returns (see include/esp_attention.h)
 
 ATTN_SIGNATURES = {
     "esp_abi_version": [],
@@ -72,6 +73,18 @@ ATTN_SIGNATURES = {
     "esp_rms_norm": [_vp, _vp, _vp, _i64, _i32, _f32, _i32, _vp],
     "esp_rotary_emb": [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
     "esp_silu_and_mul_inplace": [_vp, _i64, _i32, _i32, _vp],
+    "esp_kv_scatter_q8": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _i64, _vp],
+    "esp_kv_scatter_register_q8": [_i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _i64,
+                                   _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _vp],
+    "esp_kv_gather_q8": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _i64, _vp],
+    "esp_decode_stage1_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _vp,
+                             _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i64, _vp],
+    "esp_add_rms_norm": [_vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _vp],
+    "esp_add_rms_norm_q8": [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _vp],
+    "esp_silu_and_mul_q8": [_vp, _vp, _vp, _i64, _i32, _i32, _vp],
+    "esp_quantize_rows": [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp],
+    "esp_dequantize_rows": [_vp, _vp, _vp, _i64, _i32, _i32, _vp],
+    "esp_mm_w8a8": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp],
 }
 ATTN_STRING_FUNCS = {"esp_strerror": [_i32], "esp_last_cuda_error": []}
 

@@ -28,6 +28,27 @@ def need_cuda(*ts):
             raise RuntimeError("the ESP attention ops run on CUDA tensors only (there is no CPU path)")
 
 
+def need_here(*ts):
+    """All tensors on the CURRENT CUDA device: the kernels are launched there, on its current stream."""
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("the ESP attention ops run on CUDA tensors only (there is no CPU path)")
+    d = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise RuntimeError(f"tensor on {t.device}, but the current CUDA device is cuda:{d}: select the tensors' device first")
+
+
+_CODES = {torch.int8: _lib.ESP_CODE_INT8, torch.float8_e4m3fn: _lib.ESP_CODE_E4M3}
+
+
+def code_tag(t: torch.Tensor) -> int:
+    try:
+        return _CODES[t.dtype]
+    except KeyError:
+        raise TypeError(f"8-bit rows are torch.int8 or torch.float8_e4m3fn, not {t.dtype}") from None
+
+
 def need_i32(*ts):
     for t in ts:
         if t.dtype != torch.int32 or not t.is_contiguous():

@@ -20,8 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 
-ATTN_SOURCES = ["kv_scatter.cu", "decode_attention.cu", "prefill_attention.cu", "layer_ops.cu",
-                "pool_allocator.cpp", "prefill_scheduler.cpp"]
+ATTN_SOURCES = ["kv_scatter.cu", "decode_attention.cu", "prefill_attention.cu", "layer_ops.cu", "kv_quant.cu", "decode_q8.cu",
+                "row_quant.cu", "w8a8_gemm.cu", "pool_allocator.cpp", "prefill_scheduler.cpp"]
 ATTN_LIB = os.path.join(HERE, "libesp_attention.so")
 RNCCL_LIB = os.path.join(HERE, "libesp_rnccl.so")
 
@@ -59,7 +59,7 @@ def _run(cmd: list[str]) -> None:
 
 def build_attention(force: bool = False, verbose_ptxas: bool = False) -> str:
     srcs = [os.path.join(CSRC, s) for s in ATTN_SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in ("esp_common.cuh", "sm100_ptx.cuh")] + \
+    deps = srcs + [os.path.join(CSRC, h) for h in ("esp_common.cuh", "sm100_ptx.cuh", "quant_common.cuh")] + \
         [os.path.join(ROOT, "include", "esp_attention.h")]
     if force or _newer(ATTN_LIB, deps):
         objs = []

@@ -558,10 +558,14 @@ extern "C" int esp_set_wait_limit_cycles(int64_t cycles) {
     return set_prefill_wait_limit(v);
 }
 
+namespace esp { int decode_q8_status(int32_t out[4], int32_t clear); }
+
 extern "C" int esp_decode_device_status(int32_t out[4], int32_t clear) {
     if (!out) return ESP_ERR_BAD_ARG;
     ESP_CUDA_TRY(cudaDeviceSynchronize());
     ESP_CUDA_TRY(cudaMemcpyFromSymbol(out, g_decode_status, sizeof(int) * 4));
+    if (out[0] == 0) return decode_q8_status(out, clear);    // the 16-bit kernels' word first, then the 8-bit kernels'
+
     if (clear) {
         int zero[4] = {0, 0, 0, 0};
         ESP_CUDA_TRY(cudaMemcpyToSymbol(g_decode_status, zero, sizeof(zero)));

@@ -400,10 +400,14 @@ extern "C" int esp_mig_scatter(const void* recv_buf, int64_t total_tokens, int32
     return ESP_OK;
 }
 
+namespace esp { int kv_q8_status(int32_t out[4], int32_t clear); }
+
 extern "C" int esp_kv_device_status(int32_t out[4], int32_t clear) {
     if (!out) return ESP_ERR_BAD_ARG;
     ESP_CUDA_TRY(cudaDeviceSynchronize());
     ESP_CUDA_TRY(cudaMemcpyFromSymbol(out, g_kv_status, sizeof(int) * 4));
+    if (out[0] == 0) return kv_q8_status(out, clear);    // the 16-bit kernels' word first, then the 8-bit kernels'
+
     if (clear) {
         int zero[4] = {0, 0, 0, 0};
         ESP_CUDA_TRY(cudaMemcpyToSymbol(g_kv_status, zero, sizeof(zero)));
