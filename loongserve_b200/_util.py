@@ -14,6 +14,14 @@ def dtype_tag(t: torch.Tensor) -> int:
         raise TypeError(f"unsupported dtype {t.dtype}") from None
 
 
+def dtype16_tag(t: torch.Tensor) -> int:
+    if t.dtype == torch.bfloat16:
+        return _lib.ESP_DTYPE_BF16
+    if t.dtype == torch.float16:
+        return _lib.ESP_DTYPE_F16
+    raise TypeError(f"expected float16 or bfloat16, not {t.dtype}")
+
+
 def ptr(t):
     return 0 if t is None else t.data_ptr()
 

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._util import code_tag, dtype_tag, need_cuda, need_here, need_i32, ptr, stream_ptr
+from ._util import code_tag, dtype16_tag, dtype_tag, need_cuda, need_here, need_i32, ptr, stream_ptr
 
 
 @torch.inference_mode()
@@ -70,7 +70,7 @@ def flash_decoding_stage1_q8(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, 
         mid_o.data_ptr(), mid_o_logexpsum.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_scale.stride(0), v_scale.stride(0), req_to_tokens.data_ptr(),
         req_to_tokens.stride(0), req_to_tokens.shape[0], req_to_tokens.shape[1], b_req_idx.data_ptr(), b_seqlen.data_ptr(), batch, hq,
-        hkv, dim, int(max_len_in_batch), int(seq_block_size), dtype_tag(q), code_tag(k), float(sm_scale),
+        hkv, dim, int(max_len_in_batch), int(seq_block_size), dtype16_tag(q), code_tag(k), float(sm_scale),
         min(k.shape[0], v.shape[0]), stream_ptr())
     _lib.check(rc, "esp_decode_stage1_q8")
 

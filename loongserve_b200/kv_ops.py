@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._util import code_tag, dtype_tag, idx64_flag, need_cuda, need_here, need_i32, ptr, stream_ptr
+from ._util import code_tag, dtype16_tag, dtype_tag, idx64_flag, need_cuda, need_here, need_i32, ptr, stream_ptr
 
 
 def _rows(t):
@@ -160,7 +160,7 @@ def destindex_copy_quantize_kv(K, DestLoc, Out, OutScale):
     assert (h, d) == (heads, dim) and DestLoc.is_contiguous() and DestLoc.dim() == 1 and DestLoc.shape[0] <= K.shape[0]
     rc = _lib.attn().esp_kv_scatter_q8(K.data_ptr(), K.stride(0), K.stride(1), Out.data_ptr(), Out.stride(0), Out.stride(1),
                                        OutScale.data_ptr(), OutScale.stride(0), DestLoc.data_ptr(), idx64_flag(DestLoc),
-                                       DestLoc.shape[0], heads, dim, dtype_tag(K), code, Out.shape[0], stream_ptr())
+                                       DestLoc.shape[0], heads, dim, dtype16_tag(K), code, Out.shape[0], stream_ptr())
     _lib.check(rc, "esp_kv_scatter_q8")
 
 
@@ -182,7 +182,7 @@ def destindex_copy_quantize_and_register_kv(batch_size, new_kv_cache_len, kv_ran
         ptr(kv), kv.stride(0), kv.stride(1), ptr(kv_b_start_loc), ptr(cur_kv_cache_index), ptr(mem_index),
         idx64_flag(mem_index), ptr(total_kv_cache), total_kv_cache.stride(0), total_kv_cache.stride(1), ptr(total_kv_scale),
         total_kv_scale.stride(0), ptr(req_to_token_indexs), req_to_token_indexs.stride(0), ptr(b_req_idx),
-        int(num_used_mem_index), int(max_len_in_batch), 1 if should_register_kv else 0, heads, dim, dtype_tag(kv), code,
+        int(num_used_mem_index), int(max_len_in_batch), 1 if should_register_kv else 0, heads, dim, dtype16_tag(kv), code,
         total_kv_cache.shape[0], stream_ptr())
     _lib.check(rc, "esp_kv_scatter_register_q8")
 

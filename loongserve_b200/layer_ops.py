@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._util import dtype_tag, need_cuda, need_here, ptr, stream_ptr
+from ._util import dtype16_tag, dtype_tag, need_cuda, need_here, ptr, stream_ptr
 
 
 @torch.inference_mode()
@@ -87,7 +87,7 @@ def add_rms_norm(input: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     output = torch.empty_like(input) if out is None else out
     assert output.shape == input.shape and output.dtype == input.dtype and output.is_contiguous()
     rc = _lib.attn().esp_add_rms_norm(output.data_ptr(), residual.data_ptr(), input.data_ptr(), weight.data_ptr(), input.size(0),
-                                      input.size(1), float(eps), dtype_tag(input), stream_ptr())
+                                      input.size(1), float(eps), dtype16_tag(input), stream_ptr())
     _lib.check(rc, "esp_add_rms_norm")
     return output
 
@@ -101,7 +101,7 @@ def add_rms_norm_quant(input: torch.Tensor, residual, weight: torch.Tensor, eps:
     tokens, hidden = input.shape
     codes, scale = _rows_out(out, out_scale, tokens, hidden, input.device)
     rc = _lib.attn().esp_add_rms_norm_q8(codes.data_ptr(), scale.data_ptr(), ptr(residual), input.data_ptr(), weight.data_ptr(), tokens,
-                                         hidden, float(eps), dtype_tag(input), stream_ptr())
+                                         hidden, float(eps), dtype16_tag(input), stream_ptr())
     _lib.check(rc, "esp_add_rms_norm_q8")
     return codes, scale
 
@@ -113,7 +113,7 @@ def silu_and_mul_quant(io: torch.Tensor, out=None, out_scale=None):
     assert io.dim() == 2 and io.is_contiguous() and io.size(1) % 2 == 0
     tokens, ffn = io.size(0), io.size(1) // 2
     codes, scale = _rows_out(out, out_scale, tokens, ffn, io.device)
-    rc = _lib.attn().esp_silu_and_mul_q8(codes.data_ptr(), scale.data_ptr(), io.data_ptr(), tokens, ffn, dtype_tag(io), stream_ptr())
+    rc = _lib.attn().esp_silu_and_mul_q8(codes.data_ptr(), scale.data_ptr(), io.data_ptr(), tokens, ffn, dtype16_tag(io), stream_ptr())
     _lib.check(rc, "esp_silu_and_mul_q8")
     return codes, scale
 
@@ -125,7 +125,7 @@ def quantize_rows(x: torch.Tensor, out=None, out_scale=None):
     need_here(x, out, out_scale)
     assert x.dim() == 2 and x.stride(1) == 1
     codes, scale = _rows_out(out, out_scale, x.size(0), x.size(1), x.device)
-    rc = _lib.attn().esp_quantize_rows(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), x.stride(0), x.size(0), x.size(1), dtype_tag(x),
+    rc = _lib.attn().esp_quantize_rows(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), x.stride(0), x.size(0), x.size(1), dtype16_tag(x),
                                        stream_ptr())
     _lib.check(rc, "esp_quantize_rows")
     return codes, scale

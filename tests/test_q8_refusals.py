@@ -190,7 +190,7 @@ def test_python_entry_points_check_shapes_and_types(no_device_check):
                    dict(req_to_token_indexs=t.long()), dict(q=x.float()), dict(q=torch.zeros(2, 2, 64, dtype=bf)), dict(cache_k=c[:, :1].float(), cache_v=c[:, 1:].float()),
                    dict(req_to_token_indexs=t.t()), dict(out=x.double()), dict(out=x[:1])):
         bad.append(lambda change=change: fd.token_decode_attention_q8(**{**good, **change}))
-    for fn in bad:
+    for n, fn in enumerate(bad):
         with pytest.raises((AssertionError, TypeError)) as e:
             fn()
-        assert "reached the library" not in str(e.value)
+        assert "reached the library" not in str(e.value), n
