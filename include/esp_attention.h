@@ -106,13 +106,13 @@ int esp_prefill_state_init(void* o, int64_t o_bytes, float* m, float* l, int64_t
 /* lse[i] = ln2*m[i] + ln(l[i])  (-inf where l == 0). */
 int esp_prefill_lse(const float* m, const float* l, float* lse, int64_t n, void* stream);
 
-/* Device-side status of the bounded waits inside the prefill kernel on the current device:
- * out[0] = 0 or ESP_ERR_DEVICE_TIMEOUT, out[1] = block index, out[2] = which wait, out[3] = detail.
+/* Device-side status of the bounded waits inside the prefill kernels and esp_mm_w8a8 on the current device:
+ * out[0] = 0 or ESP_ERR_DEVICE_TIMEOUT, out[1] = block index, out[2] = which wait (100 and above: esp_mm_w8a8), out[3] = detail.
  * Synchronises the device.  `clear` != 0 resets it. */
 int esp_device_status(int32_t out[4], int32_t clear);
 
 /* Limit, in SM cycles, of every bounded in-kernel wait of this library on the CURRENT device (the mbarrier waits of the
- * prefill kernel, the flag waits of the gated decode kernels and of esp_flag_wait).  Default 2e9 (about a second).
+ * prefill kernels and of esp_mm_w8a8, the flag waits of the gated decode kernels and of esp_flag_wait).  Default 2e9 (about a second).
  * The reference has no counterpart: its kernels never wait on one another, and its NCCL calls wait without a limit. */
 int esp_set_wait_limit_cycles(int64_t cycles);
 

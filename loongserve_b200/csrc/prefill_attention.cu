@@ -1093,10 +1093,13 @@ extern "C" int esp_prefill_lse(const float* m, const float* l, float* lse, int64
 }
 
 
+namespace esp { int mm_w8a8_status(int32_t out[4], int32_t clear); }
+
 extern "C" int esp_device_status(int32_t out[4], int32_t clear) {
     if (!out) return ESP_ERR_BAD_ARG;
     ESP_CUDA_TRY(cudaDeviceSynchronize());
     ESP_CUDA_TRY(cudaMemcpyFromSymbol(out, g_esp_status, sizeof(int) * 4));
+    if (out[0] == 0) return mm_w8a8_status(out, clear);      // the prefill kernels' word first, then the integer product's
     if (clear) {
         int zero[4] = {0, 0, 0, 0};
         ESP_CUDA_TRY(cudaMemcpyToSymbol(g_esp_status, zero, sizeof(zero)));

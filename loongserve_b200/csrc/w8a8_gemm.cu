@@ -1,62 +1,495 @@
 // Product of 8-bit integer matrices with a scale for every token and every output channel:
 //   out[m, n] = (sum_k a[m, k] * w[n, k]) * a_scale[m] * w_scale[n]
-// a [M, K] int8 rows of tokens, w [N, K] int8 rows of output channels (both with K contiguous), 32-bit integer sums, one
-// rounding to the output type.  K <= 131071 keeps every sum inside 32 bits (128 * 128 * K < 2^31).
+// a [M, K] int8 rows of tokens, w [N, K] int8 rows of output channels (both with K contiguous), 32-bit integer sums in tensor
+// memory (tcgen05.mma kind::i8), two fp32 products and one rounding to the output type in the epilogue.  K <= 131071 keeps every
+// sum inside 32 bits (128 * 128 * K < 2^31).  Integer sums do not depend on their order, so every split below gives the same bits.
 //
-// First form: 64 x 64 tiles on the integer dot-product units.
+// Operand tiles are 128 bytes of K wide, 128-byte swizzle, fetched by TMA (rows and bytes behind the matrix arrive as zeros).
+#include <cuda.h>
+
 #include "quant_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace esp {
+
+using namespace ptx;
+
+constexpr int kBK = 128;                 // bytes of K per stage: one swizzle row, four MMA steps of 32
+
+// Status of the bounded mbarrier waits: {ESP_ERR_DEVICE_TIMEOUT, block, which wait, detail}; their limit in SM cycles.
+__device__ int g_mm_status[4];
+__device__ long long g_mm_wait_limit_cycles = 2000000000LL;
+
+enum MmWait { MW_EMPTY = 100, MW_FULL = 101, MW_ACC_EMPTY = 102, MW_ACC_FULL = 103, MW_DRAIN = 104 };
+
+__device__ __noinline__ void mm_timeout(int which, int detail) {
+    if (atomicCAS(&g_mm_status[0], 0, ESP_ERR_DEVICE_TIMEOUT) == 0) {
+        g_mm_status[1] = blockIdx.x + gridDim.x * blockIdx.y;
+        g_mm_status[2] = which;
+        g_mm_status[3] = detail;
+    }
+}
+// false: the wait ran out (here or, through *s_abort, in another warp of the CTA); the caller drains and leaves
+__device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, volatile int* s_abort, int which, int detail) {
+    const int r = mbar_wait_bounded(bar, parity, &g_mm_wait_limit_cycles, s_abort);
+    if (r == 2) { mm_timeout(which, detail); *s_abort = 1; }
+    return r == 0;
+}
+// after an abort: wait (bounded, whatever the abort flag says) for work of one's own that is still in flight
+__device__ __forceinline__ void mm_drain(uint32_t bar, uint32_t parity) {
+    mbar_wait_bounded(bar, parity, &g_mm_wait_limit_cycles, nullptr);
+}
 
 template <typename OT> __device__ __forceinline__ OT from_f32(float x);
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-struct MmArgs {
-    void* out; int64_t ldo; const int8_t* a; int64_t lda; const float* a_scale; const int8_t* w; int64_t ldw; const float* w_scale;
-    int64_t M, N; int K;
+template <typename OT> struct Pack16;      // 16 bytes of outputs from consecutive fp32 values
+template <> struct Pack16<float> {
+    static constexpr int n = 4;
+    static __device__ __forceinline__ uint4 go(const float* x) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+};
+template <typename OT> struct Pack16 {
+    static constexpr int n = 8;
+    static __device__ __forceinline__ uint4 go(const float* x) {
+        return make_uint4(Cvt<OT>::pack(x[0], x[1]), Cvt<OT>::pack(x[2], x[3]), Cvt<OT>::pack(x[4], x[5]), Cvt<OT>::pack(x[6], x[7]));
+    }
 };
 
+struct MmArgs {
+    void* out; int64_t ldo; const float* a_scale; const float* w_scale;
+    int64_t M, N; int kstages;           // kstages = ceil(K / 128)
+    int m_tiles, n_tiles;
+    int vec_out;                         // rows of out are 16-byte aligned
+};
+
+// ------------------------------------------------------------------------------------------------
+// Many tokens: CTA pairs (cluster of two, cta_group::2).  A pair owns 256 tokens x 256 channels; CTA c holds 128 of the tokens
+// (A) and half of the channels (B), one thread of the even CTA issues the M = 256 MMAs that run on both SMs.  Persistent: each
+// pair walks over tiles; two accumulators of 256 columns take turns, so the epilogue of one tile runs under the next one's MMAs.
+// Warps: 0 producer, 1 issuer (and tensor-memory owner), 2-3 idle, 4-7 epilogue (one token row per thread).
+constexpr int kPairM = 128, kPairN = 256, kPairStages = 6, kPairThreads = 256;
+constexpr int kPairStageBytes = kPairM * kBK + kPairN / 2 * kBK;                 // 32 KiB per CTA
+constexpr int kEpiRowBytes = 128 + 16;                                           // one staged row piece, padded against bank conflicts
+constexpr int kPairOffEpi = kPairStages * kPairStageBytes;                       // per epilogue warp: 32 row pieces, 256 channel scales
+constexpr int kPairEpiWarp = 32 * kEpiRowBytes + kPairN * 4;
+constexpr int kPairOffBar = kPairOffEpi + 4 * kPairEpiWarp;
+enum { MB_FULL = 0, MB_EMPTY = kPairStages, MB_ACC_FULL = 2 * kPairStages, MB_ACC_EMPTY = 2 * kPairStages + 2, MB_DRAIN = 2 * kPairStages + 4,
+       MB_COUNT = 2 * kPairStages + 5 };
+constexpr int kPairOffMisc = kPairOffBar + MB_COUNT * 8;
+constexpr int kPairSmem = kPairOffMisc + 16 + 1024;
+static_assert(kPairSmem <= 232448, "shared memory of one CTA");
+
+// Tiles are walked in bands of 8 token tiles: the pairs that run together share both operands' tiles in L2.
+__device__ __forceinline__ void tile_of(int t, int m_tiles, int n_tiles, int& m, int& n) {
+    constexpr int kBand = 8;
+    const int band = t / (kBand * n_tiles), in_band = t - band * kBand * n_tiles;
+    const int rows = min(kBand, m_tiles - band * kBand);
+    n = in_band / rows;
+    m = band * kBand + (in_band - n * rows);
+}
+
 template <typename OT>
-__global__ void __launch_bounds__(256) mm_w8a8_tile_kernel(MmArgs g) {
-    __shared__ uint32_t sa[64][17], sw[64][17];                  // 64 rows x 64 bytes, padded against bank conflicts
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int lr = threadIdx.x >> 2, lc = threadIdx.x & 3;       // loader: row, 16-byte piece
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < g.K; k0 += 64) {
-        uint4 va = make_uint4(0, 0, 0, 0), vw = va;
-        const int k = k0 + lc * 16;
-        if (k < g.K) {
-            if (m0 + lr < g.M) va = *reinterpret_cast<const uint4*>(g.a + (m0 + lr) * g.lda + k);
-            if (n0 + lr < g.N) vw = *reinterpret_cast<const uint4*>(g.w + (n0 + lr) * g.ldw + k);
+__global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
+                                                                       const __grid_constant__ CUtensorMap tm_w, const MmArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    auto bar = [base](int i) { return base + kPairOffBar + 8u * i; };
+    auto lbar = [&bar](int i) { return map_to_cta(bar(i), 0u); };               // the even CTA's barrier
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + kPairOffMisc);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(gen + kPairOffMisc + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cta = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int tiles = p.m_tiles * p.n_tiles;
+
+    if (threadIdx.x == 0) {
+        *s_abort = (*reinterpret_cast<volatile int*>(&g_mm_status[0]) != 0) ? 1 : 0;    // after a reported timeout nothing is started
+        for (int i = 0; i < MB_COUNT; ++i) mbar_init(bar(i), (i == MB_ACC_EMPTY || i == MB_ACC_EMPTY + 1) ? 8 : 1);
+        fence_barrier_init();
+        prefetch_tensormap(&tm_a); prefetch_tensormap(&tm_w);
+    }
+    __syncthreads();
+    if (warp == 1) { tmem_alloc_pair(base + kPairOffMisc, 2 * kPairN); tmem_relinquish_pair(); }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+
+    if (warp == 0) {
+        if (lane == 0 && !*s_abort) {
+            int it = 0;
+            bool ok = true;
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                int mt, nt;
+                tile_of(t, p.m_tiles, p.n_tiles, mt, nt);
+                const int m0 = mt * 2 * kPairM + (int)cta * kPairM, n0 = nt * kPairN + (int)cta * (kPairN / 2);
+                for (int k = 0; k < p.kstages; ++k, ++it) {
+                    const int st = it % kPairStages;
+                    if (it >= kPairStages && !(ok = mm_wait(bar(MB_EMPTY + st), ((it / kPairStages) - 1) & 1, s_abort, MW_EMPTY, it))) break;
+                    if (cta == 0) mbar_expect_tx(bar(MB_FULL + st), 2 * kPairStageBytes);
+                    const uint32_t dst = base + st * kPairStageBytes;
+                    tma_load_2d_pair(dst, &tm_a, lbar(MB_FULL + st), k * kBK, m0);
+                    tma_load_2d_pair(dst + kPairM * kBK, &tm_w, lbar(MB_FULL + st), k * kBK, n0);
+                }
+            }
+            if (!ok && cta == 0)                               // copies of both CTAs count on the even CTA's barriers
+                for (int i = it > kPairStages ? it - kPairStages : 0; i < it; ++i) mm_drain(bar(MB_FULL + i % kPairStages), (i / kPairStages) & 1);
         }
-        __syncthreads();
-        sa[lr][lc * 4] = va.x; sa[lr][lc * 4 + 1] = va.y; sa[lr][lc * 4 + 2] = va.z; sa[lr][lc * 4 + 3] = va.w;
-        sw[lr][lc * 4] = vw.x; sw[lr][lc * 4 + 1] = vw.y; sw[lr][lc * 4 + 2] = vw.z; sw[lr][lc * 4 + 3] = vw.w;
-        __syncthreads();
+    } else if (warp == 1) {
+        if (cta == 0 && lane == 0 && !*s_abort) {
+            constexpr uint32_t idesc = make_idesc_i8(2 * kPairM, kPairN);
+            int it = 0, n_tile = 0;
+            bool ok = true;
+            for (int t = pair; t < tiles && ok; t += pairs, ++n_tile) {
+                const int buf = n_tile & 1;
+                if (n_tile >= 2 && !(ok = mm_wait(bar(MB_ACC_EMPTY + buf), ((n_tile >> 1) - 1) & 1, s_abort, MW_ACC_EMPTY, n_tile))) break;
+                tc_fence_after();
+                for (int k = 0; k < p.kstages; ++k, ++it) {
+                    const int st = it % kPairStages;
+                    if (!(ok = mm_wait(bar(MB_FULL + st), (it / kPairStages) & 1, s_abort, MW_FULL, it))) break;
+                    tc_fence_after();
+                    const uint32_t sa = base + st * kPairStageBytes, sb = sa + kPairM * kBK;
 #pragma unroll
-        for (int kk = 0; kk < 16; ++kk) {
-            int x[4], y[4];
+                    for (int j = 0; j < kBK / 32; ++j)
+                        umma_i8_pair_ss(tmem + buf * kPairN, desc_kmajor_sw128(sa + j * 32), desc_kmajor_sw128(sb + j * 32), idesc, (k | j) != 0);
+                    umma_pair_commit(bar(MB_EMPTY + st));
+                }
+                if (ok) umma_pair_commit(bar(MB_ACC_FULL + buf));
+            }
+            if (!ok) { umma_pair_commit(bar(MB_DRAIN)); mm_drain(bar(MB_DRAIN), 0); }
+        }
+    } else if (warp >= 4) {
+        const int w = warp - 4;
+        uint8_t* stage = gen + kPairOffEpi + w * kPairEpiWarp;
+        float* sw = reinterpret_cast<float*>(stage + 32 * kEpiRowBytes);
+        constexpr int kCols = 128 / (int)sizeof(OT);           // channels per staged piece (128 bytes of a row)
+        OT* out = reinterpret_cast<OT*>(p.out);
+        bool ok = !*s_abort;
+        int n_tile = 0;
+        for (int t = pair; t < tiles && ok; t += pairs, ++n_tile) {
+            int mt, nt;
+            tile_of(t, p.m_tiles, p.n_tiles, mt, nt);
+            const int64_t row0 = (int64_t)mt * 2 * kPairM + (int64_t)cta * kPairM + w * 32;      // first row of this warp
+            const int64_t n0 = (int64_t)nt * kPairN;
+            const int buf = n_tile & 1;
+            __syncwarp();
+            for (int i = lane; i < kPairN; i += 32) sw[i] = n0 + i < p.N ? p.w_scale[n0 + i] : 0.f;
+            const float sa = row0 + lane < p.M ? p.a_scale[row0 + lane] : 0.f;
+            ok = mm_wait(bar(MB_ACC_FULL + buf), (n_tile >> 1) & 1, s_abort, MW_ACC_FULL, n_tile);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * kPairN + ((uint32_t)(w * 32) << 16);
+            const int rows = (int)min((int64_t)32, p.M - row0);
+#pragma unroll 1
+            for (int c0 = 0; c0 < kPairN; c0 += kCols) {
+                uint32_t r[kCols / 32][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { x[i] = (int)sa[ty + 16 * i][kk]; y[i] = (int)sw[tx + 16 * i][kk]; }
+                for (int h = 0; h < kCols / 32; ++h) tmem_ld32(acc + c0 + h * 32, r[h]);
+                tmem_wait_ld();
+                if (c0 + kCols == kPairN) {                     // the last read of this accumulator: the issuer may have it back
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(lbar(MB_ACC_EMPTY + buf));
+                }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int h = 0; h < kCols / 32; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(x[i], y[j], acc[i][j]);
+                    for (int i = 0; i < 32; i += Pack16<OT>::n) {
+                        float x[Pack16<OT>::n];
+#pragma unroll
+                        for (int j = 0; j < Pack16<OT>::n; ++j) x[j] = __int2float_rn((int)r[h][i + j]) * sa * sw[c0 + h * 32 + i + j];
+                        *reinterpret_cast<uint4*>(stage + lane * kEpiRowBytes + (h * 32 + i) * (int)sizeof(OT)) = Pack16<OT>::go(x);
+                    }
+                __syncwarp();
+                const int64_t nleft = p.N - n0 - c0;
+                const int ncols = nleft < kCols ? (int)nleft : kCols;
+                if (p.vec_out && ncols == kCols) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {               // 4 rows of 128 bytes per step
+                        const int rr = i * 4 + (lane >> 3);
+                        if (rr < rows)
+                            *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + (row0 + rr) * p.ldo + n0 + c0) + (lane & 7) * 16) =
+                                *reinterpret_cast<const uint4*>(stage + rr * kEpiRowBytes + (lane & 7) * 16);
+                    }
+                } else {
+                    for (int rr = 0; rr < rows; ++rr)
+                        for (int i = lane; i < ncols; i += 32)
+                            out[(row0 + rr) * p.ldo + n0 + c0 + i] = *reinterpret_cast<const OT*>(stage + rr * kEpiRowBytes + i * sizeof(OT));
+                }
+                __syncwarp();
+            }
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                  // neither CTA frees tensor memory while the peer's MMAs may still use it
+    if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 2 * kPairN); }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Few tokens: the weights are what is read, so channels take the 128 rows of the MMA and TN tokens its columns.  A cluster of S
+// CTAs splits K of one tile; the integer partials are summed through distributed shared memory (each CTA sums and writes TN / S
+// of the tokens).  Warps: 0 producer, 1 issuer, 2-5 epilogue (one channel per thread).
+constexpr int kSkinnyThreads = 192;
+template <int TN> struct Skinny {
+    static constexpr int kStageBytes = 128 * kBK + TN * kBK;
+    static constexpr int kStages = TN >= 256 ? 4 : (TN >= 128 ? 6 : (TN >= 64 ? 4 : 5));
+    static constexpr int kDump = 128 * TN * 4;                      // partials, over the pipeline's stages once they are used up
+    static constexpr int kBody = kStages * kStageBytes > kDump ? kStages * kStageBytes : kDump;
+    static constexpr int kOffBar = kBody;
+    static constexpr int kOffMisc = kOffBar + (2 * kStages + 1) * 8;
+    static constexpr int kSmem = kOffMisc + 16 + 1024;
+    static constexpr int kCols = TN < 32 ? 32 : TN;
+};
+
+template <typename OT, int TN>
+__global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __grid_constant__ CUtensorMap tm_a,
+                                                                        const __grid_constant__ CUtensorMap tm_w, const MmArgs p, int splits) {
+    using C = Skinny<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    auto bar = [base](int i) { return base + C::kOffBar + 8u * i; };      // full [stages], empty [stages], done
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::kOffMisc);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)cluster_ctarank();
+    const int n0 = (blockIdx.x / splits) * 128, m0 = blockIdx.y * TN;
+    const int k0 = (int)((int64_t)p.kstages * split / splits), k1 = (int)((int64_t)p.kstages * (split + 1) / splits);
+    const int nk = k1 - k0;                                               // at least one: splits <= kstages
+
+    if (threadIdx.x == 0) {
+        *s_abort = (*reinterpret_cast<volatile int*>(&g_mm_status[0]) != 0) ? 1 : 0;
+        for (int i = 0; i < 2 * C::kStages + 1; ++i) mbar_init(bar(i), 1);
+        fence_barrier_init();
+        prefetch_tensormap(&tm_a); prefetch_tensormap(&tm_w);
+    }
+    if (warp == 1) { tmem_alloc(base + C::kOffMisc, C::kCols); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    bool ok = !*s_abort;
+
+    if (warp == 0) {
+        if (lane == 0 && ok) {
+            int it = 0;
+            for (; it < nk; ++it) {
+                const int st = it % C::kStages;
+                if (it >= C::kStages && !(ok = mm_wait(bar(C::kStages + st), ((it / C::kStages) - 1) & 1, s_abort, MW_EMPTY, it))) break;
+                mbar_expect_tx(bar(st), C::kStageBytes);
+                const uint32_t dst = base + st * C::kStageBytes;
+                tma_load_2d(dst, &tm_w, bar(st), (k0 + it) * kBK, n0);
+                tma_load_2d(dst + 128 * kBK, &tm_a, bar(st), (k0 + it) * kBK, m0);
+            }
+            if (!ok)
+                for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) mm_drain(bar(i % C::kStages), (i / C::kStages) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && ok) {
+            constexpr uint32_t idesc = make_idesc_i8(128, TN);
+            for (int it = 0; it < nk; ++it) {
+                const int st = it % C::kStages;
+                if (!(ok = mm_wait(bar(st), (it / C::kStages) & 1, s_abort, MW_FULL, it))) break;
+                tc_fence_after();
+                const uint32_t sw = base + st * C::kStageBytes, sa = sw + 128 * kBK;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t m = m0 + ty + 16 * i;
-        if (m >= g.M) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t n = n0 + tx + 16 * j;
-            if (n < g.N) reinterpret_cast<OT*>(g.out)[m * g.ldo + n] = from_f32<OT>((float)acc[i][j] * g.a_scale[m] * g.w_scale[n]);
+                for (int j = 0; j < kBK / 32; ++j)
+                    umma_i8_ss(tmem, desc_kmajor_sw128(sw + j * 32), desc_kmajor_sw128(sa + j * 32), idesc, (it | j) != 0);
+                umma_commit(bar(C::kStages + st));
+            }
+            umma_commit(bar(2 * C::kStages));                             // every MMA issued, in the aborted case too
+            if (!ok) mm_drain(bar(2 * C::kStages), 0);
         }
     }
+    int32_t* dump = reinterpret_cast<int32_t*>(gen);                      // [TN][128]
+    if (warp >= 2) {
+        const int q = warp & 3;                                           // the quarter of the tensor-memory lanes this warp may read
+        if (ok) ok = mm_wait(bar(2 * C::kStages), 0, s_abort, MW_DRAIN, nk);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < TN; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dump[(c + i) * 128 + q * 32 + lane] = (int)r[i];
+            }
+            tc_fence_before();
+        }
+    }
+    // every CTA of the cluster passes here, also one whose waits ran out (its partials are then not there: the status says so)
+    __syncthreads();
+    if (splits > 1) cluster_sync_all();
+    {
+        OT* out = reinterpret_cast<OT*>(p.out);
+        const int t_lo = TN * split / splits, t_hi = TN * (split + 1) / splits;
+        const int64_t M = p.M, N = p.N;
+        const uint32_t my = base;
+        for (int i = threadIdx.x; i < (t_hi - t_lo) * 64; i += kSkinnyThreads) {       // two channels of one token
+            const int t = t_lo + (i >> 6), ch = (i & 63) * 2;
+            const int64_t m = m0 + t, n = n0 + ch;
+            if (m >= M) break;
+            if (n >= N) continue;
+            int s0 = 0, s1 = 0;
+            for (int r = 0; r < splits; ++r) {
+                int v0, v1;
+                const uint32_t at = (splits > 1 ? map_to_cta(my, r) : my) + (uint32_t)(t * 128 + ch) * 4u;
+                asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v0), "=r"(v1) : "r"(at));
+                s0 += v0; s1 += v1;
+            }
+            const float sa = p.a_scale[m];
+            const float x0 = __int2float_rn(s0) * sa * p.w_scale[n];
+            OT* o = out + m * p.ldo + n;
+            if (n + 1 < N) {
+                const float x1 = __int2float_rn(s1) * sa * p.w_scale[n + 1];
+                if (p.vec_out) {
+                    if constexpr (sizeof(OT) == 2) *reinterpret_cast<uint32_t*>(o) = Cvt<OT>::pack(x0, x1);
+                    else *reinterpret_cast<float2*>(o) = make_float2(x0, x1);
+                } else { o[0] = from_f32<OT>(x0); o[1] = from_f32<OT>(x1); }
+            } else {
+                o[0] = from_f32<OT>(x0);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (splits > 1) cluster_sync_all();                                   // peers may still read this CTA's partials
+    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, C::kCols); }
+}
+
+// ------------------------------------------------------------------------------------------------
+typedef CUresult (*MmEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// int8 matrix [rows, K]: box = 128 bytes of K x box_rows rows, 128-byte swizzle
+static int make_map(CUtensorMap* tm, const int8_t* p, int64_t rows, int64_t k, int64_t ld, int box_rows) {
+    static MmEncodeFn fn = nullptr;
+    if (!fn) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<MmEncodeFn>(f);
+        if (!fn) { snprintf(last_cuda_error_buf(), 256, "cuTensorMapEncodeTiled entry point not found"); return ESP_ERR_CUDA; }
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows}, es[2] = {1, 1};
+    const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(last_cuda_error_buf(), 256, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+        return ESP_ERR_CUDA;
+    }
+    return ESP_OK;
+}
+
+constexpr int kMaxMmDevices = 64;
+
+// How many CTA pairs the device keeps resident at once (asked once per device and kernel).
+template <typename OT>
+static int resident_pairs(int* out) {
+    static int known[kMaxMmDevices] = {0};
+    int dev = -1;
+    ESP_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= kMaxMmDevices) return ESP_ERR_UNSUPPORTED;
+    if (!known[dev]) {
+        ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_pair_kernel<OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(kNumSMs / 2 * 2); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = kPairSmem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        cfg.attrs = at; cfg.numAttrs = 1;
+        int n = 0;
+        ESP_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, mm_w8a8_pair_kernel<OT>, &cfg));
+        known[dev] = n > 0 ? n : 1;
+    }
+    *out = known[dev];
+    return ESP_OK;
+}
+
+template <typename OT>
+static int launch_pair(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, int64_t k, MmArgs g, cudaStream_t s) {
+    CUtensorMap ta, tw;
+    int rc = make_map(&ta, a, g.M, k, lda, kPairM);
+    if (!rc) rc = make_map(&tw, w, g.N, k, ldw, kPairN / 2);
+    int pairs = 0;
+    if (!rc) rc = resident_pairs<OT>(&pairs);
+    if (rc) return rc;
+    g.m_tiles = (int)((g.M + 2 * kPairM - 1) / (2 * kPairM));
+    g.n_tiles = (int)((g.N + kPairN - 1) / kPairN);
+    const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles;
+    if (tiles > 2147483647LL) return ESP_ERR_TOO_LARGE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)); cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem; cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_pair_kernel<OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    ESP_CUDA_TRY(cudaLaunchKernelEx(&cfg, mm_w8a8_pair_kernel<OT>, ta, tw, g));
+    return ESP_OK;
+}
+
+template <typename OT, int TN>
+static int launch_skinny(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, int64_t k, MmArgs g, int splits, cudaStream_t s) {
+    using C = Skinny<TN>;
+    CUtensorMap ta, tw;
+    int rc = make_map(&ta, a, g.M, k, lda, TN);
+    if (!rc) rc = make_map(&tw, w, g.N, k, ldw, 128);
+    if (rc) return rc;
+    const int64_t nt = (g.N + 127) / 128, mt = (g.M + TN - 1) / TN;
+    if (mt > 65535 || nt * splits > 2147483647LL) return ESP_ERR_TOO_LARGE;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(nt * splits), (unsigned)mt); cfg.blockDim = dim3(kSkinnyThreads);
+    cfg.dynamicSmemBytes = C::kSmem; cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_skinny_kernel<OT, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    ESP_CUDA_TRY(cudaLaunchKernelEx(&cfg, mm_w8a8_skinny_kernel<OT, TN>, ta, tw, g, splits));
+    return ESP_OK;
+}
+
+template <typename OT>
+static int launch_mm(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, int64_t k, MmArgs g, cudaStream_t s) {
+    g.kstages = (int)((k + kBK - 1) / kBK);
+    g.vec_out = ((uintptr_t)g.out % 16 == 0 && (g.ldo * (int64_t)sizeof(OT)) % 16 == 0) ? 1 : 0;
+    if (g.M > 256) return launch_pair<OT>(a, lda, w, ldw, k, g, s);
+    // enough CTAs that two per SM have work, as long as each keeps a few stages of K
+    const int64_t nt = (g.N + 127) / 128;
+    int splits = (int)(2 * kNumSMs / nt);
+    splits = splits > 8 ? 8 : (splits < 1 ? 1 : splits);
+    while (splits > 1 && g.kstages < 4 * splits) --splits;
+    if (g.M <= 16) return launch_skinny<OT, 16>(a, lda, w, ldw, k, g, splits, s);
+    if (g.M <= 32) return launch_skinny<OT, 32>(a, lda, w, ldw, k, g, splits, s);
+    if (g.M <= 64) return launch_skinny<OT, 64>(a, lda, w, ldw, k, g, splits, s);
+    if (g.M <= 128) return launch_skinny<OT, 128>(a, lda, w, ldw, k, g, splits, s);
+    return launch_skinny<OT, 256>(a, lda, w, ldw, k, g, splits, s);
+}
+
+int mm_w8a8_status(int32_t out[4], int32_t clear) {
+    ESP_CUDA_TRY(cudaMemcpyFromSymbol(out, g_mm_status, sizeof(int) * 4));
+    if (clear) {
+        int zero[4] = {0, 0, 0, 0};
+        ESP_CUDA_TRY(cudaMemcpyToSymbol(g_mm_status, zero, sizeof(zero)));
+    }
+    return ESP_OK;
+}
+int set_mm_wait_limit(long long cycles) {
+    ESP_CUDA_TRY(cudaMemcpyToSymbol(g_mm_wait_limit_cycles, &cycles, sizeof(cycles)));
+    return ESP_OK;
 }
 
 }  // namespace esp
@@ -67,16 +500,13 @@ extern "C" int esp_mm_w8a8(void* out, int64_t out_row_stride, const int8_t* a, i
                            int64_t w_row_stride, const float* w_scale, int64_t m, int64_t n, int64_t k, int32_t out_dtype, void* stream) {
     if (m == 0 || n == 0) return ESP_OK;
     if (!out || !a || !a_scale || !w || !w_scale || m < 0 || n < 0 || k <= 0) return ESP_ERR_BAD_ARG;
+    if (out_dtype != ESP_DTYPE_F16 && out_dtype != ESP_DTYPE_BF16 && out_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
     if (out_row_stride < n || a_row_stride < k || w_row_stride < k) return ESP_ERR_BAD_ARG;
     if (k % 16 || a_row_stride % 16 || w_row_stride % 16 || !aligned16(a) || !aligned16(w)) return ESP_ERR_ALIGNMENT;
-    if (k > 131071 || m > 4194240 || n > 2147483647LL) return ESP_ERR_TOO_LARGE;
-    const MmArgs g{out, out_row_stride, a, a_row_stride, a_scale, w, w_row_stride, w_scale, m, n, (int)k};
-    const dim3 grid((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64));
+    if (k > 131071 || m > 2147483392LL || n > 2147483392LL) return ESP_ERR_TOO_LARGE;       // tile coordinates are 32-bit
+    MmArgs g{out, out_row_stride, a_scale, w_scale, m, n, 0, 0, 0, 0};
     cudaStream_t s = (cudaStream_t)stream;
-    if (out_dtype == ESP_DTYPE_F16) mm_w8a8_tile_kernel<__half><<<grid, 256, 0, s>>>(g);
-    else if (out_dtype == ESP_DTYPE_BF16) mm_w8a8_tile_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(g);
-    else if (out_dtype == ESP_DTYPE_F32) mm_w8a8_tile_kernel<float><<<grid, 256, 0, s>>>(g);
-    else return ESP_ERR_BAD_ARG;
-    ESP_LAUNCH_CHECK("mm_w8a8_tile_kernel");
-    return ESP_OK;
+    if (out_dtype == ESP_DTYPE_F16) return launch_mm<__half>(a, a_row_stride, w, w_row_stride, k, g, s);
+    if (out_dtype == ESP_DTYPE_BF16) return launch_mm<__nv_bfloat16>(a, a_row_stride, w, w_row_stride, k, g, s);
+    return launch_mm<float>(a, a_row_stride, w, w_row_stride, k, g, s);
 }
