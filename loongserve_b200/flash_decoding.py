@@ -76,10 +76,10 @@ def flash_decoding_stage1_q8(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, 
 
 
 def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -> int:
-    """Tokens per split: enough CTAs to fill the GPU several times over when rows are few, not below 256 tokens."""
+    """Tokens per split: enough CTAs to fill the GPU several times over when rows are few, not below 128 tokens."""
     ctas = max(1, batch * kv_heads * ((group + 7) // 8))
-    splits = max(1, (148 * 8 + ctas - 1) // ctas)
-    return max(256, -(-max(int(max_len_in_batch), 1) // splits // 64) * 64)
+    splits = max(1, (148 * 12 + ctas - 1) // ctas)
+    return min(1024, max(128, -(-max(int(max_len_in_batch), 1) // splits // 128) * 128))
 
 
 @torch.inference_mode()

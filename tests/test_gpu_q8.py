@@ -175,12 +175,13 @@ def decode_case(lens, hq, hkv, dtype, code, seed, q_scale=1.5, pool_extra=3):
 
 
 def decode_exact(c, lens=None, sm_scale=None):
-    """(o, lse, sum p|v| / sum p, max over tokens of sum|q k| * sm_scale) in 64 bits."""
+    """(o, lse, sum p|v| / sum p, max over tokens of sum|q k| * sm_scale, tokens * largest v scale * top code) in 64 bits."""
     B, hq, _ = c["q"].shape
     hkv = c["hkv"]
     sm = sm_scale or D ** -0.5
     o = torch.zeros(B, hq, D, dtype=torch.float64); lse = torch.full((B, hq), -math.inf, dtype=torch.float64)
     wabs = torch.zeros_like(o); sabs = torch.zeros(B, hq, dtype=torch.float64)
+    floor = torch.zeros(B, hq, 1, dtype=torch.float64)
     for b, n in enumerate(lens if lens is not None else c["lens"].tolist()):
         if n == 0:
             continue
@@ -196,16 +197,21 @@ def decode_exact(c, lens=None, sm_scale=None):
         o[b] = (p[..., None] * v).sum(0).cpu(); wabs[b] = (p[..., None] * v.abs()).sum(0).cpu()
         lse[b] = torch.logsumexp(s, 0).cpu()
         sabs[b] = ((q[None] * k).abs().sum(-1) * sm).amax(0).cpu()
-    return o, lse, wabs, sabs
+        top = c["scales"][slots, hkv:].double().amax(0).repeat_interleave(hq // hkv) * TOP[c["codes"].dtype]
+        floor[b, :, 0] = len(slots) * top.cpu()
+    return o, lse, wabs, sabs, floor
 
 
 def check_decode(o, lse, ref, n_max):
     """Roundings: a score is a sum of 128 products and three factors (at most 131 * 2^-24 of sum|q k|); p carries the score's
-    error, one more of 2^-22 (ex2) and its rounding to 11 bits before the second product (2^-11); sums of n terms in fp32 lose at most n * 2^-24 of the sum of magnitudes; the output is rounded once."""
-    ro, rl, wabs, sabs = ref
+    error, one more of 2^-22 (ex2) and the rounding of p * v_scale to f16 before the second product (2^-11 relative; below f16's
+    normal range 2^-25 absolute of a number that is held as p * v_scale * 2^12 / v_ref with v_ref <= 4 * the largest v_scale, while
+    some p is 1 and so sum p >= 1: at most 2^-25 * 4 / 2^12 = 2^-35 of the largest v_scale * top code for each of n tokens); sums of
+    n terms in fp32 lose at most n * 2^-24 of the sum of magnitudes; the output is rounded once."""
+    ro, rl, wabs, sabs, floor = ref
     ds = 131 * U32 * sabs
     tol = ((2.0 ** -11 + 2.0 ** -20 + 2 * min(n_max, 4096) * U32) + 2 * ds)[..., None] * wabs
-    tol = tol + (half_step(o.dtype) if o.dtype != torch.float32 else U32) * ro.abs() * 1.01 + 1e-30
+    tol = tol + 2.0 ** -35 * floor + (half_step(o.dtype) if o.dtype != torch.float32 else U32) * ro.abs() * 1.01 + 1e-30
     if o.dtype == F16:
         tol = tol + 2.0 ** -25
     err = (o.double().cpu() - ro).abs()
