@@ -43,7 +43,7 @@ const char* esp_last_cuda_error(void);
 /* ABI version of this header (bumped on incompatible change).  Version 2: the peer-memory entry points take `value_base`.
  * Version 3: the kernels that dereference slot ids take the pool's row count; the self-test kernels left the library.
  * Version 4: esp_prefill_step_strided added (nothing removed or changed).
- * Version 5: the 8-bit entry points (esp_kv_*_q8, esp_decode_stage1_q8, esp_add_rms_norm*, esp_silu_and_mul_q8,
+ * Version 5: the 8-bit entry points (esp_kv_*_q8, esp_decode_*_q8, esp_add_rms_norm*, esp_silu_and_mul_q8,
  * esp_quantize_rows, esp_dequantize_rows, esp_mm_w8a8) added (nothing removed or changed). */
 #define ESP_ABI_VERSION 5
 int esp_abi_version(void);
@@ -430,6 +430,19 @@ int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q, const void
                          int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                          int32_t max_len_in_batch, int32_t seq_block_size, int32_t dtype, int32_t code,
                          float sm_scale, int64_t pool_rows, void* stream);
+
+/* Stage 1 and merge of a pool held in 8 bits in one call.  o [batch, Hq, D] (o_dtype F16/BF16/F32), lse fp32 [batch, Hq];
+ * workspace: ceil(max(max_len_in_batch, 1) / seq_block_size) * batch * Hq * (D + 1) floats, 16-byte aligned, used by this call
+ * alone until it has run (may be NULL when there is one split: the results are then written at once).  Other arguments as
+ * esp_decode_stage1_q8.  A request of length zero gets o = 0, lse = -inf. */
+int esp_decode_attention_q8(void* o, float* lse, float* workspace, const void* q, const void* k, const void* v,
+                            const float* k_scale, const float* v_scale, int64_t k_stride_t, int64_t k_stride_h,
+                            int64_t v_stride_t, int64_t v_stride_h, int64_t k_scale_stride_t,
+                            int64_t v_scale_stride_t, const int32_t* req_to_tokens, int64_t req_to_tokens_stride,
+                            int32_t req_rows, int32_t req_cols, const int32_t* b_req_idx,
+                            const int32_t* b_seqlen, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t max_len_in_batch, int32_t seq_block_size, int32_t dtype,
+                            int32_t o_dtype, int32_t code, float sm_scale, int64_t pool_rows, void* stream);
 
 /* t = in + residual; residual <- t rounded; out = t * rsqrt(mean(t^2) + eps) * weight, of the unrounded t.  Contiguous
  * [tokens, hidden], hidden a multiple of 8 and at most 65536; dtype F16/BF16; fp32 arithmetic. */

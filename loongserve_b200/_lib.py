@@ -79,6 +79,8 @@ ATTN_SIGNATURES = {
     "esp_kv_gather_q8": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _i64, _vp],
     "esp_decode_stage1_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _vp,
                              _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i64, _vp],
+    "esp_decode_attention_q8": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp,
+                                _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i64, _vp],
     "esp_add_rms_norm": [_vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _vp],
     "esp_add_rms_norm_q8": [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _vp],
     "esp_silu_and_mul_q8": [_vp, _vp, _vp, _i64, _i32, _i32, _vp],

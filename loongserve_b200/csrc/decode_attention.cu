@@ -549,14 +549,16 @@ extern "C" int esp_flag_wait(const int32_t* flag, int32_t value, const int32_t* 
     return ESP_OK;
 }
 
-namespace esp { int set_prefill_wait_limit(long long cycles); int set_mm_wait_limit(long long cycles); }
+namespace esp { int set_prefill_wait_limit(long long cycles); int set_mm_wait_limit(long long cycles); int set_decode_q8_wait_limit(long long cycles); }
 
 extern "C" int esp_set_wait_limit_cycles(int64_t cycles) {
     if (cycles <= 0) return ESP_ERR_BAD_ARG;
     const long long v = cycles;
     ESP_CUDA_TRY(cudaMemcpyToSymbol(g_gate_limit_cycles, &v, sizeof(v)));
     const int rc = set_prefill_wait_limit(v);
-    return rc ? rc : set_mm_wait_limit(v);
+    if (rc) return rc;
+    const int rc2 = set_mm_wait_limit(v);
+    return rc2 ? rc2 : set_decode_q8_wait_limit(v);
 }
 
 namespace esp { int decode_q8_status(int32_t out[4], int32_t clear); }

@@ -5,13 +5,13 @@
 // Bound by HBM: 2 * (128 + 4) bytes per token and kv head, each read once.  At that rate one SM has to take in a code every
 // 1/23 of a cycle and multiply it with up to 8 query heads, which is past what fp32 lanes do next to the conversion; so codes
 // become f16 (exactly: 8 bits fit) and the products run on the tensor cores (mma.sync m16n8k16, fp32 sums), which are far
-// from their limit here.  No shared memory and no shuffles of data: each lane loads 16-byte pieces straight from global
-// memory and its pieces ARE operand fragments, because the order of the summed index (head dims for S, tokens for O) is free:
+// from their limit here.  A lane reads 16-byte pieces of the rows and its pieces ARE operand fragments, because the order of
+// the summed index (head dims for S, tokens for O) is free:
 //   S [heads 16 x tokens 8] = Q K^T   B fragment of lane (g, c): token g, dims {16c..16c+15, 64+16c..64+16c+15}, one word of
 //                                     four codes per MMA; Q fragments are loaded once in the same dim order.
 //   O^T [dims 16 x heads 8] += V^T P^T  A fragment of lane (g, c): dims 16g..16g+15, tokens 2c, 2c+1, 2c+8, 2c+9 (words of two
 //                                     tokens interleaved byte by byte); P^T's fragment is what the lane holds of S.
-// (lane = 4g + c.)  A warp takes 16 tokens per step, the next step's loads are in flight meanwhile.
+// (lane = 4g + c.)  A warp takes 16 tokens of one head tile per step.
 //
 // Precision.  q is scaled by a power of two per head so that its largest element is near 2^7 in f16: exact down to 2^-21 of
 // it.  Scores, maxima, sums and outputs are fp32.  The weights p * v_scale are rounded to f16 (11 bits) before the second
@@ -41,7 +41,9 @@ struct DecodeQ8Args {
     const int32_t* req_to_tokens; int64_t rtt_stride; int rtt_rows, rtt_cols;
     const int32_t *b_req_idx, *b_seqlen;
     int batch, num_q_heads, num_kv_heads, group, seq_block_size;
-    float scale_log2; int64_t pool_rows; int head_tiles;
+    float scale_log2; int64_t pool_rows;
+    int head_tiles, head_groups, scale_vec;      // tiles of up to 8 q heads of one kv head; CTAs that cover them all for one split
+    void* o; float* lse; int o_dtype; // with one split only: the results themselves instead of partials (o != nullptr)
 };
 
 constexpr int kQ8Warps = 4, kQ8HeadTile = 8;
@@ -67,104 +69,167 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
     }
 }
 
-// A warp's steps (16 tokens of one kv head each) pass through a ring in shared memory, filled with 16-byte asynchronous copies.
-// Every lane reads back exactly the bytes it copied, so the ring is a register file that does not hold registers while the
-// copies are under way; only the scales and the mask of present tokens pass between lanes.
-constexpr int kQ8Stages = 4;
-struct StepQ8 {
-    uint4 kv[8][32];        // [piece][lane]: K tokens g, g + 8 x dims (16c.., 64 + 16c..), V tokens 2c, 2c + 1, 2c + 8, 2c + 9 x dims 16g..
-    float k_scale[16], v_scale[16];
+// A CTA covers NH neighbouring kv heads (or one group of 8 q heads of one kv head) and one split of the tokens: its four consumer
+// warps are NH heads x WT = 4 / NH interleaved shares of the split's tokens.  A fifth warp fetches, with 16-byte asynchronous
+// copies: one instruction takes the NH heads' K (or V) codes of WT tokens, 512 contiguous bytes for NH = 4, into a ring of
+// stages of 16 * WT tokens, counted on mbarriers.  Against fetches by the consumer warps themselves this takes address
+// arithmetic and slot lookups out of their instruction streams, and a scale's 32-byte sector is asked for once per CTA instead
+// of once per head.  (One bulk copy per token and operand instead: 81 cycles each from one warp, 3.3 TB/s at best.)  Row
+// pitches in shared memory are chosen so that the fragment reads (16 bytes per lane) have no bank conflicts: K rows an odd
+// multiple of 64 bytes apart, V rows an odd multiple of 16.
+template <int NH> struct RingQ8 {
+    static constexpr int WT = kQ8Warps / NH, kTokens = 16 * WT;
+    static constexpr int kPitchK = NH * 128 + 64, kPitchV = NH * 128 + 16;
+    static constexpr int kOffV = kTokens * kPitchK, kOffScale = kOffV + kTokens * kPitchV;      // scales [K, V][token][NH]
+    static constexpr int kOffPresent = kOffScale + 2 * kTokens * NH * 4;                        // WT masks of 16 tokens
+    static constexpr int kStageBytes = kOffPresent + 16;
+    static constexpr int kStages = NH == 4 ? 4 : 3;                                     // three CTAs to an SM
+    static constexpr int kOffBar = kStages * kStageBytes;                                       // full [kStages], empty [kStages]
+    static constexpr int kSmem = kOffBar + 2 * kStages * 8 + 16;
 };
-struct SmemQ8 {
-    StepQ8 ring[kQ8Warps][kQ8Stages];
-    uint32_t present[kQ8Warps][kQ8Stages];      // bit t: token t of the step exists
-};
-struct MergeQ8 {                                // over the ring, once it is used up
+struct MergeQ8 {                      // over the ring, once it is used up
     float o[kQ8Warps][kQ8HeadTile][132];
     float m[kQ8Warps][kQ8HeadTile], l[kQ8Warps][kQ8HeadTile], v[kQ8Warps];
 };
-static_assert(sizeof(MergeQ8) <= sizeof(SmemQ8), "the merge reuses the ring");
+static_assert(sizeof(MergeQ8) <= RingQ8<1>::kOffBar && sizeof(MergeQ8) <= RingQ8<4>::kOffBar, "the merge reuses the stages");
 
-// copies `bytes` (16 or, for a token that does not exist, 0: the rest is filled with zeros)
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+// copies 16 or 4 bytes, or fills them with zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(void* dst, const void* src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool have) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
+// one arrival (of the barrier's count) once this thread's asynchronous copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-template <typename T, int CODE>
-__global__ void __launch_bounds__(kQ8Warps * 32, 3) decode_stage1_q8_kernel(DecodeQ8Args a) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    SmemQ8& sm = *reinterpret_cast<SmemQ8*>(smem_raw);
-    // all kv heads of a split run next to each other: their rows and their scales (eight heads to a 32-byte sector) are neighbours
-    const int blk = blockIdx.x / a.head_tiles, ht = blockIdx.x - blk * a.head_tiles, b = blockIdx.y;
+// Limit of the mbarrier waits in SM cycles; on expiry {ESP_ERR_DEVICE_TIMEOUT, block, which (8 producer, 9 consumer), step} is
+// recorded, the CTA writes no results, and later launches return at once until the status has been read.
+__device__ long long g_decode_q8_wait_limit_cycles = 2000000000LL;
+__device__ __noinline__ void q8_timeout(int which, int step) {
+    int old = atomicCAS(&g_decode_q8_status[0], 0, ESP_ERR_DEVICE_TIMEOUT);
+    if (old == ESP_ERR_BAD_SLOT) old = atomicCAS(&g_decode_q8_status[0], ESP_ERR_BAD_SLOT, ESP_ERR_DEVICE_TIMEOUT) == ESP_ERR_BAD_SLOT ? 0 : 1;
+    if (old == 0) {                                  // results that are missing come before a token that was left out
+        g_decode_q8_status[1] = blockIdx.x + gridDim.x * blockIdx.y;
+        g_decode_q8_status[2] = which;
+        g_decode_q8_status[3] = step;
+    }
+}
+__device__ __forceinline__ bool q8_wait(uint32_t bar, uint32_t parity, volatile int* abort, int which, int step) {
+    const int r = ptx::mbar_wait_bounded(bar, parity, &g_decode_q8_wait_limit_cycles, abort);
+    if (r == 2) { q8_timeout(which, step); *abort = 1; }
+    return r == 0;
+}
+
+__device__ __forceinline__ void store_as(void* o, int64_t i, float x, int dtype) {
+    if (dtype == ESP_DTYPE_F32) reinterpret_cast<float*>(o)[i] = x;
+    else if (dtype == ESP_DTYPE_F16) reinterpret_cast<__half*>(o)[i] = __float2half_rn(x);
+    else reinterpret_cast<__nv_bfloat16*>(o)[i] = __float2bfloat16_rn(x);
+}
+
+template <typename T, int CODE, int NH>
+__global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel(DecodeQ8Args a) {
+    using R = RingQ8<NH>;
+    constexpr int WT = R::WT;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t sbase = ptx::smem_u32(smem);
+    auto full = [sbase](int st) { return sbase + R::kOffBar + 8u * st; };
+    auto empty = [sbase](int st) { return sbase + R::kOffBar + 8u * (R::kStages + st); };
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + R::kOffBar + 16 * R::kStages);
+    // all head groups of a split run next to each other: their rows are neighbours in memory
+    const int blk = blockIdx.x / a.head_groups, hg = blockIdx.x - blk * a.head_groups, b = blockIdx.y;
     const int len = a.b_seqlen[b];
+    const int req = a.b_req_idx[b];
     const int t0 = blk * a.seq_block_size;
     int t1 = min(t0 + a.seq_block_size, len);
-    if (t1 <= t0) return;
-    const int tiles_per_kv = (a.group + kQ8HeadTile - 1) / kQ8HeadTile;
-    const int kvh = ht / tiles_per_kv, hsub = ht - kvh * tiles_per_kv;
-    const int h0 = kvh * a.group + hsub * kQ8HeadTile;
-    const int nheads = min(kQ8HeadTile, a.group - hsub * kQ8HeadTile);
-    const int req = a.b_req_idx[b];
-    if (req < 0 || req >= a.rtt_rows || len > a.rtt_cols) {
+    if (t1 <= t0 && a.o == nullptr) return;              // as results, an empty request's zeros have to be written
+    if (t1 > t0 && (req < 0 || req >= a.rtt_rows || len > a.rtt_cols)) {
         if (threadIdx.x == 0) q8_report(1, req);
         t1 = t0;
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int steps = t1 > t0 ? (t1 - t0 + R::kTokens - 1) / R::kTokens : 0;
+    if (threadIdx.x == 0) {
+        *s_abort = *reinterpret_cast<volatile int*>(&g_decode_q8_status[0]) == ESP_ERR_DEVICE_TIMEOUT ? 1 : 0;
+        for (int i = 0; i < R::kStages; ++i) { ptx::mbar_init(full(i), 33); ptx::mbar_init(empty(i), kQ8Warps); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    // head tiles of this CTA: kv heads kv0 .. kv0 + NH - 1, or (a group of more than 8 q heads, NH = 1) tile `sub` of one
+    const int tiles_per_kv = (a.group + kQ8HeadTile - 1) / kQ8HeadTile;
+    const int kv0 = hg * NH / tiles_per_kv, sub = hg * NH - kv0 * tiles_per_kv;
+    const int nheads = min(kQ8HeadTile, a.group - sub * kQ8HeadTile);
 
-    // tokens [w0, w1) of this warp, whole groups of 32 except at the end
-    const int per_warp = ((t1 - t0 + kQ8Warps * 32 - 1) / (kQ8Warps * 32)) * 32;
-    const int w0 = min(t0 + warp * per_warp, t1), w1 = min(w0 + per_warp, t1);
-    const int32_t* rtt = a.req_to_tokens + (w1 > w0 ? (int64_t)req * a.rtt_stride : 0);
-    const uint8_t* kbase = a.k + (int64_t)kvh * a.k_stride_h + c * 16;
-    const uint8_t* vbase = a.v + (int64_t)kvh * a.v_stride_h + g * 16;
-    const float* sbase = lane < 16 ? a.k_scale + kvh : a.v_scale + kvh;
-    const int64_t s_stride = lane < 16 ? a.ks_stride_t : a.vs_stride_t;
-
-    // slots of 32 tokens, one per lane; -1: no such token
-    auto load_slots = [&](int t) -> int {
-        if (t + lane >= w1) return -1;
-        const int s = rtt[t + lane];
-        if (s < 0 || s >= a.pool_rows) { q8_report(0, s); return -1; }
-        return s;
-    };
-    // copies step `half` of the group of 32 tokens whose slots the lanes hold; a token that does not exist (its address would
-    // be that of slot 0, which is there) is filled with zeros
-    auto issue = [&](int stage, int group_slots, int half) {
-        StepQ8& d = sm.ring[warp][stage];
-        const int mine = __shfl_sync(0xffffffffu, group_slots, half * 16 + (lane & 15));
-        const uint32_t present = __ballot_sync(0xffffffffu, mine >= 0) & 0xffffu;
-        if (lane == 0) sm.present[warp][stage] = present;
+    if (warp == kQ8Warps) {
+        // ------------------------------------------------------------------ producer
+        const int tok = lane & 15, isv = lane >> 4;
+        const int32_t* rtt = a.req_to_tokens + (steps > 0 ? (int64_t)req * a.rtt_stride : 0);
+        const int piece = lane % (NH * 8), share = lane / (NH * 8);         // 16 bytes of a row; which of an instruction's WT tokens
+        const uint8_t* ksrc = a.k + (int64_t)kv0 * a.k_stride_h + piece * 16;
+        const uint8_t* vsrc = a.v + (int64_t)kv0 * a.v_stride_h + piece * 16;
+        const float* ssrc = isv ? a.v_scale + kv0 : a.k_scale + kv0;
+        const int64_t ssrc_stride = isv ? a.vs_stride_t : a.ks_stride_t;
+        // slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u; -1: no such token
+        auto load_slots = [&](int i, int u) -> int {
+            const int t = t0 + ((i + isv) * WT + u) * 16 + tok;
+            if (i + isv >= steps || t >= t1) return -1;
+            const int s = rtt[t];
+            if (s < 0 || s >= a.pool_rows) { q8_report(0, s); return -1; }
+            return s;
+        };
+        int slots[WT], slots_next[WT];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int s = __shfl_sync(0xffffffffu, mine, g + 8 * i);
-            const uint8_t* p = kbase + (int64_t)max(s, 0) * a.k_stride_t;
-            cp_async16(&d.kv[2 * i][lane], p, s >= 0 ? 16 : 0);
-            cp_async16(&d.kv[2 * i + 1][lane], p + 64, s >= 0 ? 16 : 0);
-        }
+        for (int u = 0; u < WT; ++u) { slots[u] = load_slots(0, u); slots_next[u] = load_slots(2, u); }
+        bool ok = !*s_abort;
+        int i = 0;
+        for (; i < steps && ok; ++i) {
+            const int st = i % R::kStages;
+            if (i >= R::kStages) {
+                ok = __all_sync(0xffffffffu, q8_wait(empty(st), ((i / R::kStages) - 1) & 1, s_abort, 8, i));
+                if (!ok) break;
+            }
+            const uint32_t stage = sbase + st * R::kStageBytes;
+            int s[WT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = __shfl_sync(0xffffffffu, mine, 2 * c + (i & 1) + 8 * (i >> 1));
-            cp_async16(&d.kv[4 + i][lane], vbase + (int64_t)max(s, 0) * a.v_stride_t, s >= 0 ? 16 : 0);
-        }
-        cp_async4(lane < 16 ? &d.k_scale[lane] : &d.v_scale[lane - 16], sbase + (int64_t)max(mine, 0) * s_stride, mine >= 0 ? 4 : 0);
-    };
-
-    // the next step to copy: step n_issue of the warp, from group n_issue / 2
-    const int steps = (w1 - w0 + 15) >> 4;
-    int n_issue = 0, slots = load_slots(w0), slots_next = load_slots(w0 + 32);
-    auto issue_next = [&](int stage) {
-        if (n_issue < steps) {
-            issue(stage, slots, n_issue & 1);
-            if (n_issue & 1) { slots = slots_next; slots_next = load_slots(w0 + (n_issue + 1) * 16 + 32); }
-            ++n_issue;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");             // an empty group keeps the count
-    };
+            for (int u = 0; u < WT; ++u) {
+                s[u] = __shfl_sync(0xffffffffu, slots[u], (i & 1) * 16 + tok);
+                const uint32_t present = __ballot_sync(0xffffffffu, s[u] >= 0) & 0xffffu;
+                if (lane == 0) *reinterpret_cast<uint32_t*>(smem + st * R::kStageBytes + R::kOffPresent + 4 * u) = present;
+            }
+            if (lane == 0) ptx::mbar_arrive(full(st));                // publishes the masks
 #pragma unroll
-    for (int i = 0; i < kQ8Stages - 1; ++i) issue_next(i);
+            for (int j = 0; j < 16; ++j) {                            // tokens j * WT + share; absent ones are filled with zeros
+                const int slot = __shfl_sync(0xffffffffu, s[j * WT / 16], j * WT % 16 + share);
+                const int64_t row = max(slot, 0);
+                const uint32_t at = j * WT + share;
+                cp_async16(stage + at * R::kPitchK + piece * 16, ksrc + row * a.k_stride_t, slot >= 0);
+                cp_async16(stage + R::kOffV + at * R::kPitchV + piece * 16, vsrc + row * a.v_stride_t, slot >= 0);
+            }
+#pragma unroll
+            for (int u = 0; u < WT; ++u) {                            // scales: lanes 0-15 K, lanes 16-31 V of 16 tokens
+                const uint32_t sd = stage + R::kOffScale + ((isv * R::kTokens + u * 16 + tok) * NH) * 4;
+                const float* sp = ssrc + (int64_t)max(s[u], 0) * ssrc_stride;
+                if (NH == 4 && a.scale_vec) cp_async16(sd, sp, s[u] >= 0);
+                else
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) cp_async4(sd + 4 * h, sp + h, s[u] >= 0);
+            }
+            cp_async_arrive(full(st));
+            if (i & 1) {
+#pragma unroll
+                for (int u = 0; u < WT; ++u) { slots[u] = slots_next[u]; slots_next[u] = load_slots(i + 3, u); }
+            }
+        }
+        if (!ok)                                                      // copies still under way: wait for them, bounded
+            for (int j = i > R::kStages ? i - R::kStages : 0; j < i; ++j)
+                ptx::mbar_wait_bounded(full(j % R::kStages), (j / R::kStages) & 1, &g_decode_q8_wait_limit_cycles, nullptr);
+    }
+    const int g = lane >> 2, c = lane & 3;
+    const int hw = warp % NH, wt = warp / NH;            // consumer warps: kv head within the CTA, share of its tokens
+    const int h0 = (kv0 + hw) * a.group + sub * kQ8HeadTile;
+    const bool consumer = warp < kQ8Warps;
 
     // Q fragments: row g is head g of the tile (rows 8-15 of the MMA stay zero), dims in the order of the K words
     uint32_t qf[8][2];
@@ -174,7 +239,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32, 3) decode_stage1_q8_kernel(Deco
         const T* qp = reinterpret_cast<const T*>(a.q) + ((int64_t)b * a.num_q_heads + h0 + g) * 128 + c * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 u = g < nheads ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
+            const uint4 u = consumer && g < nheads ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -201,11 +266,16 @@ __global__ void __launch_bounds__(kQ8Warps * 32, 3) decode_stage1_q8_kernel(Deco
     float m_ref = -INFINITY, l_run = 0.f; // of head g; l over this lane's tokens only
     float v_ref = 0.f, v_mul = 0.f;       // weights are held as p * v_scale * v_mul, v_mul = 2^12 / v_ref, v_ref >= every v_scale so far
 
-    auto compute = [&](const StepQ8& d, uint32_t present) {
+    auto compute = [&](const uint8_t* d) {
+        const uint8_t* krow = d + (wt * 16 + g) * R::kPitchK + hw * 128 + c * 16;
+        const uint8_t* vrow = d + R::kOffV + (wt * 16 + 2 * c) * R::kPitchV + hw * 128 + g * 16;
+        const float* scl = reinterpret_cast<const float*>(d + R::kOffScale) + wt * 16 * NH + hw;
+        const uint32_t present = *reinterpret_cast<const uint32_t*>(d + R::kOffPresent + 4 * wt);
         float s[2][4] = {};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint4 x = d.kv[2 * i][lane], y = d.kv[2 * i + 1][lane];
+            const uint4 x = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitchK);
+            const uint4 y = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitchK + 64);
             const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -216,11 +286,10 @@ __global__ void __launch_bounds__(kQ8Warps * 32, 3) decode_stage1_q8_kernel(Deco
         }
         float sc[4], vs[4];               // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float2 kf = *reinterpret_cast<const float2*>(&d.k_scale[2 * c + 8 * i]);
-            const float2 vf = *reinterpret_cast<const float2*>(&d.v_scale[2 * c + 8 * i]);
-            sc[2 * i] = s[i][0] * (kf.x * qs); sc[2 * i + 1] = s[i][1] * (kf.y * qs);
-            vs[2 * i] = vf.x; vs[2 * i + 1] = vf.y;
+        for (int i = 0; i < 4; ++i) {
+            const int t = 2 * c + (i & 1) + 8 * (i >> 1);
+            sc[i] = s[i >> 1][i & 1] * (scl[t * NH] * qs);
+            vs[i] = scl[(R::kTokens + t) * NH];
         }
         if (present != 0xffffu) {         // zeros were copied for the others: only their scores need a word
 #pragma unroll
@@ -259,7 +328,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32, 3) decode_stage1_q8_kernel(Deco
         const uint32_t b0 = Cvt<__half>::pack(wgt[0], wgt[1]), b1 = Cvt<__half>::pack(wgt[2], wgt[3]);
         uint32_t vw[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const uint4 x = d.kv[4 + i][lane]; vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w; }
+        for (int i = 0; i < 4; ++i) { const uint4 x = *reinterpret_cast<const uint4*>(vrow + ((i & 1) + 8 * (i >> 1)) * R::kPitchV); vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w; }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
 #pragma unroll
@@ -273,47 +342,118 @@ __global__ void __launch_bounds__(kQ8Warps * 32, 3) decode_stage1_q8_kernel(Deco
         }
     };
 
-    int stage = 0;
+    if (consumer) {
+        bool ok = !*s_abort;
 #pragma unroll 1
-    for (int i = 0; i < steps; ++i) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kQ8Stages - 2) : "memory");
-        __syncwarp();                     // the other lanes' scales and the mask are there; all have left the stage filled next
-        issue_next(stage == 0 ? kQ8Stages - 1 : stage - 1);
-        compute(sm.ring[warp][stage], sm.present[warp][stage]);
-        stage = stage + 1 == kQ8Stages ? 0 : stage + 1;
+        for (int i = 0, st = 0, phase = 0; i < steps && ok; ++i) {
+            ok = __all_sync(0xffffffffu, q8_wait(full(st), phase, s_abort, 9, i));
+            if (!ok) break;
+            compute(smem + st * R::kStageBytes);
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(empty(st));
+            if (++st == R::kStages) { st = 0; phase ^= 1; }
+        }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
+    if (*s_abort) return;
 
-    // the four warps' states: heads of this tile, in units of each warp's own reference
-    MergeQ8& mg = *reinterpret_cast<MergeQ8*>(smem_raw);
+    // the warps' states: heads of their tiles, in units of each warp's own reference
+    MergeQ8& mg = *reinterpret_cast<MergeQ8*>(smem);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    if (c == 0) { mg.m[warp][g] = m_ref; mg.l[warp][g] = l_run; }
-    if (lane == 0) mg.v[warp] = v_ref * (1.f / 4096.f);
+    if (consumer) {
+        if (c == 0) { mg.m[warp][g] = m_ref; mg.l[warp][g] = l_run; }
+        if (lane == 0) mg.v[warp] = v_ref * (1.f / 4096.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        *reinterpret_cast<float2*>(&mg.o[warp][2 * c][16 * g + 2 * j]) = make_float2(acc[j][0], acc[j][2]);
-        *reinterpret_cast<float2*>(&mg.o[warp][2 * c + 1][16 * g + 2 * j]) = make_float2(acc[j][1], acc[j][3]);
+        for (int j = 0; j < 8; ++j) {
+            *reinterpret_cast<float2*>(&mg.o[warp][2 * c][16 * g + 2 * j]) = make_float2(acc[j][0], acc[j][2]);
+            *reinterpret_cast<float2*>(&mg.o[warp][2 * c + 1][16 * g + 2 * j]) = make_float2(acc[j][1], acc[j][3]);
+        }
     }
     __syncthreads();
+    if (!consumer) return;
     const int d = threadIdx.x;
-    for (int h = 0; h < nheads; ++h) {
-        float M = -INFINITY;
+#pragma unroll 1
+    for (int i = 0; i < NH; ++i) {
+        const int first = (kv0 + i) * a.group + sub * kQ8HeadTile;
+        for (int h = 0; h < nheads; ++h) {
+            float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kQ8Warps; ++w) M = fmaxf(M, mg.m[w][h]);
-        const float Mu = M == -INFINITY ? 0.f : M;
-        float L = 0.f, o = 0.f;
+            for (int w = 0; w < WT; ++w) M = fmaxf(M, mg.m[w * NH + i][h]);
+            const float Mu = M == -INFINITY ? 0.f : M;
+            float L = 0.f, o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kQ8Warps; ++w) {
-            const float f = exp2f(mg.m[w][h] - Mu);             // 0 for a warp that saw no token
-            L += mg.l[w][h] * f;
-            o += mg.o[w][h][d] * (f * mg.v[w]);
+            for (int w = 0; w < WT; ++w) {
+                const float f = exp2f(mg.m[w * NH + i][h] - Mu);          // 0 for a warp that saw no token
+                L += mg.l[w * NH + i][h] * f;
+                o += mg.o[w * NH + i][h][d] * (f * mg.v[w * NH + i]);
+            }
+            o = L == 0.f ? 0.f : o / L;
+            const float lse = L == 0.f ? -INFINITY : (Mu + log2f(L)) * kLn2Q8;
+            if (a.o != nullptr) {
+                const int64_t row = (int64_t)b * a.num_q_heads + first + h;
+                store_as(a.o, row * 128 + d, o, a.o_dtype);
+                if (d == 0) a.lse[row] = lse;
+            } else {
+                const int64_t row = ((int64_t)blk * a.batch + b) * a.num_q_heads + first + h;
+                a.mid_o[row * 128 + d] = o;
+                if (d == 0) a.mid_lse[row] = lse;
+            }
         }
-        const int64_t row = ((int64_t)blk * a.batch + b) * a.num_q_heads + h0 + h;
-        a.mid_o[row * 128 + d] = L == 0.f ? 0.f : o / L;
-        if (d == 0) a.mid_lse[row] = L == 0.f ? -INFINITY : (Mu + log2f(L)) * kLn2Q8;
     }
+}
+
+// The partials of one (request, head), by a CTA: at few rows and many splits (two requests of 262144 tokens: 64 rows x 256 splits)
+// one warp per row leaves most of the GPU idle.  Warp w takes splits w, w + 4, ...; lanes hold four dims each.
+__global__ void __launch_bounds__(128) decode_merge_q8_kernel(void* o, float* __restrict__ lse, const int32_t* __restrict__ b_seqlen,
+                                                              const float* __restrict__ mid_o, const float* __restrict__ mid_lse, int batch,
+                                                              int num_heads, int num_blocks, int block_seq, int o_dtype) {
+    const int pair = blockIdx.x, b = pair / num_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int len = b_seqlen[b];
+    const int n = len <= 0 ? 0 : min((len - 1) / block_seq + 1, num_blocks);
+    const int64_t bh = (int64_t)batch * num_heads;
+    __shared__ float s_m[4], s_l[4], s_o[4][128];
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = warp; j0 < n; j0 += 4 * 32) {                // up to 32 splits of this warp at a time, one lse per lane
+        const int j = j0 + 4 * lane;
+        const float x = j < n ? mid_lse[j * bh + pair] : -INFINITY;
+        float mx = x;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float m_new = fmaxf(m, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float al = exp2f((m - m_use) * kLog2eQ8), w = exp2f((x - m_use) * kLog2eQ8);
+        l = l * al + w;                                        // this lane's share of the sum
+        acc.x *= al; acc.y *= al; acc.z *= al; acc.w *= al;
+        m = m_new;
+        const int cnt = min(32, (n - j0 + 3) / 4);
+#pragma unroll 8
+        for (int i = 0; i < cnt; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float4 v = *reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + 4 * i) * bh + pair) * 128 + lane * 4);
+            acc.x = fmaf(wi, v.x, acc.x); acc.y = fmaf(wi, v.y, acc.y); acc.z = fmaf(wi, v.z, acc.z); acc.w = fmaf(wi, v.w, acc.w);
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+    *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), Mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = exp2f((s_m[w] - Mu) * kLog2eQ8);
+        L += s_l[w] * f;
+        x += s_o[w][threadIdx.x] * f;
+    }
+    store_as(o, (int64_t)pair * 128 + threadIdx.x, L == 0.f ? 0.f : x / L, o_dtype);
+    if (threadIdx.x == 0) lse[pair] = L == 0.f ? -INFINITY : Mu + log2f(L) * kLn2Q8;
+}
+
+int set_decode_q8_wait_limit(long long cycles) {
+    ESP_CUDA_TRY(cudaMemcpyToSymbol(g_decode_q8_wait_limit_cycles, &cycles, sizeof(cycles)));
+    return ESP_OK;
 }
 
 int decode_q8_status(int32_t out[4], int32_t clear) {
@@ -329,6 +469,54 @@ int decode_q8_status(int32_t out[4], int32_t clear) {
 
 using namespace esp;
 
+namespace esp {
+
+template <typename T, int CODE>
+static int launch_stage1_q8(DecodeQ8Args& a, int64_t nblk, cudaStream_t s) {
+    // neighbouring kv heads to a CTA, four or two where they divide evenly and lie next to each other; else one, whose tokens the
+    // four warps share
+    const bool dense = a.group <= kQ8HeadTile && a.k_stride_h == 128 && a.v_stride_h == 128;
+    const int nh = dense && a.head_tiles % 4 == 0 ? 4 : (dense && a.head_tiles % 2 == 0 ? 2 : 1);
+    a.head_groups = a.head_tiles / nh;
+    a.scale_vec = aligned16(a.k_scale) && aligned16(a.v_scale) && a.ks_stride_t % 4 == 0 && a.vs_stride_t % 4 == 0;
+    if (nblk * a.head_groups > 2147483647LL) return ESP_ERR_TOO_LARGE;
+    const dim3 grid((unsigned)(nblk * a.head_groups), a.batch);
+#define ESP_S1Q(NH)                                                                                                               \
+    {                                                                                                                            \
+        ESP_CUDA_TRY(cudaFuncSetAttribute(decode_stage1_q8_kernel<T, CODE, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, RingQ8<NH>::kSmem)); \
+        decode_stage1_q8_kernel<T, CODE, NH><<<grid, kQ8Warps * 32 + 32, RingQ8<NH>::kSmem, s>>>(a);                                              \
+    }
+    if (nh == 4) ESP_S1Q(4) else if (nh == 2) ESP_S1Q(2) else ESP_S1Q(1)
+#undef ESP_S1Q
+    ESP_LAUNCH_CHECK("decode_stage1_q8_kernel");
+    return ESP_OK;
+}
+
+static int stage1_q8(DecodeQ8Args& a, int head_dim, int max_len, int dtype, int code, float sm_scale, cudaStream_t s) {
+    if (!a.q || !a.k || !a.v || !a.k_scale || !a.v_scale || !a.req_to_tokens || !a.b_req_idx || !a.b_seqlen || a.batch < 0 ||
+        a.num_q_heads <= 0 || a.num_kv_heads <= 0 || a.num_q_heads % a.num_kv_heads || a.seq_block_size <= 0 || a.rtt_rows <= 0 ||
+        a.rtt_cols <= 0 || a.pool_rows <= 0)
+        return ESP_ERR_BAD_ARG;
+    if (dtype != ESP_DTYPE_F16 && dtype != ESP_DTYPE_BF16) return ESP_ERR_BAD_ARG;
+    if (code != ESP_CODE_INT8 && code != ESP_CODE_E4M3) return ESP_ERR_BAD_ARG;
+    if (head_dim != 128) return ESP_ERR_UNSUPPORTED;
+    if (a.batch > 65535 || a.num_q_heads > 65535) return ESP_ERR_TOO_LARGE;
+    if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || a.k_stride_t % 16 || a.k_stride_h % 16 || a.v_stride_t % 16 ||
+        a.v_stride_h % 16 || ((uintptr_t)a.k_scale & 3u) || ((uintptr_t)a.v_scale & 3u))
+        return ESP_ERR_ALIGNMENT;
+    const int64_t nblk = (max_len + (int64_t)a.seq_block_size - 1) / a.seq_block_size;
+    if (nblk * a.seq_block_size > 2147483647LL - 65536) return ESP_ERR_TOO_LARGE;
+    a.group = a.num_q_heads / a.num_kv_heads;
+    a.head_tiles = a.num_kv_heads * ((a.group + kQ8HeadTile - 1) / kQ8HeadTile);
+    a.scale_log2 = (sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)head_dim)) * kLog2eQ8;
+    if (dtype == ESP_DTYPE_F16)
+        return code == ESP_CODE_INT8 ? launch_stage1_q8<__half, ESP_CODE_INT8>(a, nblk, s) : launch_stage1_q8<__half, ESP_CODE_E4M3>(a, nblk, s);
+    return code == ESP_CODE_INT8 ? launch_stage1_q8<__nv_bfloat16, ESP_CODE_INT8>(a, nblk, s)
+                                 : launch_stage1_q8<__nv_bfloat16, ESP_CODE_E4M3>(a, nblk, s);
+}
+
+}  // namespace esp
+
 extern "C" int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q, const void* k, const void* v, const float* k_scale,
                                     const float* v_scale, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
                                     int64_t k_scale_stride_t, int64_t v_scale_stride_t, const int32_t* req_to_tokens,
@@ -337,37 +525,37 @@ extern "C" int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q,
                                     int32_t max_len_in_batch, int32_t seq_block_size, int32_t dtype, int32_t code, float sm_scale,
                                     int64_t pool_rows, void* stream) {
     if (batch == 0 || max_len_in_batch <= 0) return ESP_OK;
-    if (!mid_o || !mid_lse || !q || !k || !v || !k_scale || !v_scale || !req_to_tokens || !b_req_idx || !b_seqlen || batch < 0 ||
-        num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || seq_block_size <= 0 || req_rows <= 0 || req_cols <= 0 ||
-        pool_rows <= 0)
-        return ESP_ERR_BAD_ARG;
-    if (dtype != ESP_DTYPE_F16 && dtype != ESP_DTYPE_BF16) return ESP_ERR_BAD_ARG;
-    if (code != ESP_CODE_INT8 && code != ESP_CODE_E4M3) return ESP_ERR_BAD_ARG;
-    if (head_dim != 128) return ESP_ERR_UNSUPPORTED;
-    if (batch > 65535 || num_q_heads > 65535) return ESP_ERR_TOO_LARGE;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || k_stride_t % 16 || k_stride_h % 16 || v_stride_t % 16 || v_stride_h % 16 ||
-        ((uintptr_t)k_scale & 3u) || ((uintptr_t)v_scale & 3u))
-        return ESP_ERR_ALIGNMENT;
+    if (!mid_o || !mid_lse) return ESP_ERR_BAD_ARG;
     DecodeQ8Args a{mid_o, mid_lse, q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h,
                    k_scale_stride_t, v_scale_stride_t, req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch,
-                   num_q_heads, num_kv_heads, num_q_heads / num_kv_heads, seq_block_size,
-                   (sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)head_dim)) * kLog2eQ8, pool_rows, 0};
-    a.head_tiles = num_kv_heads * ((a.group + kQ8HeadTile - 1) / kQ8HeadTile);
-    const int64_t nblk = (max_len_in_batch + (int64_t)seq_block_size - 1) / seq_block_size;
-    if (nblk * a.head_tiles > 2147483647LL || nblk * seq_block_size > 2147483647LL) return ESP_ERR_TOO_LARGE;
-    const dim3 grid((unsigned)(nblk * a.head_tiles), batch);
+                   num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0, nullptr, nullptr, 0};
+    return stage1_q8(a, head_dim, max_len_in_batch, dtype, code, sm_scale, (cudaStream_t)stream);
+}
+
+extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, const void* q, const void* k, const void* v,
+                                       const float* k_scale, const float* v_scale, int64_t k_stride_t, int64_t k_stride_h,
+                                       int64_t v_stride_t, int64_t v_stride_h, int64_t k_scale_stride_t, int64_t v_scale_stride_t,
+                                       const int32_t* req_to_tokens, int64_t req_to_tokens_stride, int32_t req_rows, int32_t req_cols,
+                                       const int32_t* b_req_idx, const int32_t* b_seqlen, int32_t batch, int32_t num_q_heads,
+                                       int32_t num_kv_heads, int32_t head_dim, int32_t max_len_in_batch, int32_t seq_block_size,
+                                       int32_t dtype, int32_t o_dtype, int32_t code, float sm_scale, int64_t pool_rows, void* stream) {
+    if (batch == 0) return ESP_OK;
+    if (!o || !lse || max_len_in_batch < 0 || seq_block_size <= 0) return ESP_ERR_BAD_ARG;
+    if (o_dtype != ESP_DTYPE_F16 && o_dtype != ESP_DTYPE_BF16 && o_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
+    const int32_t max_len = max_len_in_batch > 0 ? max_len_in_batch : 1;
+    const int64_t nblk = (max_len + (int64_t)seq_block_size - 1) / seq_block_size;
+    if (nblk > 1 && !workspace) return ESP_ERR_BAD_ARG;
+    if (nblk > 1 && !aligned16(workspace)) return ESP_ERR_ALIGNMENT;
+    const int64_t rows = nblk * batch * num_q_heads;
+    DecodeQ8Args a{workspace, workspace + rows * 128, q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, k_stride_t, k_stride_h,
+                   v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t, req_to_tokens, req_to_tokens_stride, req_rows, req_cols,
+                   b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0,
+                   nblk == 1 ? o : nullptr, nblk == 1 ? lse : nullptr, o_dtype};
     cudaStream_t s = (cudaStream_t)stream;
-#define ESP_S1Q(T, C)                                                                                                             \
-    {                                                                                                                            \
-        ESP_CUDA_TRY(cudaFuncSetAttribute(decode_stage1_q8_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmemQ8))); \
-        decode_stage1_q8_kernel<T, C><<<grid, kQ8Warps * 32, sizeof(SmemQ8), s>>>(a);                                              \
-    }
-    if (dtype == ESP_DTYPE_F16) {
-        if (code == ESP_CODE_INT8) ESP_S1Q(__half, ESP_CODE_INT8) else ESP_S1Q(__half, ESP_CODE_E4M3)
-    } else {
-        if (code == ESP_CODE_INT8) ESP_S1Q(__nv_bfloat16, ESP_CODE_INT8) else ESP_S1Q(__nv_bfloat16, ESP_CODE_E4M3)
-    }
-#undef ESP_S1Q
-    ESP_LAUNCH_CHECK("decode_stage1_q8_kernel");
+    const int rc = stage1_q8(a, head_dim, max_len, dtype, code, sm_scale, s);
+    if (rc || nblk == 1) return rc;
+    decode_merge_q8_kernel<<<(unsigned)((int64_t)batch * num_q_heads), 128, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, batch, num_q_heads,
+                                                                                  (int)nblk, seq_block_size, o_dtype);
+    ESP_LAUNCH_CHECK("decode_merge_q8_kernel");
     return ESP_OK;
 }

@@ -45,24 +45,27 @@ def flash_decoding_stage2(o, out_logexpsum, b_seqlen, mid_o, mid_o_logexpsum, bl
     _lib.check(rc, "esp_decode_merge")
 
 
+def _q8_args(q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen):
+    assert q.dim() == 3 and q.is_contiguous() and k.dim() == 3 and v.dim() == 3 and k.stride(2) == 1 and v.stride(2) == 1
+    assert k.shape[1:] == v.shape[1:] and k.shape[2] == q.shape[2] and k_scale.shape == k.shape[:2] and v_scale.shape == v.shape[:2]
+    assert k.shape[1] == 1 or (k_scale.stride(1) == 1 and v_scale.stride(1) == 1)
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or v.dtype != k.dtype or req_to_tokens.dtype != torch.int32:
+        raise TypeError("k and v hold codes of one type, their scales are fp32, req_to_tokens is int32")
+    assert req_to_tokens.dim() == 2 and req_to_tokens.stride(1) == 1
+    need_i32(b_req_idx, b_seqlen)
+    assert b_req_idx.shape[0] == q.shape[0] and b_seqlen.shape[0] == q.shape[0]
+
+
 @torch.inference_mode()
 def flash_decoding_stage1_q8(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen,
                              max_len_in_batch: int, seq_block_size: int, sm_scale: float = 0.0):
     """``flash_decoding_stage1`` over a pool held in 8 bits: k, v int8 or e4m3 codes [slots, Hkv, 128], k_scale, v_scale fp32
     [slots, Hkv].  The partials go to ``flash_decoding_stage2`` unchanged."""
     need_here(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen)
-    assert mid_o.is_contiguous() and mid_o_logexpsum.is_contiguous() and q.is_contiguous()
-    assert q.dim() == 3 and k.dim() == 3 and v.dim() == 3 and k.stride(2) == 1 and v.stride(2) == 1
+    _q8_args(q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen)
+    assert mid_o.is_contiguous() and mid_o_logexpsum.is_contiguous()
     assert mid_o.dim() == 4 and mid_o_logexpsum.dim() == 3 and mid_o.dtype == mid_o_logexpsum.dtype == torch.float32
-    assert k.shape[1:] == v.shape[1:] and k.shape[2] == q.shape[2] and k_scale.shape == k.shape[:2] and v_scale.shape == v.shape[:2]
-    hkv = k.shape[1]
-    assert hkv == 1 or (k_scale.stride(1) == 1 and v_scale.stride(1) == 1)
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or v.dtype != k.dtype or req_to_tokens.dtype != torch.int32:
-        raise TypeError("k and v hold codes of one type, their scales are fp32, req_to_tokens is int32")
-    assert req_to_tokens.dim() == 2 and req_to_tokens.stride(1) == 1
-    need_i32(b_req_idx, b_seqlen)
     batch, hq, dim = q.shape
-    assert b_req_idx.shape[0] == batch and b_seqlen.shape[0] == batch
     nblk = (int(max_len_in_batch) + int(seq_block_size) - 1) // int(seq_block_size)
     assert mid_o.shape[0] >= nblk and mid_o.shape[1:] == q.shape
     assert mid_o_logexpsum.shape[0] >= nblk and mid_o_logexpsum.shape[1:] == q.shape[:2]
@@ -70,14 +73,15 @@ def flash_decoding_stage1_q8(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, 
         mid_o.data_ptr(), mid_o_logexpsum.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_scale.stride(0), v_scale.stride(0), req_to_tokens.data_ptr(),
         req_to_tokens.stride(0), req_to_tokens.shape[0], req_to_tokens.shape[1], b_req_idx.data_ptr(), b_seqlen.data_ptr(), batch, hq,
-        hkv, dim, int(max_len_in_batch), int(seq_block_size), dtype16_tag(q), code_tag(k), float(sm_scale),
+        k.shape[1], dim, int(max_len_in_batch), int(seq_block_size), dtype16_tag(q), code_tag(k), float(sm_scale),
         min(k.shape[0], v.shape[0]), stream_ptr())
     _lib.check(rc, "esp_decode_stage1_q8")
 
 
 def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -> int:
     """Tokens per split: enough CTAs to fill the GPU several times over when rows are few, not below 128 tokens."""
-    ctas = max(1, batch * kv_heads * ((group + 7) // 8))
+    tiles = kv_heads * ((group + 7) // 8)
+    ctas = max(1, batch * (tiles // 4 if tiles % 4 == 0 else tiles // 2 if tiles % 2 == 0 else tiles))
     splits = max(1, (148 * 12 + ctas - 1) // ctas)
     return min(1024, max(128, -(-max(int(max_len_in_batch), 1) // splits // 128) * 128))
 
@@ -85,24 +89,27 @@ def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -
 @torch.inference_mode()
 def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len,
                               max_len_in_batch: int, block_seq=None, out=None, out_logexpsum=None, sm_scale: float = 0.0):
-    """Decode attention over a pool held in 8 bits, stage 1 + stage 2: (o like q unless ``out`` is given, lse fp32).
+    """Decode attention over a pool held in 8 bits, splits and merge in one call: (o like q unless ``out`` is given, lse fp32).
     ``block_seq``: tokens per split, chosen from the sizes by default.  A request of length zero gets o = 0, lse = -inf."""
+    need_here(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len, out, out_logexpsum)
+    _q8_args(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len)
     batch, hq, dim = q.shape
+    hkv = cache_k.shape[1]
     o = torch.empty_like(q) if out is None else out
     lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device) if out_logexpsum is None else out_logexpsum
     assert o.shape == q.shape and o.is_contiguous() and lse.shape == (batch, hq) and lse.is_contiguous()
     if lse.dtype != torch.float32:
         raise TypeError("out_logexpsum is fp32")
-    dtype_tag(o)
-    if block_seq is None:
-        block_seq = q8_block_seq(batch, cache_k.shape[1], hq // max(1, cache_k.shape[1]), max_len_in_batch)
-    nblk = max(1, (int(max_len_in_batch) + block_seq - 1) // block_seq)
-    mid = torch.empty(nblk * batch * hq * (dim + 1), dtype=torch.float32, device=q.device)
-    cut = nblk * batch * hq * dim
-    mid_o, mid_lse = mid[:cut].view(nblk, batch, hq, dim), mid[cut:].view(nblk, batch, hq)
-    flash_decoding_stage1_q8(mid_o, mid_lse, q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len,
-                             max_len_in_batch, block_seq, sm_scale)
-    flash_decoding_stage2(o, lse, b_seq_len, mid_o, mid_lse, block_seq)
+    block = q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len_in_batch) if block_seq is None else int(block_seq)
+    nblk = (int(max_len_in_batch) + block - 1) // block
+    work = torch.empty(nblk * batch * hq * (dim + 1), dtype=torch.float32, device=q.device) if nblk > 1 else None
+    rc = _lib.attn().esp_decode_attention_q8(
+        o.data_ptr(), lse.data_ptr(), ptr(work), q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), cache_k.stride(0), cache_k.stride(1), cache_v.stride(0), cache_v.stride(1), k_scale.stride(0),
+        v_scale.stride(0), req_to_token_indexs.data_ptr(), req_to_token_indexs.stride(0), req_to_token_indexs.shape[0],
+        req_to_token_indexs.shape[1], b_req_idx.data_ptr(), b_seq_len.data_ptr(), batch, hq, hkv, dim, int(max_len_in_batch), block,
+        dtype16_tag(q), dtype_tag(o), code_tag(cache_k), float(sm_scale), min(cache_k.shape[0], cache_v.shape[0]), stream_ptr())
+    _lib.check(rc, "esp_decode_attention_q8")
     return o, lse
 
 
