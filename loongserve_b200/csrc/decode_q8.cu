@@ -42,6 +42,7 @@ struct DecodeQ8Args {
     const int32_t *b_req_idx, *b_seqlen;
     int batch, num_q_heads, num_kv_heads, group, seq_block_size;
     float scale_log2; int64_t pool_rows;
+    int num_blocks, compact;
     int head_tiles, head_groups, scale_vec;      // tiles of up to 8 q heads of one kv head; CTAs that cover them all for one split
     void* o; float* lse; int o_dtype; // with one split only: the results themselves instead of partials (o != nullptr)
 };
@@ -77,21 +78,28 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 // of once per head.  (One bulk copy per token and operand instead: 81 cycles each from one warp, 3.3 TB/s at best.)  Row
 // pitches in shared memory are chosen so that the fragment reads (16 bytes per lane) have no bank conflicts: K rows an odd
 // multiple of 64 bytes apart, V rows an odd multiple of 16.
+//
+// CTAs are persistent: each walks over (split, request, heads) items, and the producer runs ahead into the next item, so that
+// neither the start of an item (length, slots, queries) nor its results stop the flow of copies.  Where a CTA has several items
+// and the batch is small enough, the splits that exist are counted first (a prefix sum over the lengths), so that ragged
+// batches divide evenly.
+constexpr int kQ8MaxCompact = 256;        // requests whose lengths are held in shared memory
+struct WarpStateQ8 { float acc[32][32], m[32], l[32], v[32]; };      // [register][lane]
 template <int NH> struct RingQ8 {
     static constexpr int WT = kQ8Warps / NH, kTokens = 16 * WT;
     static constexpr int kPitchK = NH * 128 + 64, kPitchV = NH * 128 + 16;
     static constexpr int kOffV = kTokens * kPitchK, kOffScale = kOffV + kTokens * kPitchV;      // scales [K, V][token][NH]
     static constexpr int kOffPresent = kOffScale + 2 * kTokens * NH * 4;                        // WT masks of 16 tokens
     static constexpr int kStageBytes = kOffPresent + 16;
-    static constexpr int kStages = NH == 4 ? 4 : 3;                                     // three CTAs to an SM
+    static constexpr int kStages = NH == 4 ? 4 : (NH == 2 ? 3 : 2);
     static constexpr int kOffBar = kStages * kStageBytes;                                       // full [kStages], empty [kStages]
-    static constexpr int kSmem = kOffBar + 2 * kStages * 8 + 16;
+    static constexpr int kOffAbort = kOffBar + 2 * kStages * 8;
+    static constexpr int kOffMerge = kOffAbort + 16;                                            // states of the warps with wt > 0
+    static constexpr int kOffLen = kOffMerge + (WT - 1) * NH * (int)sizeof(WarpStateQ8);        // lengths, first blocks
+    static constexpr int kSmem = kOffLen + (2 * kQ8MaxCompact + 1) * 4;
 };
-struct MergeQ8 {                      // over the ring, once it is used up
-    float o[kQ8Warps][kQ8HeadTile][132];
-    float m[kQ8Warps][kQ8HeadTile], l[kQ8Warps][kQ8HeadTile], v[kQ8Warps];
-};
-static_assert(sizeof(MergeQ8) <= RingQ8<1>::kOffBar && sizeof(MergeQ8) <= RingQ8<4>::kOffBar, "the merge reuses the stages");
+static_assert(3 * (RingQ8<4>::kSmem + 1024) <= 233472 && 3 * (RingQ8<2>::kSmem + 1024) <= 233472 && 3 * (RingQ8<1>::kSmem + 1024) <= 233472,
+              "three CTAs to an SM");
 
 // copies 16 or 4 bytes, or fills them with zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool have) {
@@ -129,6 +137,27 @@ __device__ __forceinline__ void store_as(void* o, int64_t i, float x, int dtype)
     else reinterpret_cast<__nv_bfloat16*>(o)[i] = __float2bfloat16_rn(x);
 }
 
+// 16 values of an output row
+__device__ __forceinline__ void store_row16(void* o, int64_t i, const float (&x)[16], int dtype) {
+    if (dtype == ESP_DTYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(reinterpret_cast<float*>(o) + i)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+        return;
+    }
+    uint32_t u[8];
+    if (dtype == ESP_DTYPE_F16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = Cvt<__half>::pack(x[2 * j], x[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = Cvt<__nv_bfloat16>::pack(x[2 * j], x[2 * j + 1]);
+    }
+    uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(o) + i);
+    p[0] = make_uint4(u[0], u[1], u[2], u[3]); p[1] = make_uint4(u[4], u[5], u[6], u[7]);
+}
+
+struct ItemQ8 { int b, blk, hg, t0, t1, req, steps; bool write; };
+
 template <typename T, int CODE, int NH>
 __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel(DecodeQ8Args a) {
     using R = RingQ8<NH>;
@@ -137,59 +166,98 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     const uint32_t sbase = ptx::smem_u32(smem);
     auto full = [sbase](int st) { return sbase + R::kOffBar + 8u * st; };
     auto empty = [sbase](int st) { return sbase + R::kOffBar + 8u * (R::kStages + st); };
-    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + R::kOffBar + 16 * R::kStages);
-    // all head groups of a split run next to each other: their rows are neighbours in memory
-    const int blk = blockIdx.x / a.head_groups, hg = blockIdx.x - blk * a.head_groups, b = blockIdx.y;
-    const int len = a.b_seqlen[b];
-    const int req = a.b_req_idx[b];
-    const int t0 = blk * a.seq_block_size;
-    int t1 = min(t0 + a.seq_block_size, len);
-    if (t1 <= t0 && a.o == nullptr) return;              // as results, an empty request's zeros have to be written
-    if (t1 > t0 && (req < 0 || req >= a.rtt_rows || len > a.rtt_cols)) {
-        if (threadIdx.x == 0) q8_report(1, req);
-        t1 = t0;
-    }
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + R::kOffAbort);
+    int* s_len = reinterpret_cast<int*>(smem + R::kOffLen);               // -1: the request's row is not in the table
+    int* s_first = s_len + kQ8MaxCompact;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int steps = t1 > t0 ? (t1 - t0 + R::kTokens - 1) / R::kTokens : 0;
+    const bool direct = a.o != nullptr;                                   // one split: results, also of empty requests
     if (threadIdx.x == 0) {
         *s_abort = *reinterpret_cast<volatile int*>(&g_decode_q8_status[0]) == ESP_ERR_DEVICE_TIMEOUT ? 1 : 0;
         for (int i = 0; i < R::kStages; ++i) { ptx::mbar_init(full(i), 33); ptx::mbar_init(empty(i), kQ8Warps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    auto blocks_of = [&](int len) { return len <= 0 ? 0 : min((len - 1) / a.seq_block_size + 1, a.num_blocks); };
+    if (a.compact) {
+        for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+            const int len = a.b_seqlen[b], req = a.b_req_idx[b];
+            const bool ok = req >= 0 && req < a.rtt_rows && len <= a.rtt_cols;
+            if (!ok && len > 0) q8_report(1, req);
+            s_len[b] = ok ? len : -1;
+            s_first[b + 1] = blocks_of(len);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int carry = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 32) {
+                int x = b0 + lane < a.batch ? s_first[b0 + lane + 1] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+                if (b0 + lane < a.batch) s_first[b0 + lane + 1] = carry + x;
+                carry += __shfl_sync(0xffffffffu, x, 31);
+            }
+            if (lane == 0) s_first[0] = 0;
+        }
+    }
     __syncthreads();
-    // head tiles of this CTA: kv heads kv0 .. kv0 + NH - 1, or (a group of more than 8 q heads, NH = 1) tile `sub` of one
-    const int tiles_per_kv = (a.group + kQ8HeadTile - 1) / kQ8HeadTile;
-    const int kv0 = hg * NH / tiles_per_kv, sub = hg * NH - kv0 * tiles_per_kv;
-    const int nheads = min(kQ8HeadTile, a.group - sub * kQ8HeadTile);
+    const int items = (a.compact ? s_first[a.batch] : a.num_blocks * a.batch) * a.head_groups;
+    // all head groups of a split are neighbouring items: their rows are neighbours in memory
+    auto item_at = [&](int n) -> ItemQ8 {
+        ItemQ8 it;
+        const int bi = n / a.head_groups;
+        it.hg = n - bi * a.head_groups;
+        int len;
+        if (a.compact) {
+            int lo = 0, hi = a.batch - 1;                                 // the last request whose first block is not behind bi
+            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_first[mid] <= bi) lo = mid; else hi = mid - 1; }
+            it.b = lo; it.blk = bi - s_first[lo];
+            len = s_len[lo];
+            it.req = len > 0 ? a.b_req_idx[lo] : 0;
+            it.write = true;
+        } else {
+            it.b = bi / a.num_blocks; it.blk = bi - it.b * a.num_blocks;
+            len = a.b_seqlen[it.b];
+            it.req = a.b_req_idx[it.b];
+            it.write = direct || it.blk < blocks_of(len);
+            if (len > 0 && (it.req < 0 || it.req >= a.rtt_rows || len > a.rtt_cols)) {
+                if (threadIdx.x == 0) q8_report(1, it.req);
+                len = 0;
+            }
+        }
+        it.t0 = it.blk * a.seq_block_size;
+        it.t1 = min(it.t0 + a.seq_block_size, len);
+        it.steps = it.t1 > it.t0 ? (it.t1 - it.t0 + R::kTokens - 1) / R::kTokens : 0;
+        return it;
+    };
+    const int tiles_per_kv = (a.group + kQ8HeadTile - 1) / kQ8HeadTile;   // more than 1 only with NH = 1
 
     if (warp == kQ8Warps) {
         // ------------------------------------------------------------------ producer
         const int tok = lane & 15, isv = lane >> 4;
-        const int32_t* rtt = a.req_to_tokens + (steps > 0 ? (int64_t)req * a.rtt_stride : 0);
         const int piece = lane % (NH * 8), share = lane / (NH * 8);         // 16 bytes of a row; which of an instruction's WT tokens
-        const uint8_t* ksrc = a.k + (int64_t)kv0 * a.k_stride_h + piece * 16;
-        const uint8_t* vsrc = a.v + (int64_t)kv0 * a.v_stride_h + piece * 16;
-        const float* ssrc = isv ? a.v_scale + kv0 : a.k_scale + kv0;
         const int64_t ssrc_stride = isv ? a.vs_stride_t : a.ks_stride_t;
-        // slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u; -1: no such token
-        auto load_slots = [&](int i, int u) -> int {
-            const int t = t0 + ((i + isv) * WT + u) * 16 + tok;
-            if (i + isv >= steps || t >= t1) return -1;
+        bool ok = !*s_abort;
+        int done = 0, st = 0, phase = 1;                                  // the first pass over the ring finds it empty
+        for (int n = blockIdx.x; n < items && ok; n += gridDim.x) {
+          const ItemQ8 it = item_at(n);
+          const int kv0 = it.hg * NH / tiles_per_kv;
+          const int32_t* rtt = a.req_to_tokens + (it.steps > 0 ? (int64_t)it.req * a.rtt_stride : 0);
+          const uint8_t* ksrc = a.k + (int64_t)kv0 * a.k_stride_h + piece * 16;
+          const uint8_t* vsrc = a.v + (int64_t)kv0 * a.v_stride_h + piece * 16;
+          const float* ssrc = isv ? a.v_scale + kv0 : a.k_scale + kv0;
+          // slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u; -1: no such token
+          auto load_slots = [&](int i, int u) -> int {
+            const int t = it.t0 + ((i + isv) * WT + u) * 16 + tok;
+            if (i + isv >= it.steps || t >= it.t1) return -1;
             const int s = rtt[t];
             if (s < 0 || s >= a.pool_rows) { q8_report(0, s); return -1; }
             return s;
-        };
-        int slots[WT], slots_next[WT];
+          };
+          int slots[WT], slots_next[WT];
 #pragma unroll
-        for (int u = 0; u < WT; ++u) { slots[u] = load_slots(0, u); slots_next[u] = load_slots(2, u); }
-        bool ok = !*s_abort;
-        int i = 0;
-        for (; i < steps && ok; ++i) {
-            const int st = i % R::kStages;
-            if (i >= R::kStages) {
-                ok = __all_sync(0xffffffffu, q8_wait(empty(st), ((i / R::kStages) - 1) & 1, s_abort, 8, i));
-                if (!ok) break;
-            }
+          for (int u = 0; u < WT; ++u) { slots[u] = load_slots(0, u); slots_next[u] = load_slots(2, u); }
+          for (int i = 0; i < it.steps; ++i, ++done) {
+            ok = __all_sync(0xffffffffu, q8_wait(empty(st), phase, s_abort, 8, done));
+            if (!ok) break;
             const uint32_t stage = sbase + st * R::kStageBytes;
             int s[WT];
 #pragma unroll
@@ -221,25 +289,36 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
 #pragma unroll
                 for (int u = 0; u < WT; ++u) { slots[u] = slots_next[u]; slots_next[u] = load_slots(i + 3, u); }
             }
+            if (++st == R::kStages) { st = 0; phase ^= 1; }
+          }
         }
-        if (!ok)                                                      // copies still under way: wait for them, bounded
-            for (int j = i > R::kStages ? i - R::kStages : 0; j < i; ++j)
+        if (!ok)                                                          // copies still under way: wait for them, bounded
+            for (int j = done > R::kStages ? done - R::kStages : 0; j < done; ++j)
                 ptx::mbar_wait_bounded(full(j % R::kStages), (j / R::kStages) & 1, &g_decode_q8_wait_limit_cycles, nullptr);
+        return;
     }
     const int g = lane >> 2, c = lane & 3;
-    const int hw = warp % NH, wt = warp / NH;            // consumer warps: kv head within the CTA, share of its tokens
+    const int hw = warp % NH, wt = warp / NH;            // kv head within the CTA, share of its tokens
+    bool ok = !*s_abort;
+    int st = 0, phase = 0, done = 0;
+
+    for (int n = blockIdx.x; n < items && ok; n += gridDim.x) {
+    const ItemQ8 it = item_at(n);
+    if (!it.write) continue;                             // a split behind the request's end: no steps either
+    // head tiles of this CTA: kv heads kv0 .. kv0 + NH - 1, or (a group of more than 8 q heads, NH = 1) tile `sub` of one
+    const int kv0 = it.hg * NH / tiles_per_kv, sub = it.hg * NH - kv0 * tiles_per_kv;
+    const int nheads = min(kQ8HeadTile, a.group - sub * kQ8HeadTile);
     const int h0 = (kv0 + hw) * a.group + sub * kQ8HeadTile;
-    const bool consumer = warp < kQ8Warps;
 
     // Q fragments: row g is head g of the tile (rows 8-15 of the MMA stay zero), dims in the order of the K words
     uint32_t qf[8][2];
     float qs;
     {
         float x[32], amax = 0.f;
-        const T* qp = reinterpret_cast<const T*>(a.q) + ((int64_t)b * a.num_q_heads + h0 + g) * 128 + c * 16;
+        const T* qp = reinterpret_cast<const T*>(a.q) + ((int64_t)it.b * a.num_q_heads + h0 + g) * 128 + c * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 u = consumer && g < nheads ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
+            const uint4 u = g < nheads ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -342,81 +421,85 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         }
     };
 
-    if (consumer) {
-        bool ok = !*s_abort;
 #pragma unroll 1
-        for (int i = 0, st = 0, phase = 0; i < steps && ok; ++i) {
-            ok = __all_sync(0xffffffffu, q8_wait(full(st), phase, s_abort, 9, i));
-            if (!ok) break;
-            compute(smem + st * R::kStageBytes);
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(empty(st));
-            if (++st == R::kStages) { st = 0; phase ^= 1; }
-        }
+    for (int i = 0; i < it.steps; ++i, ++done) {
+        ok = __all_sync(0xffffffffu, q8_wait(full(st), phase, s_abort, 9, done));
+        if (!ok) break;
+        compute(smem + st * R::kStageBytes);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(empty(st));
+        if (++st == R::kStages) { st = 0; phase ^= 1; }
     }
-    __syncthreads();
-    if (*s_abort) return;
-
-    // the warps' states: heads of their tiles, in units of each warp's own reference
-    MergeQ8& mg = *reinterpret_cast<MergeQ8*>(smem);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    if (consumer) {
-        if (c == 0) { mg.m[warp][g] = m_ref; mg.l[warp][g] = l_run; }
-        if (lane == 0) mg.v[warp] = v_ref * (1.f / 4096.f);
+    if constexpr (WT > 1) {
+        // the shares of a head's tokens meet in the warp with wt = 0; every state is in units of its own references
+        WarpStateQ8* ms = reinterpret_cast<WarpStateQ8*>(smem + R::kOffMerge);
+        if (wt > 0) {
+            WarpStateQ8& w = ms[(wt - 1) * NH + hw];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            *reinterpret_cast<float2*>(&mg.o[warp][2 * c][16 * g + 2 * j]) = make_float2(acc[j][0], acc[j][2]);
-            *reinterpret_cast<float2*>(&mg.o[warp][2 * c + 1][16 * g + 2 * j]) = make_float2(acc[j][1], acc[j][3]);
+            for (int j = 0; j < 32; ++j) w.acc[j][lane] = acc[j >> 2][j & 3];
+            w.m[lane] = m_ref; w.l[lane] = l_run; w.v[lane] = v_ref;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");                    // the four consumer warps
+        if (wt == 0) {
+#pragma unroll 1
+            for (int k = 0; k < WT - 1; ++k) {
+                const WarpStateQ8& w = ms[k * NH + hw];
+                const float m_new = fmaxf(m_ref, w.m[lane]), m_use = m_new == -INFINITY ? 0.f : m_new;
+                const float f0 = exp2f(m_ref - m_use), f1 = exp2f(w.m[lane] - m_use);     // 0 for a warp that saw no token
+                const float v_new = fmaxf(v_ref, w.v[lane]);
+                // with no value scale above zero on either side both accumulators are zero
+                const float r0 = v_new > 0.f ? f0 * (v_ref / v_new) : f0, r1 = v_new > 0.f ? f1 * (w.v[lane] / v_new) : f1;
+                l_run = l_run * f0 + w.l[lane] * f1;
+                m_ref = m_new; v_ref = v_new;
+                const float x0 = __shfl_sync(0xffffffffu, r0, 8 * c), x1 = __shfl_sync(0xffffffffu, r0, 8 * c + 4);
+                const float y0 = __shfl_sync(0xffffffffu, r1, 8 * c), y1 = __shfl_sync(0xffffffffu, r1, 8 * c + 4);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[j >> 2][j & 3] = acc[j >> 2][j & 3] * (j & 1 ? x1 : x0) + w.acc[j][lane] * (j & 1 ? y1 : y0);
+            }
+        }
+        // the states may be written again; the four warps go on, or leave, together
+        int leave;
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                     : "=r"(leave) : "r"(ok ? 0 : 1) : "memory");
+        ok = leave == 0;
+    }
+    if (ok && wt == 0) {
+        const float f = l_run == 0.f ? 0.f : (v_ref * (1.f / 4096.f)) / l_run;            // of head g; no token: zeros
+        const float lse = l_run == 0.f ? -INFINITY : ((m_ref == -INFINITY ? 0.f : m_ref) + log2f(l_run)) * kLn2Q8;
+        const int64_t row0 = (direct ? (int64_t)it.b : (int64_t)it.blk * a.batch + it.b) * a.num_q_heads + h0;
+        if (c == 0 && g < nheads) (direct ? a.lse : a.mid_lse)[row0 + g] = lse;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, 8 * c + 4 * k);
+            if (2 * c + k < nheads) {
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { x[2 * j] = acc[j][k] * fk; x[2 * j + 1] = acc[j][2 + k] * fk; }
+                store_row16(direct ? a.o : a.mid_o, (row0 + 2 * c + k) * 128 + 16 * g, x, direct ? a.o_dtype : ESP_DTYPE_F32);
+            }
         }
     }
-    __syncthreads();
-    if (!consumer) return;
-    const int d = threadIdx.x;
-#pragma unroll 1
-    for (int i = 0; i < NH; ++i) {
-        const int first = (kv0 + i) * a.group + sub * kQ8HeadTile;
-        for (int h = 0; h < nheads; ++h) {
-            float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WT; ++w) M = fmaxf(M, mg.m[w * NH + i][h]);
-            const float Mu = M == -INFINITY ? 0.f : M;
-            float L = 0.f, o = 0.f;
-#pragma unroll
-            for (int w = 0; w < WT; ++w) {
-                const float f = exp2f(mg.m[w * NH + i][h] - Mu);          // 0 for a warp that saw no token
-                L += mg.l[w * NH + i][h] * f;
-                o += mg.o[w * NH + i][h][d] * (f * mg.v[w * NH + i]);
-            }
-            o = L == 0.f ? 0.f : o / L;
-            const float lse = L == 0.f ? -INFINITY : (Mu + log2f(L)) * kLn2Q8;
-            if (a.o != nullptr) {
-                const int64_t row = (int64_t)b * a.num_q_heads + first + h;
-                store_as(a.o, row * 128 + d, o, a.o_dtype);
-                if (d == 0) a.lse[row] = lse;
-            } else {
-                const int64_t row = ((int64_t)blk * a.batch + b) * a.num_q_heads + first + h;
-                a.mid_o[row * 128 + d] = o;
-                if (d == 0) a.mid_lse[row] = lse;
-            }
-        }
     }
 }
 
-// The partials of one (request, head), by a CTA: at few rows and many splits (two requests of 262144 tokens: 64 rows x 256 splits)
-// one warp per row leaves most of the GPU idle.  Warp w takes splits w, w + 4, ...; lanes hold four dims each.
-__global__ void __launch_bounds__(128) decode_merge_q8_kernel(void* o, float* __restrict__ lse, const int32_t* __restrict__ b_seqlen,
-                                                              const float* __restrict__ mid_o, const float* __restrict__ mid_lse, int batch,
-                                                              int num_heads, int num_blocks, int block_seq, int o_dtype) {
+// The partials of one (request, head), by a CTA: at few rows and many splits (two requests of 262144 tokens: 64 rows x 410 splits)
+// one warp per row leaves most of the GPU idle (130 us; four warps 31 us).  Warp w takes splits w, w + W, ...; lanes hold four
+// dims each.
+template <int W>
+__global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float* __restrict__ lse, const int32_t* __restrict__ b_seqlen,
+                                                                 const float* __restrict__ mid_o, const float* __restrict__ mid_lse,
+                                                                 int batch, int num_heads, int num_blocks, int block_seq, int o_dtype) {
     const int pair = blockIdx.x, b = pair / num_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int len = b_seqlen[b];
     const int n = len <= 0 ? 0 : min((len - 1) / block_seq + 1, num_blocks);
     const int64_t bh = (int64_t)batch * num_heads;
-    __shared__ float s_m[4], s_l[4], s_o[4][128];
+    __shared__ float s_m[W], s_l[W], s_o[W][128];
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = warp; j0 < n; j0 += 4 * 32) {                // up to 32 splits of this warp at a time, one lse per lane
-        const int j = j0 + 4 * lane;
+    for (int j0 = warp; j0 < n; j0 += W * 32) {                // up to 32 splits of this warp at a time, one lse per lane
+        const int j = j0 + W * lane;
         const float x = j < n ? mid_lse[j * bh + pair] : -INFINITY;
         float mx = x;
 #pragma unroll
@@ -426,11 +509,11 @@ __global__ void __launch_bounds__(128) decode_merge_q8_kernel(void* o, float* __
         l = l * al + w;                                        // this lane's share of the sum
         acc.x *= al; acc.y *= al; acc.z *= al; acc.w *= al;
         m = m_new;
-        const int cnt = min(32, (n - j0 + 3) / 4);
+        const int cnt = min(32, (n - j0 + W - 1) / W);
 #pragma unroll 8
         for (int i = 0; i < cnt; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float4 v = *reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + 4 * i) * bh + pair) * 128 + lane * 4);
+            const float4 v = *reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + W * i) * bh + pair) * 128 + lane * 4);
             acc.x = fmaf(wi, v.x, acc.x); acc.y = fmaf(wi, v.y, acc.y); acc.z = fmaf(wi, v.z, acc.z); acc.w = fmaf(wi, v.w, acc.w);
         }
     }
@@ -439,10 +522,14 @@ __global__ void __launch_bounds__(128) decode_merge_q8_kernel(void* o, float* __
     if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
     *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
     __syncthreads();
-    const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), Mu = M == -INFINITY ? 0.f : M;
+    if (threadIdx.x >= 128) return;
+    float M = s_m[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) M = fmaxf(M, s_m[w]);
+    const float Mu = M == -INFINITY ? 0.f : M;
     float L = 0.f, x = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
         const float f = exp2f((s_m[w] - Mu) * kLog2eQ8);
         L += s_l[w] * f;
         x += s_o[w][threadIdx.x] * f;
@@ -473,14 +560,18 @@ namespace esp {
 
 template <typename T, int CODE>
 static int launch_stage1_q8(DecodeQ8Args& a, int64_t nblk, cudaStream_t s) {
-    // neighbouring kv heads to a CTA, four or two where they divide evenly and lie next to each other; else one, whose tokens the
-    // four warps share
+    // neighbouring kv heads to a CTA, four or two where they divide evenly and lie next to each other, as long as every SM gets
+    // two CTAs; else one, whose tokens the four warps share (one request of 513 tokens, 8 kv heads: see the measurements below)
     const bool dense = a.group <= kQ8HeadTile && a.k_stride_h == 128 && a.v_stride_h == 128;
-    const int nh = dense && a.head_tiles % 4 == 0 ? 4 : (dense && a.head_tiles % 2 == 0 ? 2 : 1);
+    const int64_t tiles = nblk * a.batch * a.head_tiles;
+    if (tiles > 2147483647LL - 65536) return ESP_ERR_TOO_LARGE;
+    const int nh = dense && a.head_tiles % 4 == 0 && tiles >= 4 * 2 * kNumSMs ? 4 : (dense && a.head_tiles % 2 == 0 && tiles >= 2 * 2 * kNumSMs ? 2 : 1);
     a.head_groups = a.head_tiles / nh;
+    a.num_blocks = (int)nblk;
     a.scale_vec = aligned16(a.k_scale) && aligned16(a.v_scale) && a.ks_stride_t % 4 == 0 && a.vs_stride_t % 4 == 0;
-    if (nblk * a.head_groups > 2147483647LL) return ESP_ERR_TOO_LARGE;
-    const dim3 grid((unsigned)(nblk * a.head_groups), a.batch);
+    const int64_t items = tiles / nh, resident = 3 * kNumSMs;
+    a.compact = items > resident && a.batch <= kQ8MaxCompact && a.o == nullptr;
+    const dim3 grid((unsigned)(items < resident ? items : resident));
 #define ESP_S1Q(NH)                                                                                                               \
     {                                                                                                                            \
         ESP_CUDA_TRY(cudaFuncSetAttribute(decode_stage1_q8_kernel<T, CODE, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, RingQ8<NH>::kSmem)); \
@@ -528,7 +619,7 @@ extern "C" int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q,
     if (!mid_o || !mid_lse) return ESP_ERR_BAD_ARG;
     DecodeQ8Args a{mid_o, mid_lse, q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h,
                    k_scale_stride_t, v_scale_stride_t, req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch,
-                   num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0, nullptr, nullptr, 0};
+                   num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0, 0, 0, nullptr, nullptr, 0};
     return stage1_q8(a, head_dim, max_len_in_batch, dtype, code, sm_scale, (cudaStream_t)stream);
 }
 
@@ -549,13 +640,16 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     const int64_t rows = nblk * batch * num_q_heads;
     DecodeQ8Args a{workspace, workspace + rows * 128, q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, k_stride_t, k_stride_h,
                    v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t, req_to_tokens, req_to_tokens_stride, req_rows, req_cols,
-                   b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0,
+                   b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0, 0, 0,
                    nblk == 1 ? o : nullptr, nblk == 1 ? lse : nullptr, o_dtype};
     cudaStream_t s = (cudaStream_t)stream;
     const int rc = stage1_q8(a, head_dim, max_len, dtype, code, sm_scale, s);
     if (rc || nblk == 1) return rc;
-    decode_merge_q8_kernel<<<(unsigned)((int64_t)batch * num_q_heads), 128, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, batch, num_q_heads,
-                                                                                  (int)nblk, seq_block_size, o_dtype);
+    const unsigned pairs = (unsigned)((int64_t)batch * num_q_heads);
+    if (nblk > 64)
+        decode_merge_q8_kernel<16><<<pairs, 512, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, batch, num_q_heads, (int)nblk, seq_block_size, o_dtype);
+    else
+        decode_merge_q8_kernel<4><<<pairs, 128, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, batch, num_q_heads, (int)nblk, seq_block_size, o_dtype);
     ESP_LAUNCH_CHECK("decode_merge_q8_kernel");
     return ESP_OK;
 }
