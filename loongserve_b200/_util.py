@@ -30,21 +30,41 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+# torch's own accessors behind current_device() / current_stream(), without the Stream object that the latter builds (3 us per
+# call, as much as the launch it is for)
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+_get_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_device() -> int:
+    return _get_device() if _get_device is not None else torch.cuda.current_device()
+
+
+def stream_of(device: int) -> int:
+    """The current stream of a device, as the C ABI takes it."""
+    return _get_stream(device) if _get_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("the ESP attention ops run on CUDA tensors only (there is no CPU path)")
 
 
-def need_here(*ts):
-    """All tensors on the CURRENT CUDA device: the kernels are launched there, on its current stream."""
-    for t in ts:
-        if t is not None and not t.is_cuda:
-            raise RuntimeError("the ESP attention ops run on CUDA tensors only (there is no CPU path)")
-    d = torch.cuda.current_device()
+def need_here(first, *ts) -> int:
+    """The device of the tensors (None is skipped, the first is a tensor), which must be the CURRENT CUDA device: the kernels are
+    launched there, on its current stream."""
+    d = first.get_device()
+    if d < 0:
+        raise RuntimeError("the ESP attention ops run on CUDA tensors only (there is no CPU path)")
+    if d != current_device():
+        raise RuntimeError(f"tensor on cuda:{d}, but the current CUDA device is cuda:{current_device()}: select the tensors' device first")
     for t in ts:
         if t is not None and t.get_device() != d:
-            raise RuntimeError(f"tensor on {t.device}, but the current CUDA device is cuda:{d}: select the tensors' device first")
+            if t.get_device() < 0:
+                raise RuntimeError("the ESP attention ops run on CUDA tensors only (there is no CPU path)")
+            raise RuntimeError(f"tensor on cuda:{t.get_device()}, but the current CUDA device is cuda:{d}: all tensors of a call lie there")
+    return d
 
 
 _CODES = {torch.int8: _lib.ESP_CODE_INT8, torch.float8_e4m3fn: _lib.ESP_CODE_E4M3}

@@ -67,21 +67,23 @@ struct MmArgs {
 };
 
 // ------------------------------------------------------------------------------------------------
-// Many tokens: CTA pairs (cluster of two, cta_group::2).  A pair owns 256 tokens x 256 channels; CTA c holds 128 of the tokens
+// Many tokens: CTA pairs (cluster of two, cta_group::2).  A pair owns 256 tokens x PN channels; CTA c holds 128 of the tokens
 // (A) and half of the channels (B), one thread of the even CTA issues the M = 256 MMAs that run on both SMs.  Persistent: each
-// pair walks over tiles; two accumulators of 256 columns take turns, so the epilogue of one tile runs under the next one's MMAs.
+// pair walks over tiles; two accumulators of PN columns take turns, so the epilogue of one tile runs under the next one's MMAs.
 // Warps: 0 producer, 1 issuer (and tensor-memory owner), 2-3 idle, 4-7 epilogue (one token row per thread).
-constexpr int kPairM = 128, kPairN = 256, kPairStages = 6, kPairThreads = 256;
-constexpr int kPairStageBytes = kPairM * kBK + kPairN / 2 * kBK;                 // 32 KiB per CTA
+constexpr int kPairM = 128, kPairThreads = 256;
 constexpr int kEpiRowBytes = 128 + 16;                                           // one staged row piece, padded against bank conflicts
-constexpr int kPairOffEpi = kPairStages * kPairStageBytes;                       // per epilogue warp: 32 row pieces, 256 channel scales
-constexpr int kPairEpiWarp = 32 * kEpiRowBytes + kPairN * 4;
-constexpr int kPairOffBar = kPairOffEpi + 4 * kPairEpiWarp;
-enum { MB_FULL = 0, MB_EMPTY = kPairStages, MB_ACC_FULL = 2 * kPairStages, MB_ACC_EMPTY = 2 * kPairStages + 2, MB_DRAIN = 2 * kPairStages + 4,
-       MB_COUNT = 2 * kPairStages + 5 };
-constexpr int kPairOffMisc = kPairOffBar + MB_COUNT * 8;
-constexpr int kPairSmem = kPairOffMisc + 16 + 1024;
-static_assert(kPairSmem <= 232448, "shared memory of one CTA");
+template <int PN> struct Pair {
+    static constexpr int kStages = PN == 256 ? 6 : 8;
+    static constexpr int kStageBytes = kPairM * kBK + PN / 2 * kBK;              // 32 or 24 KiB per CTA
+    static constexpr int kOffEpi = kStages * kStageBytes;                        // per epilogue warp: 32 row pieces, PN channel scales
+    static constexpr int kEpiWarp = 32 * kEpiRowBytes + PN * 4;
+    static constexpr int kOffBar = kOffEpi + 4 * kEpiWarp;
+    static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = 2 * kStages + 2, kDrain = 2 * kStages + 4, kBars = 2 * kStages + 5;
+    static constexpr int kOffMisc = kOffBar + kBars * 8;
+    static constexpr int kSmem = kOffMisc + 16 + 1024;
+};
+static_assert(Pair<256>::kSmem <= 232448 && Pair<128>::kSmem <= 232448, "shared memory of one CTA");
 
 // Tiles are walked in bands of 8 token tiles: the pairs that run together share both operands' tiles in L2.
 __device__ __forceinline__ void tile_of(int t, int m_tiles, int n_tiles, int& m, int& n) {
@@ -92,16 +94,17 @@ __device__ __forceinline__ void tile_of(int t, int m_tiles, int n_tiles, int& m,
     m = band * kBand + (in_band - n * rows);
 }
 
-template <typename OT>
+template <typename OT, int PN>
 __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
                                                                        const __grid_constant__ CUtensorMap tm_w, const MmArgs p) {
+    using C = Pair<PN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    auto bar = [base](int i) { return base + kPairOffBar + 8u * i; };
+    auto bar = [base](int i) { return base + C::kOffBar + 8u * i; };
     auto lbar = [&bar](int i) { return map_to_cta(bar(i), 0u); };               // the even CTA's barrier
-    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + kPairOffMisc);
-    volatile int* s_abort = reinterpret_cast<volatile int*>(gen + kPairOffMisc + 4);
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::kOffMisc);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = cluster_ctarank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -109,12 +112,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
 
     if (threadIdx.x == 0) {
         *s_abort = (*reinterpret_cast<volatile int*>(&g_mm_status[0]) != 0) ? 1 : 0;    // after a reported timeout nothing is started
-        for (int i = 0; i < MB_COUNT; ++i) mbar_init(bar(i), (i == MB_ACC_EMPTY || i == MB_ACC_EMPTY + 1) ? 8 : 1);
+        for (int i = 0; i < C::kBars; ++i) mbar_init(bar(i), (i == C::kAccEmpty || i == C::kAccEmpty + 1) ? 8 : 1);
         fence_barrier_init();
         prefetch_tensormap(&tm_a); prefetch_tensormap(&tm_w);
     }
     __syncthreads();
-    if (warp == 1) { tmem_alloc_pair(base + kPairOffMisc, 2 * kPairN); tmem_relinquish_pair(); }
+    if (warp == 1) { tmem_alloc_pair(base + C::kOffMisc, 2 * PN); tmem_relinquish_pair(); }
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
@@ -128,45 +131,45 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
             for (int t = pair; t < tiles && ok; t += pairs) {
                 int mt, nt;
                 tile_of(t, p.m_tiles, p.n_tiles, mt, nt);
-                const int m0 = mt * 2 * kPairM + (int)cta * kPairM, n0 = nt * kPairN + (int)cta * (kPairN / 2);
+                const int m0 = mt * 2 * kPairM + (int)cta * kPairM, n0 = nt * PN + (int)cta * (PN / 2);
                 for (int k = 0; k < p.kstages; ++k, ++it) {
-                    const int st = it % kPairStages;
-                    if (it >= kPairStages && !(ok = mm_wait(bar(MB_EMPTY + st), ((it / kPairStages) - 1) & 1, s_abort, MW_EMPTY, it))) break;
-                    if (cta == 0) mbar_expect_tx(bar(MB_FULL + st), 2 * kPairStageBytes);
-                    const uint32_t dst = base + st * kPairStageBytes;
-                    tma_load_2d_pair(dst, &tm_a, lbar(MB_FULL + st), k * kBK, m0);
-                    tma_load_2d_pair(dst + kPairM * kBK, &tm_w, lbar(MB_FULL + st), k * kBK, n0);
+                    const int st = it % C::kStages;
+                    if (it >= C::kStages && !(ok = mm_wait(bar(C::kEmpty + st), ((it / C::kStages) - 1) & 1, s_abort, MW_EMPTY, it))) break;
+                    if (cta == 0) mbar_expect_tx(bar(C::kFull + st), 2 * C::kStageBytes);
+                    const uint32_t dst = base + st * C::kStageBytes;
+                    tma_load_2d_pair(dst, &tm_a, lbar(C::kFull + st), k * kBK, m0);
+                    tma_load_2d_pair(dst + kPairM * kBK, &tm_w, lbar(C::kFull + st), k * kBK, n0);
                 }
             }
             if (!ok && cta == 0)                               // copies of both CTAs count on the even CTA's barriers
-                for (int i = it > kPairStages ? it - kPairStages : 0; i < it; ++i) mm_drain(bar(MB_FULL + i % kPairStages), (i / kPairStages) & 1);
+                for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) mm_drain(bar(C::kFull + i % C::kStages), (i / C::kStages) & 1);
         }
     } else if (warp == 1) {
         if (cta == 0 && lane == 0 && !*s_abort) {
-            constexpr uint32_t idesc = make_idesc_i8(2 * kPairM, kPairN);
+            constexpr uint32_t idesc = make_idesc_i8(2 * kPairM, PN);
             int it = 0, n_tile = 0;
             bool ok = true;
             for (int t = pair; t < tiles && ok; t += pairs, ++n_tile) {
                 const int buf = n_tile & 1;
-                if (n_tile >= 2 && !(ok = mm_wait(bar(MB_ACC_EMPTY + buf), ((n_tile >> 1) - 1) & 1, s_abort, MW_ACC_EMPTY, n_tile))) break;
+                if (n_tile >= 2 && !(ok = mm_wait(bar(C::kAccEmpty + buf), ((n_tile >> 1) - 1) & 1, s_abort, MW_ACC_EMPTY, n_tile))) break;
                 tc_fence_after();
                 for (int k = 0; k < p.kstages; ++k, ++it) {
-                    const int st = it % kPairStages;
-                    if (!(ok = mm_wait(bar(MB_FULL + st), (it / kPairStages) & 1, s_abort, MW_FULL, it))) break;
+                    const int st = it % C::kStages;
+                    if (!(ok = mm_wait(bar(C::kFull + st), (it / C::kStages) & 1, s_abort, MW_FULL, it))) break;
                     tc_fence_after();
-                    const uint32_t sa = base + st * kPairStageBytes, sb = sa + kPairM * kBK;
+                    const uint32_t sa = base + st * C::kStageBytes, sb = sa + kPairM * kBK;
 #pragma unroll
                     for (int j = 0; j < kBK / 32; ++j)
-                        umma_i8_pair_ss(tmem + buf * kPairN, desc_kmajor_sw128(sa + j * 32), desc_kmajor_sw128(sb + j * 32), idesc, (k | j) != 0);
-                    umma_pair_commit(bar(MB_EMPTY + st));
+                        umma_i8_pair_ss(tmem + buf * PN, desc_kmajor_sw128(sa + j * 32), desc_kmajor_sw128(sb + j * 32), idesc, (k | j) != 0);
+                    umma_pair_commit(bar(C::kEmpty + st));
                 }
-                if (ok) umma_pair_commit(bar(MB_ACC_FULL + buf));
+                if (ok) umma_pair_commit(bar(C::kAccFull + buf));
             }
-            if (!ok) { umma_pair_commit(bar(MB_DRAIN)); mm_drain(bar(MB_DRAIN), 0); }
+            if (!ok) { umma_pair_commit(bar(C::kDrain)); mm_drain(bar(C::kDrain), 0); }
         }
     } else if (warp >= 4) {
         const int w = warp - 4;
-        uint8_t* stage = gen + kPairOffEpi + w * kPairEpiWarp;
+        uint8_t* stage = gen + C::kOffEpi + w * C::kEpiWarp;
         float* sw = reinterpret_cast<float*>(stage + 32 * kEpiRowBytes);
         constexpr int kCols = 128 / (int)sizeof(OT);           // channels per staged piece (128 bytes of a row)
         OT* out = reinterpret_cast<OT*>(p.out);
@@ -176,27 +179,27 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
             int mt, nt;
             tile_of(t, p.m_tiles, p.n_tiles, mt, nt);
             const int64_t row0 = (int64_t)mt * 2 * kPairM + (int64_t)cta * kPairM + w * 32;      // first row of this warp
-            const int64_t n0 = (int64_t)nt * kPairN;
+            const int64_t n0 = (int64_t)nt * PN;
             const int buf = n_tile & 1;
             __syncwarp();
-            for (int i = lane; i < kPairN; i += 32) sw[i] = n0 + i < p.N ? p.w_scale[n0 + i] : 0.f;
+            for (int i = lane; i < PN; i += 32) sw[i] = n0 + i < p.N ? p.w_scale[n0 + i] : 0.f;
             const float sa = row0 + lane < p.M ? p.a_scale[row0 + lane] : 0.f;
-            ok = mm_wait(bar(MB_ACC_FULL + buf), (n_tile >> 1) & 1, s_abort, MW_ACC_FULL, n_tile);
+            ok = mm_wait(bar(C::kAccFull + buf), (n_tile >> 1) & 1, s_abort, MW_ACC_FULL, n_tile);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t acc = tmem + buf * kPairN + ((uint32_t)(w * 32) << 16);
+            const uint32_t acc = tmem + buf * PN + ((uint32_t)(w * 32) << 16);
             const int rows = (int)min((int64_t)32, p.M - row0);
 #pragma unroll 1
-            for (int c0 = 0; c0 < kPairN; c0 += kCols) {
+            for (int c0 = 0; c0 < PN; c0 += kCols) {
                 uint32_t r[kCols / 32][32];
 #pragma unroll
                 for (int h = 0; h < kCols / 32; ++h) tmem_ld32(acc + c0 + h * 32, r[h]);
                 tmem_wait_ld();
-                if (c0 + kCols == kPairN) {                     // the last read of this accumulator: the issuer may have it back
+                if (c0 + kCols == PN) {                     // the last read of this accumulator: the issuer may have it back
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(lbar(MB_ACC_EMPTY + buf));
+                    if (lane == 0) mbar_arrive_cluster(lbar(C::kAccEmpty + buf));
                 }
 #pragma unroll
                 for (int h = 0; h < kCols / 32; ++h)
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();                  // neither CTA frees tensor memory while the peer's MMAs may still use it
-    if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 2 * kPairN); }
+    if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 2 * PN); }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -239,8 +242,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
 // of the tokens).  Warps: 0 producer, 1 issuer, 2-5 epilogue (one channel per thread).
 constexpr int kSkinnyThreads = 192;
 template <int TN> struct Skinny {
+    static_assert(TN == 16 || TN == 32 || TN == 64 || TN == 128, "tokens of a tile");
     static constexpr int kStageBytes = 128 * kBK + TN * kBK;
-    static constexpr int kStages = TN >= 256 ? 4 : (TN >= 128 ? 6 : (TN >= 64 ? 4 : 5));
+    static constexpr int kStages = TN >= 128 ? 3 : (TN >= 64 ? 4 : 5);      // two CTAs to an SM
     static constexpr int kDump = 128 * TN * 4;                      // partials, over the pipeline's stages once they are used up
     static constexpr int kBody = kStages * kStageBytes > kDump ? kStages * kStageBytes : kDump;
     static constexpr int kOffBar = kBody;
@@ -395,49 +399,49 @@ static int make_map(CUtensorMap* tm, const int8_t* p, int64_t rows, int64_t k, i
 constexpr int kMaxMmDevices = 64;
 
 // How many CTA pairs the device keeps resident at once (asked once per device and kernel).
-template <typename OT>
+template <typename OT, int PN>
 static int resident_pairs(int* out) {
     static int known[kMaxMmDevices] = {0};
     int dev = -1;
     ESP_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= kMaxMmDevices) return ESP_ERR_UNSUPPORTED;
     if (!known[dev]) {
-        ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_pair_kernel<OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_pair_kernel<OT, PN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Pair<PN>::kSmem));
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(kNumSMs / 2 * 2); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = kPairSmem;
+        cfg.gridDim = dim3(kNumSMs / 2 * 2); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = Pair<PN>::kSmem;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
         cfg.attrs = at; cfg.numAttrs = 1;
         int n = 0;
-        ESP_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, mm_w8a8_pair_kernel<OT>, &cfg));
+        ESP_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, mm_w8a8_pair_kernel<OT, PN>, &cfg));
         known[dev] = n > 0 ? n : 1;
     }
     *out = known[dev];
     return ESP_OK;
 }
 
-template <typename OT>
+template <typename OT, int PN>
 static int launch_pair(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, int64_t k, MmArgs g, cudaStream_t s) {
     CUtensorMap ta, tw;
     int rc = make_map(&ta, a, g.M, k, lda, kPairM);
-    if (!rc) rc = make_map(&tw, w, g.N, k, ldw, kPairN / 2);
+    if (!rc) rc = make_map(&tw, w, g.N, k, ldw, PN / 2);
     int pairs = 0;
-    if (!rc) rc = resident_pairs<OT>(&pairs);
+    if (!rc) rc = resident_pairs<OT, PN>(&pairs);
     if (rc) return rc;
     g.m_tiles = (int)((g.M + 2 * kPairM - 1) / (2 * kPairM));
-    g.n_tiles = (int)((g.N + kPairN - 1) / kPairN);
+    g.n_tiles = (int)((g.N + PN - 1) / PN);
     const int64_t tiles = (int64_t)g.m_tiles * g.n_tiles;
     if (tiles > 2147483647LL) return ESP_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)); cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = kPairSmem; cfg.stream = s;
+    cfg.dynamicSmemBytes = Pair<PN>::kSmem; cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
-    ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_pair_kernel<OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    ESP_CUDA_TRY(cudaLaunchKernelEx(&cfg, mm_w8a8_pair_kernel<OT>, ta, tw, g));
+    ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_pair_kernel<OT, PN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Pair<PN>::kSmem));
+    ESP_CUDA_TRY(cudaLaunchKernelEx(&cfg, mm_w8a8_pair_kernel<OT, PN>, ta, tw, g));
     return ESP_OK;
 }
 
@@ -466,17 +470,25 @@ template <typename OT>
 static int launch_mm(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, int64_t k, MmArgs g, cudaStream_t s) {
     g.kstages = (int)((k + kBK - 1) / kBK);
     g.vec_out = ((uintptr_t)g.out % 16 == 0 && (g.ldo * (int64_t)sizeof(OT)) % 16 == 0) ? 1 : 0;
-    if (g.M > 256) return launch_pair<OT>(a, lda, w, ldw, k, g, s);
-    // enough CTAs that two per SM have work, as long as each keeps a few stages of K
-    const int64_t nt = (g.N + 127) / 128;
-    int splits = (int)(2 * kNumSMs / nt);
-    splits = splits > 8 ? 8 : (splits < 1 ? 1 : splits);
-    while (splits > 1 && g.kstages < 4 * splits) --splits;
-    if (g.M <= 16) return launch_skinny<OT, 16>(a, lda, w, ldw, k, g, splits, s);
-    if (g.M <= 32) return launch_skinny<OT, 32>(a, lda, w, ldw, k, g, splits, s);
-    if (g.M <= 64) return launch_skinny<OT, 64>(a, lda, w, ldw, k, g, splits, s);
-    if (g.M <= 128) return launch_skinny<OT, 128>(a, lda, w, ldw, k, g, splits, s);
-    return launch_skinny<OT, 256>(a, lda, w, ldw, k, g, splits, s);
+    // K is split over as many CTAs (a power of two: other clusters leave SMs of a GPC unused) as two per SM can run at once, as
+    // long as each keeps four stages.
+    auto splits_of = [&](int64_t tiles) {
+        int s = 8;
+        while (s > 1 && (tiles * s > 2 * kNumSMs || g.kstages < 4 * s)) s /= 2;
+        return s;
+    };
+    const int64_t nt = (g.N + 127) / 128, mt = (g.M + 127) / 128;
+    if (g.M <= 16) return launch_skinny<OT, 16>(a, lda, w, ldw, k, g, splits_of(nt), s);
+    if (g.M <= 32) return launch_skinny<OT, 32>(a, lda, w, ldw, k, g, splits_of(nt), s);
+    if (g.M <= 64) return launch_skinny<OT, 64>(a, lda, w, ldw, k, g, splits_of(nt), s);
+    // Up to 256 tokens the pairs have too few tiles when the channels are few: 256 x 4096 x 11008 takes 20.1 us in four splits
+    // and 31.0 us on pairs; with more channels (256 x 22016 x 4096) 54.3 us and 29.7 us.
+    if (g.M <= 256 && splits_of(nt * mt) >= 4) return launch_skinny<OT, 128>(a, lda, w, ldw, k, g, splits_of(nt * mt), s);
+    // Tiles of 128 channels cost about 0.6 of those of 256: taken where they fill the last wave of pairs better.
+    const int64_t m2 = (g.M + 255) / 256, pairs = kNumSMs / 2;
+    const int64_t w256 = (m2 * ((g.N + 255) / 256) + pairs - 1) / pairs, w128 = (m2 * nt + pairs - 1) / pairs;
+    if (6 * w128 < 10 * w256) return launch_pair<OT, 128>(a, lda, w, ldw, k, g, s);
+    return launch_pair<OT, 256>(a, lda, w, ldw, k, g, s);
 }
 
 int mm_w8a8_status(int32_t out[4], int32_t clear) {

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._util import code_tag, dtype16_tag, dtype_tag, need_cuda, need_here, need_i32, ptr, stream_ptr
+from ._util import code_tag, dtype16_tag, dtype_tag, need_cuda, need_here, need_i32, ptr, stream_of, stream_ptr
 
 
 @torch.inference_mode()
@@ -46,36 +46,39 @@ def flash_decoding_stage2(o, out_logexpsum, b_seqlen, mid_o, mid_o_logexpsum, bl
 
 
 def _q8_args(q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen):
-    assert q.dim() == 3 and q.is_contiguous() and k.dim() == 3 and v.dim() == 3 and k.stride(2) == 1 and v.stride(2) == 1
-    assert k.shape[1:] == v.shape[1:] and k.shape[2] == q.shape[2] and k_scale.shape == k.shape[:2] and v_scale.shape == v.shape[:2]
-    assert k.shape[1] == 1 or (k_scale.stride(1) == 1 and v_scale.stride(1) == 1)
+    """The arguments of the C calls from q to b_seqlen and the sizes behind them, checked."""
+    qs, ks, vs = q.shape, k.shape, v.shape
+    assert len(qs) == 3 and len(ks) == 3 and len(vs) == 3 and q.is_contiguous()
+    (kt, kh, kd), (vt, vh, vd) = k.stride(), v.stride()
+    assert kd == 1 and vd == 1 and ks[1:] == vs[1:] and ks[2] == qs[2] and k_scale.shape == ks[:2] and v_scale.shape == vs[:2]
+    (kst, ksh), (vst, vsh) = k_scale.stride(), v_scale.stride()
+    assert ks[1] == 1 or (ksh == 1 and vsh == 1)
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or v.dtype != k.dtype or req_to_tokens.dtype != torch.int32:
         raise TypeError("k and v hold codes of one type, their scales are fp32, req_to_tokens is int32")
-    assert req_to_tokens.dim() == 2 and req_to_tokens.stride(1) == 1
+    ts = req_to_tokens.shape
+    assert len(ts) == 2 and req_to_tokens.stride(1) == 1
     need_i32(b_req_idx, b_seqlen)
-    assert b_req_idx.shape[0] == q.shape[0] and b_seqlen.shape[0] == q.shape[0]
+    assert b_req_idx.shape == qs[:1] and b_seqlen.shape == qs[:1]
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), kt, kh, vt, vh, kst, vst,
+            req_to_tokens.data_ptr(), req_to_tokens.stride(0), ts[0], ts[1], b_req_idx.data_ptr(), b_seqlen.data_ptr(), qs[0], qs[1],
+            ks[1], qs[2]), min(ks[0], vs[0])
 
 
-@torch.inference_mode()
 def flash_decoding_stage1_q8(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen,
                              max_len_in_batch: int, seq_block_size: int, sm_scale: float = 0.0):
     """``flash_decoding_stage1`` over a pool held in 8 bits: k, v int8 or e4m3 codes [slots, Hkv, 128], k_scale, v_scale fp32
     [slots, Hkv].  The partials go to ``flash_decoding_stage2`` unchanged."""
-    need_here(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen)
-    _q8_args(q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen)
+    dev = need_here(q, mid_o, mid_o_logexpsum, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen)
+    args, slots = _q8_args(q, k, k_scale, v, v_scale, req_to_tokens, b_req_idx, b_seqlen)
     assert mid_o.is_contiguous() and mid_o_logexpsum.is_contiguous()
     assert mid_o.dim() == 4 and mid_o_logexpsum.dim() == 3 and mid_o.dtype == mid_o_logexpsum.dtype == torch.float32
-    batch, hq, dim = q.shape
     nblk = (int(max_len_in_batch) + int(seq_block_size) - 1) // int(seq_block_size)
     assert mid_o.shape[0] >= nblk and mid_o.shape[1:] == q.shape
     assert mid_o_logexpsum.shape[0] >= nblk and mid_o_logexpsum.shape[1:] == q.shape[:2]
-    rc = _lib.attn().esp_decode_stage1_q8(
-        mid_o.data_ptr(), mid_o_logexpsum.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_scale.stride(0), v_scale.stride(0), req_to_tokens.data_ptr(),
-        req_to_tokens.stride(0), req_to_tokens.shape[0], req_to_tokens.shape[1], b_req_idx.data_ptr(), b_seqlen.data_ptr(), batch, hq,
-        k.shape[1], dim, int(max_len_in_batch), int(seq_block_size), dtype16_tag(q), code_tag(k), float(sm_scale),
-        min(k.shape[0], v.shape[0]), stream_ptr())
-    _lib.check(rc, "esp_decode_stage1_q8")
+    rc = _lib.attn().esp_decode_stage1_q8(mid_o.data_ptr(), mid_o_logexpsum.data_ptr(), *args, int(max_len_in_batch), int(seq_block_size),
+                                          dtype16_tag(q), code_tag(k), sm_scale, slots, stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_decode_stage1_q8")
 
 
 def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -> int:
@@ -87,31 +90,33 @@ def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -
     return min(512, max(128, -(-max(int(max_len_in_batch), 1) // splits // 128) * 128))
 
 
-@torch.inference_mode()
 def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len,
                               max_len_in_batch: int, block_seq=None, out=None, out_logexpsum=None, sm_scale: float = 0.0):
     """Decode attention over a pool held in 8 bits, splits and merge in one call: (o like q unless ``out`` is given, lse fp32).
     ``block_seq``: tokens per split, chosen from the sizes by default.  A request of length zero gets o = 0, lse = -inf."""
-    need_here(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len, out, out_logexpsum)
-    _q8_args(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len)
-    batch, hq, dim = q.shape
-    hkv = cache_k.shape[1]
-    o = torch.empty_like(q) if out is None else out
-    lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device) if out_logexpsum is None else out_logexpsum
-    assert o.shape == q.shape and o.is_contiguous() and lse.shape == (batch, hq) and lse.is_contiguous()
-    if lse.dtype != torch.float32:
-        raise TypeError("out_logexpsum is fp32")
-    block = q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len_in_batch) if block_seq is None else int(block_seq)
-    nblk = (int(max_len_in_batch) + block - 1) // block
-    work = torch.empty(nblk * batch * hq * (dim + 1), dtype=torch.float32, device=q.device) if nblk > 1 else None
-    rc = _lib.attn().esp_decode_attention_q8(
-        o.data_ptr(), lse.data_ptr(), ptr(work), q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), cache_k.stride(0), cache_k.stride(1), cache_v.stride(0), cache_v.stride(1), k_scale.stride(0),
-        v_scale.stride(0), req_to_token_indexs.data_ptr(), req_to_token_indexs.stride(0), req_to_token_indexs.shape[0],
-        req_to_token_indexs.shape[1], b_req_idx.data_ptr(), b_seq_len.data_ptr(), batch, hq, hkv, dim, int(max_len_in_batch), block,
-        dtype16_tag(q), dtype_tag(o), code_tag(cache_k), float(sm_scale), min(cache_k.shape[0], cache_v.shape[0]), stream_ptr())
-    _lib.check(rc, "esp_decode_attention_q8")
-    return o, lse
+    dev = need_here(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len, out, out_logexpsum)
+    args, slots = _q8_args(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len)
+    batch, hq, hkv, dim = args[-4:]
+    max_len = int(max_len_in_batch)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        assert out.shape == q.shape and out.is_contiguous()
+    if out_logexpsum is None:
+        out_logexpsum = k_scale.new_empty((batch, hq))
+    else:
+        assert out_logexpsum.shape == (batch, hq) and out_logexpsum.is_contiguous()
+        if out_logexpsum.dtype != torch.float32:
+            raise TypeError("out_logexpsum is fp32")
+    tags = dtype16_tag(q), dtype_tag(out), code_tag(cache_k)
+    block = int(block_seq) if block_seq is not None else q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len)
+    nblk = (max_len + block - 1) // block
+    work = k_scale.new_empty(nblk * batch * hq * (dim + 1)) if nblk > 1 else None
+    rc = _lib.attn().esp_decode_attention_q8(out.data_ptr(), out_logexpsum.data_ptr(), ptr(work), *args, max_len, block, *tags, sm_scale,
+                                             slots, stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_decode_attention_q8")
+    return out, out_logexpsum
 
 
 def longserve_flash_decode_stage1(q, k, v, Req_to_tokens, B_req_idx, B_Seqlen, max_len_in_batch, mid_out,

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._util import code_tag, dtype16_tag, dtype_tag, idx64_flag, need_cuda, need_here, need_i32, ptr, stream_ptr
+from ._util import code_tag, dtype16_tag, dtype_tag, idx64_flag, need_cuda, need_here, need_i32, ptr, stream_of, stream_ptr
 
 
 def _rows(t):
@@ -136,16 +136,18 @@ def decoding_stage_migration_receiver_kernel(recv_buf, req_to_token_indexes, kv_
 
 # ---------------------------------------------------------------------------------------- the pool held in 8 bits
 def _q8_pool(codes, scales):
-    """(heads, head_dim, code tag) of a pool of 8-bit rows: codes [slots, heads, head_dim], scales fp32 [slots, heads]."""
-    assert codes.dim() == 3 and codes.stride(2) == 1, "expected codes [slots, heads, head_dim] with contiguous head_dim"
-    assert scales.dim() == 2 and scales.shape == codes.shape[:2] and (scales.stride(1) == 1 or scales.shape[1] == 1), \
-        "expected scales [slots, heads] with contiguous heads"
+    """(slots, heads, head_dim, code tag, row stride, head stride, scale row stride) of a pool of 8-bit rows: codes [slots, heads,
+    head_dim], scales fp32 [slots, heads]."""
+    shape, strides = codes.shape, codes.stride()
+    assert len(shape) == 3 and strides[2] == 1, "expected codes [slots, heads, head_dim] with contiguous head_dim"
+    sr, sh = scales.stride() if scales.dim() == 2 else (0, 0)
+    assert scales.shape == shape[:2] and (sh == 1 or shape[1] == 1), "expected scales [slots, heads] with contiguous heads"
     if scales.dtype != torch.float32:
         raise TypeError("the scales of 8-bit rows are fp32")
-    return codes.shape[1], codes.shape[2], code_tag(codes)
+    # a single row's stride says nothing
+    return shape[0], shape[1], shape[2], code_tag(codes), strides[0], strides[1], sr if shape[0] > 1 else max(sr, shape[1])
 
 
-@torch.inference_mode()
 def destindex_copy_quantize_kv(K, DestLoc, Out, OutScale):
     """Out[DestLoc[i]], OutScale[DestLoc[i]] = K[i] in 8 bits: ``destindex_copy_kv`` into a pool of int8 or e4m3 codes with
     one fp32 scale per slot and head.
@@ -154,14 +156,16 @@ def destindex_copy_quantize_kv(K, DestLoc, Out, OutScale):
     amax / 448, code = e4m3(x * fl32(448 / amax)).  A head row with an infinity or a NaN gets codes 0 and scale NaN, and every
     reader of it sees NaN.  DestLoc must not name a slot twice (the slot would get parts of both rows); ids outside the pool
     are skipped and reported by ``device_status``."""
-    need_here(K, DestLoc, Out, OutScale)
-    heads, dim, _ = _rows(K)
-    h, d, code = _q8_pool(Out, OutScale)
-    assert (h, d) == (heads, dim) and DestLoc.is_contiguous() and DestLoc.dim() == 1 and DestLoc.shape[0] <= K.shape[0]
-    rc = _lib.attn().esp_kv_scatter_q8(K.data_ptr(), K.stride(0), K.stride(1), Out.data_ptr(), Out.stride(0), Out.stride(1),
-                                       OutScale.data_ptr(), OutScale.stride(0), DestLoc.data_ptr(), idx64_flag(DestLoc),
-                                       DestLoc.shape[0], heads, dim, dtype16_tag(K), code, Out.shape[0], stream_ptr())
-    _lib.check(rc, "esp_kv_scatter_q8")
+    dev = need_here(K, DestLoc, Out, OutScale)
+    slots, heads, dim, code, row, head, srow = _q8_pool(Out, OutScale)
+    shape, strides = K.shape, K.stride()
+    assert len(shape) == 3 and strides[2] == 1 and shape[1] == heads and shape[2] == dim
+    n = DestLoc.shape[0]
+    assert DestLoc.is_contiguous() and DestLoc.dim() == 1 and n <= shape[0]
+    rc = _lib.attn().esp_kv_scatter_q8(K.data_ptr(), strides[0], strides[1], Out.data_ptr(), row, head, OutScale.data_ptr(), srow,
+                                       DestLoc.data_ptr(), idx64_flag(DestLoc), n, heads, dim, dtype16_tag(K), code, slots, stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_kv_scatter_q8")
 
 
 @torch.inference_mode()
@@ -174,36 +178,35 @@ def destindex_copy_quantize_and_register_kv(batch_size, new_kv_cache_len, kv_ran
     need_i32(new_kv_cache_len, kv_range_begin, kv_range_end, kv_b_start_loc, cur_kv_cache_index, b_req_idx)
     assert new_kv_cache_len_sum.dtype == torch.int64 and new_kv_cache_len_sum.is_contiguous()
     heads, dim, _ = _rows(kv)
-    h, d, code = _q8_pool(total_kv_cache, total_kv_scale)
+    slots, h, d, code, row, head, srow = _q8_pool(total_kv_cache, total_kv_scale)
     assert (h, d) == (heads, dim)
     assert req_to_token_indexs.dtype == torch.int32 and req_to_token_indexs.stride(1) == 1 and mem_index.is_contiguous()
     rc = _lib.attn().esp_kv_scatter_register_q8(
         int(batch_size), ptr(new_kv_cache_len), ptr(kv_range_begin), ptr(kv_range_end), ptr(new_kv_cache_len_sum),
         ptr(kv), kv.stride(0), kv.stride(1), ptr(kv_b_start_loc), ptr(cur_kv_cache_index), ptr(mem_index),
-        idx64_flag(mem_index), ptr(total_kv_cache), total_kv_cache.stride(0), total_kv_cache.stride(1), ptr(total_kv_scale),
-        total_kv_scale.stride(0), ptr(req_to_token_indexs), req_to_token_indexs.stride(0), ptr(b_req_idx),
+        idx64_flag(mem_index), ptr(total_kv_cache), row, head, ptr(total_kv_scale), srow, ptr(req_to_token_indexs), req_to_token_indexs.stride(0), ptr(b_req_idx),
         int(num_used_mem_index), int(max_len_in_batch), 1 if should_register_kv else 0, heads, dim, dtype16_tag(kv), code,
-        total_kv_cache.shape[0], stream_ptr())
+        slots, stream_ptr())
     _lib.check(rc, "esp_kv_scatter_register_q8")
 
 
-@torch.inference_mode()
 def gather_dequantize_kv(Cache, CacheScale, SrcLoc, dtype=None, out=None):
     """out[i] = Cache[SrcLoc[i]] * CacheScale[SrcLoc[i]]: rows of a pool held in 8 bits as 16-bit (or fp32) rows.  ``out``
     [n, heads, head_dim] may be given instead of ``dtype``.  An id outside the pool gives a row of zeros and is reported by
     ``device_status``."""
-    need_here(Cache, CacheScale, SrcLoc, out)
-    heads, dim, code = _q8_pool(Cache, CacheScale)
+    dev = need_here(Cache, CacheScale, SrcLoc, out)
+    slots, heads, dim, code, row, head, srow = _q8_pool(Cache, CacheScale)
     assert SrcLoc.is_contiguous() and SrcLoc.dim() == 1
     n = SrcLoc.shape[0]
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=dtype or torch.bfloat16, device=Cache.device)
+        out = CacheScale.new_empty((n, heads, dim), dtype=dtype or torch.bfloat16)
     else:
-        assert out.dim() == 3 and out.shape == (n, heads, dim) and out.stride(2) == 1 and (dtype is None or dtype == out.dtype)
-    rc = _lib.attn().esp_kv_gather_q8(out.data_ptr(), out.stride(0), out.stride(1), Cache.data_ptr(), Cache.stride(0),
-                                      Cache.stride(1), CacheScale.data_ptr(), CacheScale.stride(0), SrcLoc.data_ptr(),
-                                      idx64_flag(SrcLoc), n, heads, dim, dtype_tag(out), code, Cache.shape[0], stream_ptr())
-    _lib.check(rc, "esp_kv_gather_q8")
+        assert out.shape == (n, heads, dim) and out.stride(2) == 1 and (dtype is None or dtype == out.dtype)
+    orow, ohead, _ = out.stride()
+    rc = _lib.attn().esp_kv_gather_q8(out.data_ptr(), orow, ohead, Cache.data_ptr(), row, head, CacheScale.data_ptr(), srow,
+                                      SrcLoc.data_ptr(), idx64_flag(SrcLoc), n, heads, dim, dtype_tag(out), code, slots, stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_kv_gather_q8")
     return out
 
 

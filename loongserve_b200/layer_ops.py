@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._util import dtype16_tag, dtype_tag, need_cuda, need_here, ptr, stream_ptr
+from ._util import dtype16_tag, dtype_tag, need_cuda, need_here, ptr, stream_of, stream_ptr
 
 
 @torch.inference_mode()
@@ -61,105 +61,126 @@ def ffn_block(input_embds, norm_weight, norm_eps: float, gate_up_proj, down_proj
 # ---------------------------------------------------------------------------------------- 8-bit rows
 # A row of int8 codes has one fp32 scale: scale = max(max|y|, 2^-100) / 127, code = rint(y * fl32(127 / max|y|)).  A row with an
 # infinity or a NaN gets codes 0 and scale NaN.
-def _rows_out(codes, scale, rows, cols, device):
+# (These wrappers stand in front of launches of a few microseconds: shapes are read once, and nothing is wrapped in a mode.)
+def _rows_out(like, codes, scale, rows, cols):
     if codes is None:
-        codes = torch.empty((rows, cols), dtype=torch.int8, device=device)
+        codes = like.new_empty((rows, cols), dtype=torch.int8)
+    else:
+        assert codes.shape == (rows, cols) and codes.dtype == torch.int8 and codes.is_contiguous()
     if scale is None:
-        scale = torch.empty((rows,), dtype=torch.float32, device=device)
-    assert codes.shape == (rows, cols) and codes.dtype == torch.int8 and codes.is_contiguous()
-    assert scale.shape == (rows,) and scale.dtype == torch.float32 and scale.is_contiguous()
+        scale = like.new_empty(rows, dtype=torch.float32)
+    else:
+        assert scale.shape == (rows,) and scale.dtype == torch.float32 and scale.is_contiguous()
     return codes, scale
 
 
 def _norm_args(input, residual, weight):
-    assert input.dim() == 2 and weight.dim() == 1 and input.size(1) == weight.size(0)
+    """(tokens, hidden, dtype tag) of a norm's arguments."""
+    shape = input.shape
+    tokens, hidden = shape if len(shape) == 2 else (0, -1)
+    assert hidden >= 0 and weight.shape == (hidden,), "expected input [tokens, hidden] and weight [hidden]"
     assert input.is_contiguous() and weight.is_contiguous() and weight.dtype == input.dtype
     if residual is not None:
-        assert residual.shape == input.shape and residual.dtype == input.dtype and residual.is_contiguous()
+        assert residual.shape == shape and residual.dtype == input.dtype and residual.is_contiguous()
+    return tokens, hidden, dtype16_tag(input)
 
 
-@torch.inference_mode()
 def add_rms_norm(input: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float, out=None) -> torch.Tensor:
     """residual += input (in place), and the RMSNorm of the sum.  The norm is taken of the fp32 sum before it is rounded into
     ``residual``; the output is rounded once."""
-    need_here(input, residual, weight, out)
-    _norm_args(input, residual, weight)
-    output = torch.empty_like(input) if out is None else out
-    assert output.shape == input.shape and output.dtype == input.dtype and output.is_contiguous()
-    rc = _lib.attn().esp_add_rms_norm(output.data_ptr(), residual.data_ptr(), input.data_ptr(), weight.data_ptr(), input.size(0),
-                                      input.size(1), float(eps), dtype16_tag(input), stream_ptr())
-    _lib.check(rc, "esp_add_rms_norm")
-    return output
+    dev = need_here(input, residual, weight, out)
+    tokens, hidden, tag = _norm_args(input, residual, weight)
+    if out is None:
+        out = torch.empty_like(input)
+    else:
+        assert out.shape == input.shape and out.dtype == input.dtype and out.is_contiguous()
+    rc = _lib.attn().esp_add_rms_norm(out.data_ptr(), residual.data_ptr(), input.data_ptr(), weight.data_ptr(), tokens, hidden, eps, tag,
+                                      stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_add_rms_norm")
+    return out
 
 
-@torch.inference_mode()
 def add_rms_norm_quant(input: torch.Tensor, residual, weight: torch.Tensor, eps: float, out=None, out_scale=None):
     """``add_rms_norm`` whose output is int8 rows: (codes [tokens, hidden], scale [tokens]).  ``residual`` None: the norm of
     ``input`` alone."""
-    need_here(input, residual, weight, out, out_scale)
-    _norm_args(input, residual, weight)
-    tokens, hidden = input.shape
-    codes, scale = _rows_out(out, out_scale, tokens, hidden, input.device)
+    dev = need_here(input, residual, weight, out, out_scale)
+    tokens, hidden, tag = _norm_args(input, residual, weight)
+    codes, scale = _rows_out(input, out, out_scale, tokens, hidden)
     rc = _lib.attn().esp_add_rms_norm_q8(codes.data_ptr(), scale.data_ptr(), ptr(residual), input.data_ptr(), weight.data_ptr(), tokens,
-                                         hidden, float(eps), dtype16_tag(input), stream_ptr())
-    _lib.check(rc, "esp_add_rms_norm_q8")
+                                         hidden, eps, tag, stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_add_rms_norm_q8")
     return codes, scale
 
 
-@torch.inference_mode()
 def silu_and_mul_quant(io: torch.Tensor, out=None, out_scale=None):
     """int8 rows of silu(io[:, :F]) * io[:, F:]: (codes [tokens, F], scale [tokens]).  ``io`` is left as it was."""
-    need_here(io, out, out_scale)
-    assert io.dim() == 2 and io.is_contiguous() and io.size(1) % 2 == 0
-    tokens, ffn = io.size(0), io.size(1) // 2
-    codes, scale = _rows_out(out, out_scale, tokens, ffn, io.device)
-    rc = _lib.attn().esp_silu_and_mul_q8(codes.data_ptr(), scale.data_ptr(), io.data_ptr(), tokens, ffn, dtype16_tag(io), stream_ptr())
-    _lib.check(rc, "esp_silu_and_mul_q8")
+    dev = need_here(io, out, out_scale)
+    shape = io.shape
+    assert len(shape) == 2 and shape[1] % 2 == 0 and io.is_contiguous()
+    tokens, ffn = shape[0], shape[1] // 2
+    tag = dtype16_tag(io)
+    codes, scale = _rows_out(io, out, out_scale, tokens, ffn)
+    rc = _lib.attn().esp_silu_and_mul_q8(codes.data_ptr(), scale.data_ptr(), io.data_ptr(), tokens, ffn, tag, stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_silu_and_mul_q8")
     return codes, scale
 
 
-@torch.inference_mode()
 def quantize_rows(x: torch.Tensor, out=None, out_scale=None):
     """int8 rows of x [rows, cols]: (codes, scale [rows]).  Also lays out weights for ``mm_w8a8``: ``quantize_rows(w.t().contiguous())``
     of a [in, out] weight gives its output channels as rows."""
-    need_here(x, out, out_scale)
-    assert x.dim() == 2 and x.stride(1) == 1
-    codes, scale = _rows_out(out, out_scale, x.size(0), x.size(1), x.device)
-    rc = _lib.attn().esp_quantize_rows(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), x.stride(0), x.size(0), x.size(1), dtype16_tag(x),
-                                       stream_ptr())
-    _lib.check(rc, "esp_quantize_rows")
+    dev = need_here(x, out, out_scale)
+    shape = x.shape
+    assert len(shape) == 2 and x.stride(1) == 1
+    rows, cols = shape
+    tag = dtype16_tag(x)
+    codes, scale = _rows_out(x, out, out_scale, rows, cols)
+    rc = _lib.attn().esp_quantize_rows(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), x.stride(0) if rows > 1 else cols, rows, cols, tag,
+                                       stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_quantize_rows")
     return codes, scale
 
 
-@torch.inference_mode()
 def dequantize_rows(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat16, out=None) -> torch.Tensor:
     """codes * scale per row, rounded to ``dtype``."""
-    need_here(codes, scale, out)
-    assert codes.dim() == 2 and codes.dtype == torch.int8 and codes.is_contiguous()
-    assert scale.shape == (codes.size(0),) and scale.dtype == torch.float32 and scale.is_contiguous()
-    o = torch.empty(codes.shape, dtype=dtype, device=codes.device) if out is None else out
-    assert o.shape == codes.shape and o.is_contiguous()
-    rc = _lib.attn().esp_dequantize_rows(o.data_ptr(), codes.data_ptr(), scale.data_ptr(), codes.size(0), codes.size(1), dtype_tag(o),
-                                         stream_ptr())
-    _lib.check(rc, "esp_dequantize_rows")
-    return o
+    dev = need_here(codes, scale, out)
+    shape = codes.shape
+    assert len(shape) == 2 and codes.dtype == torch.int8 and codes.is_contiguous()
+    assert scale.shape == shape[:1] and scale.dtype == torch.float32 and scale.is_contiguous()
+    if out is None:
+        out = torch.empty_like(codes, dtype=dtype)
+    else:
+        assert out.shape == shape and out.is_contiguous()
+    rc = _lib.attn().esp_dequantize_rows(out.data_ptr(), codes.data_ptr(), scale.data_ptr(), shape[0], shape[1], dtype_tag(out), stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_dequantize_rows")
+    return out
 
 
-@torch.inference_mode()
 def mm_w8a8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype=torch.bfloat16, out=None):
     """(a @ w.T) * a_scale[:, None] * w_scale[None]: int8 rows of tokens [M, K] and of output channels [N, K], exact integer sums,
     one rounding to the output type.  K a multiple of 16, at most 131071."""
-    need_here(a, a_scale, w, w_scale, out)
-    assert a.dim() == 2 and w.dim() == 2 and a.size(1) == w.size(1)
+    dev = need_here(a, a_scale, w, w_scale, out)
+    sa, sw = a.shape, w.shape
+    assert len(sa) == 2 and len(sw) == 2 and sa[1] == sw[1]
     if a.dtype != torch.int8 or w.dtype != torch.int8 or a_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
         raise TypeError("mm_w8a8 takes int8 codes and fp32 scales")
-    m, k = a.shape
-    n = w.size(0)
-    assert a.stride(1) == 1 and w.stride(1) == 1
+    (m, k), n = sa, sw[0]
+    (la, ca), (lw, cw) = a.stride(), w.stride()
+    assert ca == 1 and cw == 1
     assert a_scale.shape == (m,) and w_scale.shape == (n,) and a_scale.is_contiguous() and w_scale.is_contiguous()
-    o = torch.empty((m, n), dtype=out_dtype, device=a.device) if out is None else out
-    assert o.shape == (m, n) and (n == 1 or o.stride(1) == 1)
-    rc = _lib.attn().esp_mm_w8a8(o.data_ptr(), o.stride(0), a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0),
-                                 w_scale.data_ptr(), m, n, k, dtype_tag(o), stream_ptr())
-    _lib.check(rc, "esp_mm_w8a8")
-    return o
+    if out is None:
+        out = a_scale.new_empty((m, n), dtype=out_dtype)
+        lo = n
+    else:
+        assert out.shape == (m, n) and (n == 1 or out.stride(1) == 1)
+        lo = out.stride(0) if m > 1 else n
+    # a single row's stride says nothing
+    rc = _lib.attn().esp_mm_w8a8(out.data_ptr(), lo, a.data_ptr(), la if m > 1 else k, a_scale.data_ptr(), w.data_ptr(),
+                                 lw if n > 1 else k, w_scale.data_ptr(), m, n, k, dtype_tag(out), stream_of(dev))
+    if rc:
+        _lib.check(rc, "esp_mm_w8a8")
+    return out

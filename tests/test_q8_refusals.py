@@ -132,7 +132,7 @@ class _On:
 
 def test_tensors_of_another_device_are_refused(monkeypatch):
     from loongserve_b200 import _util
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(_util, "current_device", lambda: 0)
     _util.need_here(_On(0), None, _On(0))
     with pytest.raises(RuntimeError, match="current CUDA device"):
         _util.need_here(_On(0), _On(1))
@@ -146,7 +146,7 @@ def no_device_check(monkeypatch):
     from loongserve_b200 import flash_decoding, kv_ops, layer_ops
     for mod in (flash_decoding, kv_ops, layer_ops):
         monkeypatch.setattr(mod, "need_here", lambda *a: None)
-        monkeypatch.setattr(mod, "stream_ptr", lambda: 0)
+        monkeypatch.setattr(mod, "stream_of", lambda device: 0)
 
     class Refuse:
         def __getattr__(self, name):
