@@ -213,18 +213,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
                 __syncwarp();
                 const int64_t nleft = p.N - n0 - c0;
                 const int ncols = nleft < kCols ? (int)nleft : kCols;
-                if (p.vec_out && ncols == kCols) {
+                if (p.vec_out) {
+                    const int c16 = (lane & 7) * Pack16<OT>::n;             // 4 rows of 128 bytes per step, 16 bytes per lane
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {               // 4 rows of 128 bytes per step
+                    for (int i = 0; i < 8; ++i) {
                         const int rr = i * 4 + (lane >> 3);
-                        if (rr < rows)
-                            *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + (row0 + rr) * p.ldo + n0 + c0) + (lane & 7) * 16) =
-                                *reinterpret_cast<const uint4*>(stage + rr * kEpiRowBytes + (lane & 7) * 16);
+                        if (rr >= rows || c16 >= ncols) continue;
+                        const uint8_t* from = stage + rr * kEpiRowBytes + (lane & 7) * 16;
+                        OT* to = out + (row0 + rr) * p.ldo + n0 + c0 + c16;
+                        if (c16 + Pack16<OT>::n <= ncols) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+                        else
+                            for (int j = 0; j < ncols - c16; ++j) to[j] = reinterpret_cast<const OT*>(from)[j];
                     }
                 } else {
-                    for (int rr = 0; rr < rows; ++rr)
-                        for (int i = lane; i < ncols; i += 32)
+                    for (int i = lane; i < ncols; i += 32) {
+#pragma unroll 8
+                        for (int rr = 0; rr < rows; ++rr)
                             out[(row0 + rr) * p.ldo + n0 + c0 + i] = *reinterpret_cast<const OT*>(stage + rr * kEpiRowBytes + i * sizeof(OT));
+                    }
                 }
                 __syncwarp();
             }
@@ -470,25 +476,36 @@ template <typename OT>
 static int launch_mm(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw, int64_t k, MmArgs g, cudaStream_t s) {
     g.kstages = (int)((k + kBK - 1) / kBK);
     g.vec_out = ((uintptr_t)g.out % 16 == 0 && (g.ldo * (int64_t)sizeof(OT)) % 16 == 0) ? 1 : 0;
-    // K is split over as many CTAs (a power of two: other clusters leave SMs of a GPC unused) as two per SM can run at once, as
-    // long as each keeps four stages.
-    auto splits_of = [&](int64_t tiles) {
-        int s = 8;
-        while (s > 1 && (tiles * s > 2 * kNumSMs || g.kstages < 4 * s)) s /= 2;
-        return s;
-    };
-    const int64_t nt = (g.N + 127) / 128, mt = (g.M + 127) / 128;
-    if (g.M <= 16) return launch_skinny<OT, 16>(a, lda, w, ldw, k, g, splits_of(nt), s);
-    if (g.M <= 32) return launch_skinny<OT, 32>(a, lda, w, ldw, k, g, splits_of(nt), s);
-    if (g.M <= 64) return launch_skinny<OT, 64>(a, lda, w, ldw, k, g, splits_of(nt), s);
-    // Up to 256 tokens the pairs have too few tiles when the channels are few: 256 x 4096 x 11008 takes 20.1 us in four splits
-    // and 31.0 us on pairs; with more channels (256 x 22016 x 4096) 54.3 us and 29.7 us.
-    if (g.M <= 256 && splits_of(nt * mt) >= 4) return launch_skinny<OT, 128>(a, lda, w, ldw, k, g, splits_of(nt * mt), s);
-    // Tiles of 128 channels cost about 0.6 of those of 256: taken where they fill the last wave of pairs better.
-    const int64_t m2 = (g.M + 255) / 256, pairs = kNumSMs / 2;
-    const int64_t w256 = (m2 * ((g.N + 255) / 256) + pairs - 1) / pairs, w128 = (m2 * nt + pairs - 1) / pairs;
-    if (6 * w128 < 10 * w256) return launch_pair<OT, 128>(a, lda, w, ldw, k, g, s);
-    return launch_pair<OT, 256>(a, lda, w, ldw, k, g, s);
+    // The variant with the least estimated time (us).  A skinny CTA costs about 6 us around its stages; a stage costs less while
+    // every SM has one CTA than with two (which then share the SM's intake).  A pair costs 5.4 or 6.5 us and 0.29 or 0.31 us per
+    // stage and wave of tiles.  Measured against these estimates (B200, tokens x channels x K, us):
+    //   64 x 4096 x 11008: TN 64 in 8 splits 13.8, 4 splits 15.2, 1 split 29.2, pairs 31.0      256 x 4096 x 11008: TN 128 in 4 splits 20.1, pairs 31.0
+    //   256 x 22016 x 4096: TN 64 50.8, TN 128 54.3, pairs of 256 29.7                          512 x 4096 x 1280: TN 64 12.9, pairs of 128 8.3, of 256 9.6
+    //   600 x 600 x 8000: TN 64 in 4 splits 12.4, TN 128 in 8 splits 12.5, pairs of 128 24.6    400 x 8000 x 2992: pairs of 256 17.2, of 128 21.0, TN 128 36.7
+    // Splits are powers of two: clusters of other sizes leave SMs of a GPC unused (64 x 12288 x 4096: 25.3 us in 3 splits, 17.7 in 2).
+    const int64_t nt = (g.N + 127) / 128, m2 = (g.M + 255) / 256, pairs = kNumSMs / 2;
+    const int ks = g.kstages;
+    auto waves = [](int64_t n, int64_t per) { return (double)((n + per - 1) / per); };
+    const double pair256 = 6.5 + waves(m2 * ((g.N + 255) / 256), pairs) * ks * 0.31, pair128 = 5.4 + waves(m2 * nt, pairs) * ks * 0.29;
+    double best = pair256 < pair128 ? pair256 : pair128;
+    int tn = 0, splits = 1;
+    const int tn_first = g.M <= 16 ? 16 : (g.M <= 32 ? 32 : 64), tn_last = g.M <= 64 ? tn_first : 128;
+    if (g.M <= 4096)
+        for (int t = tn_first; t <= tn_last; t *= 2)
+            for (int sp = 1; sp <= 8 && sp <= ks; sp *= 2) {
+                const int64_t ctas = nt * ((g.M + t - 1) / t) * sp;
+                const double one = t <= 32 ? 0.26 : (t == 64 ? 0.33 : 0.45), two = t <= 32 ? 0.50 : (t == 64 ? 0.62 : 0.75);
+                const double est = waves(ctas, 2 * kNumSMs) * (6.0 + (ks + sp - 1) / sp * (ctas <= kNumSMs ? one : two));
+                if (est < best) { best = est; tn = t; splits = sp; }
+            }
+    switch (tn) {
+        case 16: return launch_skinny<OT, 16>(a, lda, w, ldw, k, g, splits, s);
+        case 32: return launch_skinny<OT, 32>(a, lda, w, ldw, k, g, splits, s);
+        case 64: return launch_skinny<OT, 64>(a, lda, w, ldw, k, g, splits, s);
+        case 128: return launch_skinny<OT, 128>(a, lda, w, ldw, k, g, splits, s);
+        default: break;
+    }
+    return pair256 <= pair128 ? launch_pair<OT, 256>(a, lda, w, ldw, k, g, s) : launch_pair<OT, 128>(a, lda, w, ldw, k, g, s);
 }
 
 int mm_w8a8_status(int32_t out[4], int32_t clear) {
