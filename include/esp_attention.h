@@ -391,7 +391,7 @@ int esp_silu_and_mul_inplace(void* io, int64_t tokens, int32_t ffn_inter_dim, in
  *
  * KV pool in 8 bits.  Per slot and head: head_dim codes and one fp32 scale (slots are handed out token by token, so the
  * scale belongs to one token and head).  codes: strides in bytes, multiples of 16, base 16-byte aligned; scales: the heads of
- * a slot are next to each other, `scales_row_stride` fp32 elements between slots.  head_dim a multiple of 16, at most 512
+ * a slot are next to each other, `scales_row_stride` fp32 elements between slots.  head_dim a multiple of 16, at most 256
  * (esp_decode_stage1_q8: 128).  Slot ids outside [0, pool_rows) are skipped and reported by esp_kv_device_status; unlike
  * the 16-bit entry points pool_rows must be given.  A slot that `dest` names twice ends up with parts of both rows. */
 

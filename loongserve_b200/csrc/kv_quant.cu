@@ -4,9 +4,10 @@
 // slots are handed out token by token, so tokens of different requests may be neighbours and a scale over several slots
 // would have to be revised by every later write.
 //
-// HBM bound.  Per head row of D: write reads 2*D and stores D + 4 bytes, read-back the other way round.  LPR lanes share a
-// head row, 16 elements each: two 16-byte loads, one 16-byte store of codes; the row's maximum is a shuffle reduction over
-// its lanes, so the data is read once and stays in registers.
+// HBM bound.  Per head row of D: write reads 2*D and stores D + 4 bytes, read-back the other way round.  Writing, LPR lanes share a
+// head row with 16 elements each: two 16-byte loads, the row's maximum by shuffles over its lanes, a 16-byte store of codes; the
+// data is read once and stays in registers.  A lane group's token and head come from shifts, not from a division of the row
+// number: with the division, and with 8 elements per lane, the instructions were the bound (16384 tokens x 64 heads: 82 and 108 us).
 #include "quant_common.cuh"
 
 namespace esp {
@@ -35,22 +36,28 @@ struct PoolQ8 {
     int64_t rows;
 };
 
-// One head row: LPR lanes, 16 elements each (lanes at or beyond D/16 idle).  All lanes of the warp call it.
+// One head row: LPR lanes, 16 elements each (lanes at or beyond D/16 idle).  Loading and storing are apart, so that a lane group has
+// several rows' loads in flight.  All lanes of the warp call both.
+struct HeadRow { uint4 a, b; };
+template <typename T>
+__device__ __forceinline__ HeadRow load_head_row(const T* src, int lane_in_row, bool mine) {
+    HeadRow h{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (mine) {
+        h.a = ld_nc_v4_keep(src + lane_in_row * 16);
+        h.b = ld_nc_v4_keep(src + lane_in_row * 16 + 8);
+    }
+    return h;
+}
 template <typename T, int CODE, int LPR>
-__device__ __forceinline__ void quantise_head_row(const T* src, uint8_t* codes, float* scale, int lane_in_row, int lanes_used, bool on) {
+__device__ __forceinline__ void store_head_row(const HeadRow& h, uint8_t* codes, float* scale, int lane_in_row, bool mine) {
     float x[16];
     uint32_t amax = 0;
-    const bool mine = on && lane_in_row < lanes_used;
-    if (mine) {
-        const uint4 a = *reinterpret_cast<const uint4*>(src + lane_in_row * 16);
-        const uint4 b = *reinterpret_cast<const uint4*>(src + lane_in_row * 16 + 8);
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const uint32_t w[8] = {h.a.x, h.a.y, h.a.z, h.a.w, h.b.x, h.b.y, h.b.z, h.b.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 f = Cvt<T>::to_f2(w[i]);
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
-            amax = max(amax, max(abs_bits(f.x), abs_bits(f.y)));
-        }
+    for (int i = 0; i < 8; ++i) {
+        const float2 f = Cvt<T>::to_f2(w[i]);
+        x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        amax = max(amax, max(abs_bits(f.x), abs_bits(f.y)));
     }
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -66,24 +73,40 @@ __device__ __forceinline__ void quantise_head_row(const T* src, uint8_t* codes, 
 }
 
 constexpr int kQ8Threads = 256;
+constexpr int kQ8Rows = 2;             // rows of a lane group in flight
 
-// Head rows (token, head) are spread over the grid; consecutive lane groups take consecutive heads of a token.
+// A pass of a CTA: kQ8Rows times (kQ8Threads / LPR) >> hshift tokens x 1 << hshift heads (hshift: the power of two that covers
+// heads2, as far as the CTA's lane groups reach); more heads are further passes over the same tokens.
 template <typename T, int CODE, int LPR>
 __global__ void __launch_bounds__(kQ8Threads) kv_scatter_q8_kernel(const T* __restrict__ src, int64_t src_row, int64_t src_head,
                                                                    PoolQ8 p, const void* __restrict__ dest, int idx64, int64_t n,
-                                                                   int heads2, int lanes_used) {
-    constexpr int kRowsPerCta = kQ8Threads / LPR;
+                                                                   int heads2, int hshift, int lanes_used) {
     const int sub = threadIdx.x / LPR, lane_in_row = threadIdx.x % LPR;
-    const int64_t total = n * heads2;
-    for (int64_t base = (int64_t)blockIdx.x * kRowsPerCta; base < total; base += (int64_t)gridDim.x * kRowsPerCta) {
-        const int64_t r = base + sub;
-        bool on = r < total;
-        const int64_t t = on ? r / heads2 : 0;
-        const int h = on ? (int)(r - t * heads2) : 0;
-        const int64_t slot = on ? idx_at(dest, idx64, t) : 0;
-        on = on && q8_slot_ok(slot, p.rows, 5, t);
-        quantise_head_row<T, CODE, LPR>(src + t * src_row + (int64_t)h * src_head, p.codes + slot * p.row_b + (int64_t)h * p.head_b,
-                                        p.scales + slot * p.scale_row + h, lane_in_row, lanes_used, on);
+    const int tokens = (kQ8Threads / LPR) >> hshift, h0 = sub & ((1 << hshift) - 1);
+    for (int64_t base = (int64_t)blockIdx.x * tokens * kQ8Rows; base < n; base += (int64_t)gridDim.x * tokens * kQ8Rows) {
+        int64_t t[kQ8Rows], slot[kQ8Rows];
+        bool on[kQ8Rows];
+#pragma unroll
+        for (int u = 0; u < kQ8Rows; ++u) {
+            t[u] = base + u * tokens + (sub >> hshift);
+            on[u] = t[u] < n;
+            slot[u] = on[u] ? idx_at(dest, idx64, t[u]) : 0;
+        }
+        for (int h = h0; h < heads2 + h0; h += 1 << hshift) {           // the same number of turns for every lane
+            HeadRow row[kQ8Rows];
+            const bool head_on = h < heads2 && lane_in_row < lanes_used;
+#pragma unroll
+            for (int u = 0; u < kQ8Rows; ++u)
+                row[u] = load_head_row<T>(src + t[u] * src_row + (int64_t)h * src_head, lane_in_row, on[u] && head_on);
+            if (h == h0) {
+#pragma unroll
+                for (int u = 0; u < kQ8Rows; ++u) on[u] = on[u] && q8_slot_ok(slot[u], p.rows, 5, t[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kQ8Rows; ++u)
+                store_head_row<T, CODE, LPR>(row[u], p.codes + slot[u] * p.row_b + (int64_t)h * p.head_b, p.scales + slot[u] * p.scale_row + h,
+                                             lane_in_row, on[u] && head_on);
+        }
     }
 }
 
@@ -95,7 +118,7 @@ __global__ void __launch_bounds__(kQ8Threads) kv_scatter_register_q8_kernel(
     const int64_t* __restrict__ new_len_cumsum, const T* __restrict__ kv, int64_t kv_row, int64_t kv_head,
     const int32_t* __restrict__ kv_b_start_loc, const int32_t* __restrict__ cur_kv_cache_index, const void* __restrict__ mem_index,
     int idx64, PoolQ8 p, int32_t* __restrict__ req_to_token, int64_t rtt_stride, const int32_t* __restrict__ b_req_idx,
-    int64_t num_used, int row_cap, int should_register, int heads2, int lanes_used) {
+    int64_t num_used, int row_cap, int should_register, int heads2, int hshift, int lanes_used) {
     const int b = blockIdx.y;
     int n_new = new_len[b];
     const int rb = range_begin[b], re = range_end[b];
@@ -107,17 +130,21 @@ __global__ void __launch_bounds__(kQ8Threads) kv_scatter_register_q8_kernel(
     if (should_register) rtt = req_to_token + (int64_t)b_req_idx[b] * rtt_stride + cur_kv_cache_index[b];
     constexpr int kRowsPerCta = kQ8Threads / LPR;
     const int sub = threadIdx.x / LPR, lane_in_row = threadIdx.x % LPR;
-    const int64_t total = (int64_t)n_new * heads2;
-    for (int64_t base = (int64_t)blockIdx.x * kRowsPerCta; base < total; base += (int64_t)gridDim.x * kRowsPerCta) {
-        const int64_t r = base + sub;
-        bool on = r < total;
-        const int64_t t = on ? r / heads2 : 0;
-        const int h = on ? (int)(r - t * heads2) : 0;
-        const int64_t slot = on ? idx_at(mem_index, idx64, base0 + t) : 0;
-        on = on && q8_slot_ok(slot, p.rows, 6, base0 + t);
-        quantise_head_row<T, CODE, LPR>(kv + (src0 + t) * kv_row + (int64_t)h * kv_head, p.codes + slot * p.row_b + (int64_t)h * p.head_b,
-                                        p.scales + slot * p.scale_row + h, lane_in_row, lanes_used, on);
-        if (on && should_register && h == 0 && lane_in_row == 0) rtt[t] = (int32_t)slot;
+    const int tokens = kRowsPerCta >> hshift, h0 = sub & ((1 << hshift) - 1);
+    for (int t0 = blockIdx.x * tokens + (sub >> hshift); ; t0 += gridDim.x * tokens) {
+        if (!__syncthreads_or(t0 < n_new)) return;
+        const bool on = t0 < n_new;
+        const int64_t slot = on ? idx_at(mem_index, idx64, base0 + t0) : 0;
+        const T* from = kv + (src0 + (on ? t0 : 0)) * kv_row;
+        const bool ok = on && q8_slot_ok(slot, p.rows, 6, base0 + t0);
+        for (int hb = 0; hb < heads2; hb += 1 << hshift) {
+            const int h = hb + h0;
+            const bool mine = ok && h < heads2 && lane_in_row < lanes_used;
+            const HeadRow row = load_head_row<T>(from + (int64_t)h * kv_head, lane_in_row, mine);
+            store_head_row<T, CODE, LPR>(row, p.codes + slot * p.row_b + (int64_t)h * p.head_b, p.scales + slot * p.scale_row + h,
+                                         lane_in_row, mine);
+        }
+        if (ok && should_register && h0 == 0 && lane_in_row == 0) rtt[t0] = (int32_t)slot;
     }
 }
 
@@ -181,7 +208,7 @@ static int check_pool_q8(const void* codes, int64_t row, int64_t head, const voi
                          int32_t head_dim, int32_t code, int64_t pool_rows) {
     if (!codes || !scales || heads2 <= 0 || head_dim <= 0 || pool_rows <= 0) return ESP_ERR_BAD_ARG;
     if (code != ESP_CODE_INT8 && code != ESP_CODE_E4M3) return ESP_ERR_BAD_ARG;
-    if (head_dim > 512) return ESP_ERR_UNSUPPORTED;
+    if (head_dim > 256) return ESP_ERR_UNSUPPORTED;
     if (head_dim % 16 || row % 16 || head % 16 || !aligned16(codes)) return ESP_ERR_ALIGNMENT;
     if (scale_row < heads2 || ((uintptr_t)scales & 3u)) return ESP_ERR_BAD_ARG;
     return ESP_OK;
@@ -192,6 +219,13 @@ static int lanes_per_row(int head_dim) {
     int l = 1;
     while (l * 16 < head_dim) l *= 2;
     return l;
+}
+
+// log2 of the heads of a pass: the power of two that covers them, within the lane groups of a CTA
+static int head_shift(int heads2, int lpr) {
+    int h = 0;
+    while ((1 << h) < heads2 && (1 << h) < kQ8Threads / lpr) ++h;
+    return h;
 }
 
 static unsigned q8_grid(int64_t head_rows, int rows_per_cta) {
@@ -211,8 +245,9 @@ int kv_q8_status(int32_t out[4], int32_t clear) {
 template <typename T, int CODE, int LPR>
 static int launch_scatter_q8(const void* src, int64_t sr, int64_t sh, const PoolQ8& p, const void* dest, int idx64, int64_t n, int heads2,
                              int lanes_used, cudaStream_t s) {
-    kv_scatter_q8_kernel<T, CODE, LPR><<<q8_grid(n * heads2, kQ8Threads / LPR), kQ8Threads, 0, s>>>((const T*)src, sr, sh, p, dest, idx64, n,
-                                                                                                    heads2, lanes_used);
+    const int hshift = head_shift(heads2, LPR);
+    kv_scatter_q8_kernel<T, CODE, LPR><<<q8_grid(n, kQ8Rows * ((kQ8Threads / LPR) >> hshift)), kQ8Threads, 0, s>>>((const T*)src, sr, sh, p, dest, idx64, n, heads2,
+                                                                                                      hshift, lanes_used);
     ESP_LAUNCH_CHECK("kv_scatter_q8_kernel");
     return ESP_OK;
 }
@@ -225,7 +260,7 @@ template <typename T, int CODE, int LPR>
 static int launch_register_q8(const RegisterArgs& a, const void* kv, int64_t kr, int64_t kh, const PoolQ8& p, int heads2, int lanes_used, cudaStream_t s) {
     kv_scatter_register_q8_kernel<T, CODE, LPR><<<a.grid, kQ8Threads, 0, s>>>(
         a.new_len, a.range_begin, a.range_end, a.cumsum, (const T*)kv, kr, kh, a.start_loc, a.cur, a.mem_index, a.idx64, p, a.rtt, a.rtt_stride,
-        a.b_req_idx, a.num_used, a.row_cap, a.should_register, heads2, lanes_used);
+        a.b_req_idx, a.num_used, a.row_cap, a.should_register, heads2, head_shift(heads2, LPR), lanes_used);
     ESP_LAUNCH_CHECK("kv_scatter_register_q8_kernel");
     return ESP_OK;
 }
@@ -238,7 +273,7 @@ using namespace esp;
 #define ESP_Q8_LANES(CALL, T, CODE, LPR_)                                                                                        \
     switch (LPR_) {                                                                                                              \
         case 1: return CALL(T, CODE, 1); case 2: return CALL(T, CODE, 2); case 4: return CALL(T, CODE, 4);                        \
-        case 8: return CALL(T, CODE, 8); case 16: return CALL(T, CODE, 16); default: return CALL(T, CODE, 32);                    \
+        case 8: return CALL(T, CODE, 8); default: return CALL(T, CODE, 16);                    \
     }
 #define ESP_Q8_DISPATCH(CALL, dtype, code, LPR_)                                                                                 \
     if (dtype == ESP_DTYPE_F16) {                                                                                                \
@@ -285,7 +320,7 @@ extern "C" int esp_kv_scatter_register_q8(
                    req_to_token_stride, b_req_idx, num_used_mem_index, ((max_len_in_batch + 255) / 256) * 256, should_register, dim3(1)};
     // the 16-bit form's row cap: rows past max_len_in_batch rounded up to 256 are not copied
     const int64_t per = ((int64_t)kNumSMs * 32 + batch - 1) / batch;
-    int64_t gx = q8_grid((int64_t)max_len_in_batch * heads2, kQ8Threads / lpr);
+    int64_t gx = q8_grid(max_len_in_batch, (kQ8Threads / lpr) >> head_shift(heads2, lpr));
     a.grid = dim3((unsigned)(gx < per ? gx : per), batch);
     cudaStream_t s = (cudaStream_t)stream;
 #define ESP_CALL(T, CODE, LPR) launch_register_q8<T, CODE, LPR>(a, kv, kv_row_stride, kv_head_stride, p, heads2, head_dim / 16, s)

@@ -7,7 +7,9 @@
 // The norm is taken of the unrounded sum, so the output is rounded once; what is kept for the next layer is the rounded one.
 //
 // HBM bound: every element is read once, held in registers in fp32 (up to 8 * VPT per thread) across the row's reduction,
-// and written once.  One CTA per row; the sum of squares and the maximum go through one shuffle + shared-memory reduction.
+// and written once.  Rows of up to 512 elements: a warp per row, eight rows to a CTA (60000 rows of 256: a CTA of one warp per row
+// took 33 us, this form 9-20 us).  Wider rows: a CTA per row; CTAs walk over the rows and load the next one before they reduce the
+// one in hand, which keeps copies in flight through the reduction (norm into codes, 16384 x 4096: 44.9 -> 37 us).
 #include "quant_common.cuh"
 
 namespace esp {
@@ -20,120 +22,171 @@ struct RowArgs {
     void* out; int8_t* codes; float* scale;                  // one of out / codes
     int nvec;                                                // cols / 8
     float eps, inv_cols;
+    int64_t rows;
 };
 
-template <typename T, int MODE, int VPT, bool QUANT>
-__global__ void __launch_bounds__(1024) row_kernel(RowArgs a) {
-    const int64_t row = blockIdx.x;
-    const int nt = blockDim.x;
-    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.in) + row * a.in_stride);
-    uint4* res = MODE == ROW_ADD_NORM ? reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.residual) + row * (int64_t)a.nvec * 8) : nullptr;
-    const uint4* wv = reinterpret_cast<const uint4*>(a.weight);
+template <int VPT> struct RowData { uint4 a[VPT], b[VPT]; };
+
+// nt threads share a row: a warp (WARP) or the CTA
+template <typename T, int MODE, int VPT, bool QUANT, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : (VPT == 2 ? 512 : (VPT == 4 ? 512 : 1024))) row_kernel(RowArgs a) {
     constexpr bool kNorm = MODE == ROW_ADD_NORM || MODE == ROW_NORM;
-    float t[VPT][8];
-    uint4 v0[VPT], v1[VPT];
-#pragma unroll
-    for (int c = 0; c < VPT; ++c) {
-        const int i = threadIdx.x + c * nt;
-        if (i < a.nvec) {
-            v0[c] = src[i];
-            if (MODE == ROW_ADD_NORM) v1[c] = res[i];
-            if (MODE == ROW_SILU) v1[c] = src[a.nvec + i];
-        }
-    }
-    float ss = 0.f;
-    uint32_t amax = 0;
-#pragma unroll
-    for (int c = 0; c < VPT; ++c) {
-        const int i = threadIdx.x + c * nt;
-        if (i < a.nvec) {
-            const uint32_t u[4] = {v0[c].x, v0[c].y, v0[c].z, v0[c].w}, q[4] = {v1[c].x, v1[c].y, v1[c].z, v1[c].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float2 f = Cvt<T>::to_f2(u[k]);
-                if (MODE == ROW_ADD_NORM) { const float2 g = Cvt<T>::to_f2(q[k]); f.x += g.x; f.y += g.y; }
-                if (MODE == ROW_SILU) {
-                    const float2 g = Cvt<T>::to_f2(q[k]);
-                    f.x = __fdividef(f.x, 1.f + __expf(-f.x)) * g.x;
-                    f.y = __fdividef(f.y, 1.f + __expf(-f.y)) * g.y;
-                }
-                if (kNorm) { ss = fmaf(f.x, f.x, ss); ss = fmaf(f.y, f.y, ss); }
-                t[c][2 * k] = f.x; t[c][2 * k + 1] = f.y;
-            }
-            if (MODE == ROW_ADD_NORM)
-                res[i] = make_uint4(Cvt<T>::pack(t[c][0], t[c][1]), Cvt<T>::pack(t[c][2], t[c][3]), Cvt<T>::pack(t[c][4], t[c][5]), Cvt<T>::pack(t[c][6], t[c][7]));
-            if (kNorm) {
-                const uint4 w = wv[i];
-                const uint32_t g[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { const float2 h = Cvt<T>::to_f2(g[k]); t[c][2 * k] *= h.x; t[c][2 * k + 1] *= h.y; }
-            }
-            if (QUANT) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) amax = max(amax, abs_bits(t[c][k]));
-            }
-        }
-    }
+    const int lane = threadIdx.x & 31;
+    const int tid = WARP ? lane : threadIdx.x, nt = WARP ? 32 : blockDim.x;
+    const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : a.rows;      // a CTA takes one row
+    const uint4* wv = reinterpret_cast<const uint4*>(a.weight);
     __shared__ float s_ss[32];
     __shared__ uint32_t s_mx[32];
-    if (kNorm) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
-    if (QUANT) amax = __reduce_max_sync(0xffffffffu, amax);
-    const int warps = nt >> 5;
-    if ((threadIdx.x & 31) == 0) { s_ss[threadIdx.x >> 5] = ss; s_mx[threadIdx.x >> 5] = amax; }
-    __syncthreads();
-    ss = 0.f; amax = 0;
-    for (int i = 0; i < warps; ++i) { ss += s_ss[i]; amax = max(amax, s_mx[i]); }
-    const float rstd = kNorm ? rsqrtf(fmaf(ss, a.inv_cols, a.eps)) : 1.f;
-    if (QUANT) {
-        // the maximum of |t * w * rstd| is that of |t * w| times rstd: rounding a product is monotonic
-        const RowScale r = row_scale(abs_bits(__uint_as_float(amax) * rstd), kInt8Top);
-        if (threadIdx.x == 0) a.scale[row] = r.scale;
-        uint2* dst = reinterpret_cast<uint2*>(a.codes + row * (int64_t)a.nvec * 8);
+
+    auto load = [&](int64_t row, RowData<VPT>& d) {
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.in) + row * a.in_stride);
+        const uint4* res = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.residual) + row * (int64_t)a.nvec * 8);
 #pragma unroll
         for (int c = 0; c < VPT; ++c) {
-            const int i = threadIdx.x + c * nt;
+            const int i = tid + c * nt;
             if (i < a.nvec) {
-                float y[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = t[c][k] * rstd;
-                dst[i] = make_uint2(pack_codes4<ESP_CODE_INT8>(y, r.inv, r.finite), pack_codes4<ESP_CODE_INT8>(y + 4, r.inv, r.finite));
+                d.a[c] = src[i];
+                if (MODE == ROW_ADD_NORM) d.b[c] = res[i];
+                if (MODE == ROW_SILU) d.b[c] = src[a.nvec + i];
             }
         }
-    } else {
-        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + row * (int64_t)a.nvec * 8);
+    };
+    RowData<VPT> d;
+    if (first < a.rows) load(first, d);
+#pragma unroll 1
+    for (int64_t row = first; row < a.rows; row += step) {
+        float t[VPT][8];
+        float ss = 0.f;
+        uint32_t amax = 0;
+        uint4* res = MODE == ROW_ADD_NORM ? reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.residual) + row * (int64_t)a.nvec * 8) : nullptr;
 #pragma unroll
         for (int c = 0; c < VPT; ++c) {
-            const int i = threadIdx.x + c * nt;
+            const int i = tid + c * nt;
             if (i < a.nvec) {
-                uint32_t o[4];
+                const uint32_t u[4] = {d.a[c].x, d.a[c].y, d.a[c].z, d.a[c].w}, q[4] = {d.b[c].x, d.b[c].y, d.b[c].z, d.b[c].w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = Cvt<T>::pack(t[c][2 * k] * rstd, t[c][2 * k + 1] * rstd);
-                dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+                for (int k = 0; k < 4; ++k) {
+                    float2 f = Cvt<T>::to_f2(u[k]);
+                    if (MODE == ROW_ADD_NORM) { const float2 g = Cvt<T>::to_f2(q[k]); f.x += g.x; f.y += g.y; }
+                    if (MODE == ROW_SILU) {
+                        const float2 g = Cvt<T>::to_f2(q[k]);
+                        f.x = __fdividef(f.x, 1.f + __expf(-f.x)) * g.x;
+                        f.y = __fdividef(f.y, 1.f + __expf(-f.y)) * g.y;
+                    }
+                    if (kNorm) { ss = fmaf(f.x, f.x, ss); ss = fmaf(f.y, f.y, ss); }
+                    t[c][2 * k] = f.x; t[c][2 * k + 1] = f.y;
+                }
+                if (MODE == ROW_ADD_NORM)
+                    res[i] = make_uint4(Cvt<T>::pack(t[c][0], t[c][1]), Cvt<T>::pack(t[c][2], t[c][3]), Cvt<T>::pack(t[c][4], t[c][5]), Cvt<T>::pack(t[c][6], t[c][7]));
+            }
+        }
+        if (WARP && row + step < a.rows) load(row + step, d);
+#pragma unroll
+        for (int c = 0; c < VPT; ++c) {
+            const int i = tid + c * nt;
+            if (i < a.nvec) {
+                if (kNorm) {
+                    const uint4 w = __ldg(wv + i);
+                    const uint32_t g[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { const float2 h = Cvt<T>::to_f2(g[k]); t[c][2 * k] *= h.x; t[c][2 * k + 1] *= h.y; }
+                }
+                if (QUANT) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) amax = max(amax, abs_bits(t[c][k]));
+                }
+            }
+        }
+        if (kNorm) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+        if (QUANT) amax = __reduce_max_sync(0xffffffffu, amax);
+        if (!WARP) {
+            const int warps = nt >> 5;
+            if (lane == 0) { s_ss[threadIdx.x >> 5] = ss; s_mx[threadIdx.x >> 5] = amax; }
+            __syncthreads();
+            ss = 0.f; amax = 0;
+            for (int i = 0; i < warps; ++i) { ss += s_ss[i]; amax = max(amax, s_mx[i]); }
+        }
+        const float rstd = kNorm ? rsqrtf(fmaf(ss, a.inv_cols, a.eps)) : 1.f;
+        if (QUANT) {
+            // the maximum of |t * w * rstd| is that of |t * w| times rstd: rounding a product is monotonic
+            const RowScale r = row_scale(abs_bits(__uint_as_float(amax) * rstd), kInt8Top);
+            if (tid == 0) a.scale[row] = r.scale;
+            uint2* dst = reinterpret_cast<uint2*>(a.codes + row * (int64_t)a.nvec * 8);
+#pragma unroll
+            for (int c = 0; c < VPT; ++c) {
+                const int i = tid + c * nt;
+                if (i < a.nvec) {
+                    float y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = t[c][k] * rstd;
+                    dst[i] = make_uint2(pack_codes4<ESP_CODE_INT8>(y, r.inv, r.finite), pack_codes4<ESP_CODE_INT8>(y + 4, r.inv, r.finite));
+                }
+            }
+        } else {
+            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + row * (int64_t)a.nvec * 8);
+#pragma unroll
+            for (int c = 0; c < VPT; ++c) {
+                const int i = tid + c * nt;
+                if (i < a.nvec) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[k] = Cvt<T>::pack(t[c][2 * k] * rstd, t[c][2 * k + 1] * rstd);
+                    dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+                }
             }
         }
     }
 }
 
-// 16 codes per lane and step
-template <typename OT>
+// V codes per lane and step, U steps in flight
+template <typename OT, int V, int U>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(OT* __restrict__ out, const int8_t* __restrict__ codes,
                                                               const float* __restrict__ scale, int64_t rows, int vecs) {
     const int64_t total = rows * vecs, stride = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-        const uint2 w = reinterpret_cast<const uint2*>(codes)[i];
-        const float s = scale[i / vecs];
-        float f[4], g[4];
-        unpack_codes4<ESP_CODE_INT8>(w.x, f); unpack_codes4<ESP_CODE_INT8>(w.y, g);
-        if constexpr (sizeof(OT) == 4) {
-            float4* o = reinterpret_cast<float4*>(out + i * 8);
-            o[0] = make_float4(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
-            o[1] = make_float4(g[0] * s, g[1] * s, g[2] * s, g[3] * s);
-        } else {
-            *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(Cvt<OT>::pack(f[0] * s, f[1] * s), Cvt<OT>::pack(f[2] * s, f[3] * s),
-                                                               Cvt<OT>::pack(g[0] * s, g[1] * s), Cvt<OT>::pack(g[2] * s, g[3] * s));
+    for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += U * stride) {
+        uint32_t w[U][V / 4];
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = i0 + u * stride;
+            if (i < total) {
+                if constexpr (V == 16) {
+                    const uint4 x = __ldcs(reinterpret_cast<const uint4*>(codes) + i);
+                    w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
+                } else {
+                    const uint2 x = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
+                    w[u][0] = x.x; w[u][1] = x.y;
+                }
+                s[u] = scale[i / vecs];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = i0 + u * stride;
+            if (i >= total) continue;
+            float f[V];
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) {
+                float x[4];
+                unpack_codes4<ESP_CODE_INT8>(w[u][j], x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[4 * j + k] = x[k] * s[u];
+            }
+            if constexpr (sizeof(OT) == 4) {
+                float4* o = reinterpret_cast<float4*>(out + i * V);
+#pragma unroll
+                for (int j = 0; j < V / 4; ++j) o[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+            } else {
+                uint4* o = reinterpret_cast<uint4*>(out + i * V);
+#pragma unroll
+                for (int j = 0; j < V / 8; ++j)
+                    o[j] = make_uint4(Cvt<OT>::pack(f[8 * j], f[8 * j + 1]), Cvt<OT>::pack(f[8 * j + 2], f[8 * j + 3]),
+                                      Cvt<OT>::pack(f[8 * j + 4], f[8 * j + 5]), Cvt<OT>::pack(f[8 * j + 6], f[8 * j + 7]));
+            }
         }
     }
 }
@@ -144,13 +197,21 @@ template <typename T, int MODE, bool QUANT>
 static int launch_row(RowArgs a, int64_t rows, int cols, cudaStream_t s) {
     a.nvec = cols / 8;
     a.inv_cols = 1.f / (float)cols;
-    // 16-byte vectors per thread: 2 keeps a row of 4096 in 256 threads; wider rows hold more per thread up to 8
-    const int vpt = a.nvec <= 2 * 512 ? 2 : (a.nvec <= 4 * 512 ? 4 : 8);
-    int nt = ((a.nvec + vpt - 1) / vpt + 31) / 32 * 32;
-    const unsigned grid = (unsigned)rows;
-    if (vpt == 2) row_kernel<T, MODE, 2, QUANT><<<grid, nt, 0, s>>>(a);
-    else if (vpt == 4) row_kernel<T, MODE, 4, QUANT><<<grid, nt, 0, s>>>(a);
-    else row_kernel<T, MODE, 8, QUANT><<<grid, nt, 0, s>>>(a);
+    a.rows = rows;
+    if (a.nvec <= 64) {
+        const int64_t want = (rows + 7) / 8, cap = kNumSMs * 16;
+        const unsigned grid = (unsigned)(want < cap ? want : cap);
+        if (a.nvec <= 32) row_kernel<T, MODE, 1, QUANT, true><<<grid, 256, 0, s>>>(a);
+        else row_kernel<T, MODE, 2, QUANT, true><<<grid, 256, 0, s>>>(a);
+    } else {
+        // 16-byte vectors per thread: 2 keeps a row of 4096 in 256 threads; wider rows hold more per thread up to 8
+        const int vpt = a.nvec <= 2 * 512 ? 2 : (a.nvec <= 4 * 512 ? 4 : 8);
+        const int nt = ((a.nvec + vpt - 1) / vpt + 31) / 32 * 32;
+        const unsigned grid = (unsigned)rows;
+        if (vpt == 2) row_kernel<T, MODE, 2, QUANT, false><<<grid, nt, 0, s>>>(a);
+        else if (vpt == 4) row_kernel<T, MODE, 4, QUANT, false><<<grid, nt, 0, s>>>(a);
+        else row_kernel<T, MODE, 8, QUANT, false><<<grid, nt, 0, s>>>(a);
+    }
     ESP_LAUNCH_CHECK("row_kernel");
     return ESP_OK;
 }
@@ -173,7 +234,7 @@ extern "C" int esp_add_rms_norm(void* out, void* residual, const void* in, const
     const int rc = check_row(tokens, hidden, dtype);
     if (rc) return rc;
     if (!aligned16(out) || !aligned16(residual) || !aligned16(in) || !aligned16(weight)) return ESP_ERR_ALIGNMENT;
-    RowArgs a{in, weight, residual, hidden, out, nullptr, nullptr, 0, eps, 0.f};
+    RowArgs a{in, weight, residual, hidden, out, nullptr, nullptr, 0, eps, 0.f, 0};
     return dtype == ESP_DTYPE_F16 ? launch_row<__half, ROW_ADD_NORM, false>(a, tokens, hidden, (cudaStream_t)stream)
                                   : launch_row<__nv_bfloat16, ROW_ADD_NORM, false>(a, tokens, hidden, (cudaStream_t)stream);
 }
@@ -185,7 +246,7 @@ extern "C" int esp_add_rms_norm_q8(int8_t* codes, float* scale, void* residual, 
     const int rc = check_row(tokens, hidden, dtype);
     if (rc) return rc;
     if (!aligned16(codes) || !aligned16(residual) || !aligned16(in) || !aligned16(weight)) return ESP_ERR_ALIGNMENT;
-    RowArgs a{in, weight, residual, hidden, nullptr, codes, scale, 0, eps, 0.f};
+    RowArgs a{in, weight, residual, hidden, nullptr, codes, scale, 0, eps, 0.f, 0};
     cudaStream_t s = (cudaStream_t)stream;
     if (residual)
         return dtype == ESP_DTYPE_F16 ? launch_row<__half, ROW_ADD_NORM, true>(a, tokens, hidden, s)
@@ -201,7 +262,7 @@ extern "C" int esp_silu_and_mul_q8(int8_t* codes, float* scale, const void* io, 
     const int rc = check_row(tokens, ffn_inter_dim, dtype);
     if (rc) return rc;
     if (!aligned16(codes) || !aligned16(io)) return ESP_ERR_ALIGNMENT;
-    RowArgs a{io, nullptr, nullptr, 2 * (int64_t)ffn_inter_dim, nullptr, codes, scale, 0, 0.f, 0.f};
+    RowArgs a{io, nullptr, nullptr, 2 * (int64_t)ffn_inter_dim, nullptr, codes, scale, 0, 0.f, 0.f, 0};
     return dtype == ESP_DTYPE_F16 ? launch_row<__half, ROW_SILU, true>(a, tokens, ffn_inter_dim, (cudaStream_t)stream)
                                   : launch_row<__nv_bfloat16, ROW_SILU, true>(a, tokens, ffn_inter_dim, (cudaStream_t)stream);
 }
@@ -213,7 +274,7 @@ extern "C" int esp_quantize_rows(int8_t* codes, float* scale, const void* x, int
     const int rc = check_row(rows, cols, dtype);
     if (rc) return rc;
     if (!aligned16(codes) || !aligned16(x) || x_row_stride % 8) return ESP_ERR_ALIGNMENT;
-    RowArgs a{x, nullptr, nullptr, x_row_stride, nullptr, codes, scale, 0, 0.f, 0.f};
+    RowArgs a{x, nullptr, nullptr, x_row_stride, nullptr, codes, scale, 0, 0.f, 0.f, 0};
     return dtype == ESP_DTYPE_F16 ? launch_row<__half, ROW_PLAIN, true>(a, rows, cols, (cudaStream_t)stream)
                                   : launch_row<__nv_bfloat16, ROW_PLAIN, true>(a, rows, cols, (cudaStream_t)stream);
 }
@@ -222,13 +283,15 @@ extern "C" int esp_dequantize_rows(void* out, const int8_t* codes, const float* 
     if (rows == 0) return ESP_OK;
     if (!out || !codes || !scale || rows < 0 || cols <= 0) return ESP_ERR_BAD_ARG;
     if (cols % 8 || !aligned16(out) || ((uintptr_t)codes & 7u)) return ESP_ERR_ALIGNMENT;
-    const int64_t want = (rows * (cols / 8) + 255) / 256, cap = (int64_t)kNumSMs * 32;
+    const int64_t want = (rows * (cols / 8) + 1023) / 1024, cap = (int64_t)kNumSMs * 32;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == ESP_DTYPE_F16) dequantize_rows_kernel<__half><<<grid, 256, 0, s>>>((__half*)out, codes, scale, rows, cols / 8);
-    else if (dtype == ESP_DTYPE_BF16) dequantize_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>((__nv_bfloat16*)out, codes, scale, rows, cols / 8);
-    else if (dtype == ESP_DTYPE_F32) dequantize_rows_kernel<float><<<grid, 256, 0, s>>>((float*)out, codes, scale, rows, cols / 8);
+#define ESP_DQ(OT) dequantize_rows_kernel<OT, 8, 4><<<grid, 256, 0, s>>>((OT*)out, codes, scale, rows, cols / 8);
+    if (dtype == ESP_DTYPE_F16) ESP_DQ(__half)
+    else if (dtype == ESP_DTYPE_BF16) ESP_DQ(__nv_bfloat16)
+    else if (dtype == ESP_DTYPE_F32) ESP_DQ(float)
     else return ESP_ERR_BAD_ARG;
+#undef ESP_DQ
     ESP_LAUNCH_CHECK("dequantize_rows_kernel");
     return ESP_OK;
 }

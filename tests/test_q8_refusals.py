@@ -28,7 +28,7 @@ SCATTER = dict(src=P, src_row=256, src_head=128, codes=P, codes_row=272, codes_h
 
 @pytest.mark.parametrize("change,rc", [
     (dict(n=0), 0), (dict(n=-1), BAD), (dict(src=None), BAD), (dict(codes=None), BAD), (dict(scales=None), BAD), (dict(dest=None), BAD),
-    (dict(heads2=0), BAD), (dict(head_dim=0), BAD), (dict(head_dim=528), UNSUP), (dict(head_dim=24), ALIGN), (dict(dtype=2), BAD), (dict(dtype=7), BAD),
+    (dict(heads2=0), BAD), (dict(head_dim=0), BAD), (dict(head_dim=272), UNSUP), (dict(head_dim=24), ALIGN), (dict(dtype=2), BAD), (dict(dtype=7), BAD),
     (dict(code=2), BAD), (dict(code=-1), BAD), (dict(pool_rows=0), BAD), (dict(src=P + 8), ALIGN), (dict(src_row=252), ALIGN), (dict(src_head=4), ALIGN),
     (dict(codes=P + 4), ALIGN), (dict(codes_row=264), ALIGN), (dict(codes_head=120), ALIGN), (dict(scales=P + 2), BAD), (dict(scales_row=1), BAD)])
 def test_scatter(lib, change, rc):
