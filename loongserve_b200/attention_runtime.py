@@ -19,7 +19,7 @@ from . import context_attention as ca
 from . import flash_decoding as fd
 from . import kv_ops
 from . import ring as ringmod
-from .mem_manager import LongServeMemoryManager, LongServeReqManager
+from .mem_manager import LongServeMemoryManager, LongServeReqManager, QuantizedKVMemoryManager
 
 
 def next_power_of_2(n: int) -> int:
@@ -30,16 +30,31 @@ class LongServeLlamaInferStateInfo(SimpleNamespace):
     """Per-batch state; attribute names as in the reference's class of the same name."""
 
 
+def _keep_quantized(batch_size, new_len, range_begin, range_end, new_len_sum, kv, kv_b_start_loc, cur_index, mem_index, pool_layer, *rest):
+    """``destindex_copy_and_register_kv`` for a layer of an 8-bit pool, in the argument order of the ring's keep step."""
+    kv_ops.destindex_copy_quantize_and_register_kv(batch_size, new_len, range_begin, range_end, new_len_sum, kv, kv_b_start_loc,
+                                                   cur_index, mem_index, pool_layer.codes, pool_layer.scales, *rest)
+
+
+def _stage1_quantized(mid_o, mid_lse, q, k, v, *rest):
+    """``flash_decoding_stage1`` for the K and V halves of a layer of an 8-bit pool."""
+    fd.flash_decoding_stage1_q8(mid_o, mid_lse, q, k.codes, k.scales, v.codes, v.scales, *rest)
+
+
 class ESPAttentionRuntime:
     """Owns the KV pool, the request table and the SP communicator of one instance (one GPU).
 
     ``sp_comm`` needs the RNCCLComm surface; it may be None when every batch runs on this instance alone.
-    ``total_rank`` is this instance's SP rank.  ``dtype`` is the KV / activation dtype (fp16 or bf16)."""
+    ``total_rank`` is this instance's SP rank.  ``dtype`` is the KV / activation dtype (fp16 or bf16).
+    ``kv_dtype`` torch.int8 or torch.float8_e4m3fn holds the pool in 8 bits (all instances alike): K/V rows are computed and
+    attended to in ``dtype`` during prefill, quantised as they are written to the pool, and read as codes by decode and
+    migration.  The peer-memory decode exchange is not available then (the message exchange is)."""
 
     def __init__(self, *, layers_num: int, q_head_num: int, kv_head_num: int, head_dim: int, max_total_token_num: int,
                  max_req_num: int, max_seq_length: int, sp_world_size: int = 1, total_rank: int = 0, sp_comm=None,
                  dtype=torch.bfloat16, device="cuda", decode_block_seq: Optional[int] = None,
-                 peer_memory_decode="auto", peer_memory_max_batch: Optional[int] = None, gathered_prefill: bool = False):
+                 peer_memory_decode="auto", peer_memory_max_batch: Optional[int] = None, gathered_prefill: bool = False,
+                 kv_dtype=None):
         self.layers_num = layers_num
         self.tp_q_head_num_ = q_head_num
         self.tp_k_head_num_ = kv_head_num
@@ -52,8 +67,10 @@ class ESPAttentionRuntime:
         self.device = torch.device(device)
         self.decode_block_seq = decode_block_seq
         # longserve_model.py:120-133: sp_world_size spare rows are appended to the pool and never handed out
-        self.mem_manager = LongServeMemoryManager(max_total_token_num, dtype, kv_head_num, head_dim, layers_num,
-                                                  num_idle_slots=sp_world_size, device=device)
+        self.kv_quantized = kv_dtype is not None and kv_dtype != dtype
+        manager = QuantizedKVMemoryManager if self.kv_quantized else LongServeMemoryManager
+        self.mem_manager = manager(max_total_token_num, kv_dtype if self.kv_quantized else dtype, kv_head_num, head_dim, layers_num,
+                                   num_idle_slots=sp_world_size, device=device)
         self.req_manager = LongServeReqManager(max_req_num, max_seq_length, self.mem_manager)
         self._fused_groups = {}
         # Striped prefill passes over all instances in two attention launches instead of sp_world_size (every block copied to
@@ -68,6 +85,10 @@ class ESPAttentionRuntime:
         # Multi-master decode exchanges queries and partials over peer memory (NVLink stores and flags inside the kernels)
         # whenever all instances sit in one node; the NCCL message exchange of the reference stays available
         # (peer_memory_decode=False) and is what batches that do not span every instance use.
+        if self.kv_quantized:
+            if peer_memory_decode is True:
+                raise ValueError("the peer-memory decode exchange reads a 16-bit pool: use the message exchange with kv_dtype")
+            peer_memory_decode = False
         if peer_memory_decode == "auto":
             peer_memory_decode = (sp_comm is not None and sp_world_size > 1 and self.device.type == "cuda"
                                   and hasattr(sp_comm, "nccl_send") and torch.cuda.device_count() >= sp_world_size)
@@ -81,10 +102,27 @@ class ESPAttentionRuntime:
         for decode batches whose only master is ``master_rank`` and whose peers are all instances.  Collective:
         every instance must call it, with an ``all_gather_bytes`` that returns each rank's bytes in rank order."""
         from .peer_decode import FusedDecodeGroup
+        if self.kv_quantized:
+            raise ValueError("the peer-memory decode exchange reads a 16-bit pool")
         if master_rank in self._fused_groups:
             self._fused_groups.pop(master_rank).close()
         self._fused_groups[master_rank] = FusedDecodeGroup(self.total_rank_, self.sp_world_size, master_rank, max_batch,
                                                            self.tp_q_head_num_, self.head_dim_, all_gather_bytes, self.dtype)
+
+    def _write_pool(self, rows, slots, layer_idx: int):
+        """Rows of a layer into their slots, quantised where the pool is held in 8 bits."""
+        layer = self.mem_manager.layer(layer_idx)
+        if self.kv_quantized:
+            kv_ops.destindex_copy_quantize_kv(rows, slots, layer.codes, layer.scales)
+        else:
+            kv_ops.destindex_copy_kv(rows, slots, layer)
+
+    def read_kv(self, slots, layer_idx: int):
+        """Rows [n, 2*Hkv, D] of a layer in the activation dtype, whatever the pool holds (hand-over of cached requests, checks)."""
+        layer = self.mem_manager.layer(layer_idx)
+        if self.kv_quantized:
+            return kv_ops.gather_dequantize_kv(layer.codes, layer.scales, slots.contiguous(), self.dtype)
+        return layer[slots.long()]
 
     def _ring_all_gather_bytes(self, mine: bytes) -> List[bytes]:
         """Every instance's 64 bytes in SP-rank order, passed round the ring of all instances over the communicator."""
@@ -159,7 +197,8 @@ class ESPAttentionRuntime:
             assert kv_cache_index_begin.shape[0] == kv_cache_index_end.shape[0] == batch_size
             st.kv_cache_index_begin, st.kv_cache_index_end = kv_cache_index_begin, kv_cache_index_end
             st.cur_kv_cache_index = torch.empty((batch_size,), dtype=torch.int32, device=self.device)
-        alloc_mem = self.mem_manager.alloc_contiguous(total_token_num) if not need_context_migration else None
+        # rows of an 8-bit pool are quantised from the scratch block: they are never computed in place
+        alloc_mem = self.mem_manager.alloc_contiguous(total_token_num) if not need_context_migration and not self.kv_quantized else None
         if alloc_mem is not None:
             st.mem_is_contiguous = True
             st.mem_index, st.mem_start, st.mem_end = alloc_mem
@@ -266,7 +305,7 @@ class ESPAttentionRuntime:
         else:
             kv = st.kv_buffer
             if not st.need_context_migration:
-                kv_ops.destindex_copy_kv(kv[:st.total_token_num], st.mem_index, self.mem_manager.kv_buffer[layer_idx])
+                self._write_pool(kv[:st.total_token_num], st.mem_index, layer_idx)
         o = torch.empty_like(q) if out is None else out
         if getattr(st, "gather_plans", None) is not None:
             ringmod.gathered_context_attention(
@@ -282,8 +321,9 @@ class ESPAttentionRuntime:
             recv_buffers=[st.peer_kv_buffer, st.kv_buffer], attention_fn=ca.context_attention_fwd,
             init_fn=ca.init_attention_state, overlap=overlap,
             keep=st.keep_plan if st.need_context_migration else None,
-            pool_layer=self.mem_manager.kv_buffer[layer_idx], layer_idx=layer_idx,
-            keep_fns=(kv_ops.pre_copy_and_register_kv, kv_ops.destindex_copy_and_register_kv))
+            pool_layer=self.mem_manager.layer(layer_idx), layer_idx=layer_idx,
+            keep_fns=(kv_ops.pre_copy_and_register_kv,
+                      _keep_quantized if self.kv_quantized else kv_ops.destindex_copy_and_register_kv))
         return o
 
     # ------------------------------------------------------------------------------------------ decode
@@ -305,7 +345,7 @@ class ESPAttentionRuntime:
         H2 = self.tp_k_head_num_ + self.tp_v_head_num_
         if is_master:
             assert b_req_idx.shape[0] == b_seq_len.shape[0] == batch_size == total_token_num and total_token_num > 0
-            alloc_mem = self.mem_manager.alloc_contiguous(total_token_num)
+            alloc_mem = None if self.kv_quantized else self.mem_manager.alloc_contiguous(total_token_num)
             if alloc_mem is not None:
                 st.mem_is_contiguous = True
                 st.mem_index, st.mem_start, st.mem_end = alloc_mem
@@ -362,13 +402,13 @@ class ESPAttentionRuntime:
     @torch.inference_mode()
     def post_decode_cache_kv(self, st, layer_idx: int):
         if not st.mem_is_contiguous:
-            kv_ops.destindex_copy_kv(st.kv_buffer, st.mem_index, self.mem_manager.kv_buffer[layer_idx])
+            self._write_pool(st.kv_buffer, st.mem_index, layer_idx)
 
     @torch.inference_mode()
     def token_attention(self, q, st, layer_idx: int, out=None):
         """One layer's decode attention on this instance in its master and/or peer role
         (longserve_transformer_layer_infer.py:224-370).  Masters get the attention output, pure peers None."""
-        pool_layer = self.mem_manager.kv_buffer[layer_idx]
+        pool_layer = self.mem_manager.layer(layer_idx)
         self._decode_calls += 1
         if (self.status_check_interval and self._decode_calls % self.status_check_interval == 0
                 and not torch.cuda.is_current_stream_capturing()):
@@ -379,6 +419,12 @@ class ESPAttentionRuntime:
             mp = st.master_plan
             Hkv = self.tp_k_head_num_
             qv = q.view(-1, self.tp_q_head_num_, self.head_dim_)
+            if self.kv_quantized:
+                k, v = pool_layer[:, :Hkv, :], pool_layer[:, Hkv:, :]
+                o, _ = fd.token_decode_attention_q8(qv.contiguous(), k.codes, k.scales, v.codes, v.scales, self.req_manager.req_to_token_indexs,
+                                                    mp.b_req_idx, mp.b_seq_len, mp.max_len_in_batch,
+                                                    out=None if out is None else out.view_as(qv), out_logexpsum=mp.global_out_lse)
+                return o if out is None else out
             fd.flash_decoding_stage1(mp.global_mid_o, mp.global_mid_lse, qv, pool_layer[:, :Hkv, :], pool_layer[:, Hkv:, :],
                                      self.req_manager.req_to_token_indexs, mp.b_req_idx, mp.b_seq_len, mp.max_len_in_batch,
                                      mp.block_seq)
@@ -391,7 +437,8 @@ class ESPAttentionRuntime:
             return self._token_attention_peer_memory(qv, st, pool_layer, out)
         return ringmod.multi_master_decode_attention(qv, pool_layer, self.req_manager.req_to_token_indexs, self.tp_k_head_num_,
                                                      self.sp_comm, self.total_rank_, st.master_plan, st.peer_plan,
-                                                     fd.flash_decoding_stage1, fd.flash_decoding_stage2, out=out)
+                                                     _stage1_quantized if self.kv_quantized else fd.flash_decoding_stage1,
+                                                     fd.flash_decoding_stage2, out=out)
 
     def _fused_covers(self, st) -> bool:
         """Whether this decode step goes over peer memory.  Decided from what EVERY instance of the batch knows -- the
@@ -452,8 +499,8 @@ class ESPAttentionRuntime:
         """longserve_model.py:563-622.  Assumes a reference count of one on the migrated slots, like the
         reference.  ``migration_len_sum`` / ``max_migration_len`` (host ints) avoid the two device->host reads."""
         total = int(migration_len_sum) if migration_len_sum is not None else int(torch.sum(b_migration_len).item())
-        H2 = self.tp_k_head_num_ + self.tp_v_head_num_
-        buf = torch.empty((self.layers_num, total, H2, self.head_dim_), dtype=self.dtype, device=self.device)
+        pool = self.mem_manager.migration_view              # whole rows travel: codes and scales of an 8-bit pool together
+        buf = torch.empty((self.layers_num, total) + tuple(pool.shape[2:]), dtype=pool.dtype, device=self.device)
         if total == 0:
             return
         if is_receiver:
@@ -463,11 +510,11 @@ class ESPAttentionRuntime:
             self.sp_comm.nccl_recv(buf, peer_sp_rank)
             alloc_mem = self.mem_manager.alloc(total)
             self.sp_comm.let_default_stream_wait()
-            kv_ops.decoding_stage_migration_receiver_kernel(buf, self.req_manager.req_to_token_indexs, self.mem_manager.kv_buffer,
+            kv_ops.decoding_stage_migration_receiver_kernel(buf, self.req_manager.req_to_token_indexs, pool,
                                                             alloc_mem, b_req_idx, b_migration_len, b_seq_len, max_migration_len)
         else:
             kv_ops.decoding_stage_migration_sender_kernel(buf, self.req_manager.req_to_token_indexs, self.mem_manager.mem_state,
-                                                          self.mem_manager.kv_buffer, b_req_idx, b_migration_len, b_seq_len,
+                                                          pool, b_req_idx, b_migration_len, b_seq_len,
                                                           max_migration_len)
             self.sp_comm.wait_for_default_stream()
             self.sp_comm.nccl_send(buf, peer_sp_rank)

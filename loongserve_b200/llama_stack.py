@@ -54,6 +54,23 @@ class LlamaWeights:
         self.lm_head = w(H, cfg.vocab)
 
 
+class LlamaW8A8Weights:
+    """The projections of ``LlamaWeights`` as int8 rows of output channels with one scale each, laid out once; embeddings, norms and
+    the output head stay as they are.  With these weights the stack runs every projection as an 8-bit integer product on int8
+    rows of activations (one scale per token)."""
+
+    w8a8 = True
+
+    def __init__(self, cfg: LlamaConfig, weights: LlamaWeights):
+        if cfg.hidden % 16 or (cfg.num_q_heads * cfg.head_dim) % 16 or cfg.ffn % 16:
+            raise ValueError("8-bit projections need hidden, q width and ffn to be multiples of 16")
+        self.embed, self.final_norm, self.lm_head = weights.embed, weights.final_norm, weights.lm_head
+        self.layers = []
+        for lw in weights.layers:
+            q8 = {n: layer_ops.quantize_rows(lw[n].t().contiguous()) for n in ("q", "kv", "o", "gate_up", "down")}
+            self.layers.append(dict(att_norm=lw["att_norm"], ffn_norm=lw["ffn_norm"], **q8))
+
+
 def rope_cos_sin(positions: torch.Tensor, head_dim: int, base: float, dtype):
     """cos/sin rows for the given global positions (rotate-half convention), built in fp32 then cast, as the
     reference's table is (longserve_model.py:264-275)."""
@@ -63,8 +80,31 @@ def rope_cos_sin(positions: torch.Tensor, head_dim: int, base: float, dtype):
 
 
 class LlamaESPStack:
-    def __init__(self, cfg: LlamaConfig, weights: LlamaWeights, runtime: ESPAttentionRuntime):
+    def __init__(self, cfg: LlamaConfig, weights, runtime: ESPAttentionRuntime):
+        """``weights``: ``LlamaWeights``, or ``LlamaW8A8Weights`` for 8-bit projections (with any ``kv_dtype`` of the runtime)."""
         self.cfg, self.w, self.rt = cfg, weights, runtime
+        self.w8a8 = getattr(weights, "w8a8", False)
+
+    # ------------------------------------------------------------------ a layer with 8-bit projections
+    def _w8a8_qkv(self, x, delta, lw, cos, sin, cache_kv):
+        """x += delta (the previous layer's output), the norm as int8 rows, q and the K/V rows of ``cache_kv``."""
+        cfg = self.cfg
+        h, hs = layer_ops.add_rms_norm_quant(x if delta is None else delta, None if delta is None else x, lw["att_norm"], cfg.rms_eps)
+        q = layer_ops.mm_w8a8(h, hs, *lw["q"], out_dtype=x.dtype).view(-1, cfg.num_q_heads, cfg.head_dim)
+        layer_ops.mm_w8a8(h, hs, *lw["kv"], out=cache_kv)
+        layer_ops.rotary_emb(q, cache_kv.view(-1, 2 * cfg.num_kv_heads, cfg.head_dim)[:, :cfg.num_kv_heads, :], cos, sin)
+        return q
+
+    def _w8a8_rest(self, x, o, lw):
+        """Output projection, x += it, and the FFN; the FFN's output is left for the next norm to add."""
+        cfg = self.cfg
+        att = layer_ops.mm_w8a8(*layer_ops.quantize_rows(o.view(x.shape[0], -1)), *lw["o"], out_dtype=x.dtype)
+        h, hs = layer_ops.add_rms_norm_quant(att, x, lw["ffn_norm"], cfg.rms_eps)
+        gu = layer_ops.mm_w8a8(h, hs, *lw["gate_up"], out_dtype=x.dtype)
+        return layer_ops.mm_w8a8(*layer_ops.silu_and_mul_quant(gu), *lw["down"], out_dtype=x.dtype)
+
+    def _w8a8_logits(self, x, delta):
+        return torch.mm(layer_ops.add_rms_norm(delta, x, self.w.final_norm, self.cfg.rms_eps), self.w.lm_head).float()
 
     # ------------------------------------------------------------------ prefill (every instance of the ring)
     @torch.inference_mode()
@@ -77,6 +117,15 @@ class LlamaESPStack:
         x = self.w.embed[input_ids.long()]
         n = x.shape[0]
         cos, sin = rope_cos_sin(positions, D, cfg.rope_base, x.dtype)
+        if self.w8a8:
+            delta = None
+            for li, lw in enumerate(self.w.layers):
+                q = self._w8a8_qkv(x, delta, lw, cos, sin, rt.pre_cache_kv(st, li).view(-1, 2 * Hkv * D)[:n])
+                delta = self._w8a8_rest(x, rt.context_attention(q, st, li), lw)
+            if last_token_rows is None:
+                return x.add_(delta)
+            rows = last_token_rows.long()
+            return self._w8a8_logits(x[rows], delta[rows])
         for li, lw in enumerate(self.w.layers):
             h = layer_ops.rms_norm(x, lw["att_norm"], cfg.rms_eps)
             q = torch.mm(h, lw["q"])
@@ -102,6 +151,16 @@ class LlamaESPStack:
             x = self.w.embed[input_ids.long()]
             n = x.shape[0]
             cos, sin = rope_cos_sin(positions, D, cfg.rope_base, x.dtype)
+        if self.w8a8:
+            delta = None
+            for li, lw in enumerate(self.w.layers):
+                if not is_master:
+                    rt.token_attention(None, st, li)
+                    continue
+                q = self._w8a8_qkv(x, delta, lw, cos, sin, rt.decode_cache_kv(st, li).view(-1, 2 * Hkv * D)[:n])
+                rt.post_decode_cache_kv(st, li)
+                delta = self._w8a8_rest(x, rt.token_attention(q, st, li), lw)
+            return self._w8a8_logits(x, delta) if is_master else None
         for li, lw in enumerate(self.w.layers):
             if is_master:
                 h = layer_ops.rms_norm(x, lw["att_norm"], cfg.rms_eps)
@@ -176,6 +235,8 @@ class GraphedDecode:
         token of every request."""
         self.stack, self.group = stack, group
         rt, cfg = stack.rt, stack.cfg
+        if stack.w8a8 or rt.kv_quantized:
+            raise ValueError("the recorded decode step runs 16-bit projections over a 16-bit pool")
         self.is_master = group.rank == group.master
         dev = b_seq_len.device
         B = b_seq_len.shape[0]

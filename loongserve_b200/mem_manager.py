@@ -96,8 +96,17 @@ class LongServeMemoryManager:
         self._slots = HostSlotAllocator(size)
         self.mem_state = torch.zeros((size,), dtype=torch.int32, device=self.device)
         self.indexes = torch.arange(0, size, dtype=torch.long, device=self.device)
-        self.kv_buffer = torch.empty((self.layer_num, size + self.num_idle_slots, 2 * self.head_num, self.head_dim),
-                                     dtype=self.dtype, device=self.device)
+        self.kv_buffer = self._make_buffer(size + self.num_idle_slots)
+
+    def _make_buffer(self, rows: int):
+        return torch.empty((self.layer_num, rows, 2 * self.head_num, self.head_dim), dtype=self.dtype, device=self.device)
+
+    def layer(self, layer_idx: int):
+        return self.kv_buffer[layer_idx]
+
+    @property
+    def migration_view(self):
+        return self.kv_buffer
 
     @property
     def can_use_mem_size(self) -> int:
@@ -154,8 +163,59 @@ class LongServeMemoryManager:
 
     @torch.inference_mode()
     def resize_mem(self, new_size):
-        self.kv_buffer = None                     # let the old pool go before the new one is allocated
+        self.kv_buffer = self._layers = None      # let the old pool go before the new one is allocated
         self._build(int(new_size))
+
+
+class QuantizedPoolLayer:
+    """One layer of a pool held in 8 bits: ``codes`` [slots, heads, head_dim] (int8 or e4m3) and ``scales`` fp32 [slots, heads].
+    ``layer[:, a:b, :]`` is the same for a range of heads, as callers slice a 16-bit pool layer into its K and V halves."""
+
+    def __init__(self, codes, scales):
+        self.codes, self.scales = codes, scales
+
+    def __getitem__(self, index):
+        rows, heads, dims = index
+        assert rows == slice(None) and dims == slice(None) and isinstance(heads, slice), "a range of heads: layer[:, a:b, :]"
+        return QuantizedPoolLayer(self.codes[:, heads], self.scales[:, heads])
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+class QuantizedKVMemoryManager(LongServeMemoryManager):
+    """The pool in 8 bits: ``kv_buffer`` uint8 [layer, size + num_idle_slots, row_bytes], where a row keeps all that a layer knows
+    of a token -- 2*head_num*head_dim codes, then 2*head_num fp32 scales, padded to 16 bytes -- so that slots are allocated,
+    migrated and freed exactly as 16-bit ones.  ``layer(i)`` gives the codes and scales as tensors.  For 32 + 32 heads of 128 a row
+    has 8448 bytes instead of 16384: the same memory holds 1.94 times as many tokens.  ``dtype``: torch.int8 or
+    torch.float8_e4m3fn."""
+
+    def __init__(self, size, dtype, head_num, head_dim, layer_num, num_idle_slots=0, always_copy=False, device="cuda"):
+        if dtype not in (torch.int8, torch.float8_e4m3fn):
+            raise TypeError(f"a pool in 8 bits holds torch.int8 or torch.float8_e4m3fn codes, not {dtype}")
+        if head_dim % 16:
+            raise ValueError("head_dim must be a multiple of 16")
+        self.row_bytes = (2 * head_num * (head_dim + 4) + 15) // 16 * 16
+        super().__init__(size, dtype, head_num, head_dim, layer_num, num_idle_slots, always_copy, device)
+
+    def _make_buffer(self, rows):
+        self._layers = {}
+        return torch.empty((self.layer_num, rows, self.row_bytes), dtype=torch.uint8, device=self.device)
+
+    def layer(self, layer_idx: int) -> QuantizedPoolLayer:
+        got = self._layers.get(layer_idx)
+        if got is None:
+            rows, heads2, cut = self.kv_buffer[layer_idx], 2 * self.head_num, 2 * self.head_num * self.head_dim
+            got = QuantizedPoolLayer(rows[:, :cut].view(self.dtype).unflatten(1, (heads2, self.head_dim)),
+                                     rows[:, cut:cut + 4 * heads2].view(torch.float32))
+            self._layers[layer_idx] = got
+        return got
+
+    @property
+    def migration_view(self):
+        """The pool as the migration kernels take it: rows of bytes."""
+        return self.kv_buffer.unsqueeze(2)
 
 
 # earlier name of the host-decided manager, kept for callers written against it
