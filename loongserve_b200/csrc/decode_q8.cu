@@ -1,6 +1,7 @@
 // Split-KV decode attention over a KV pool held in 8 bits (codes and one fp32 scale per slot and head, quant_common.cuh):
 //   s_t = (q . ck_t) * k_scale_t * sm_scale,   p_t = exp(s_t - m),   o = sum_t p_t * v_scale_t * cv_t / sum_t p_t
-// Same splits, partials and merge as the 16-bit form (decode_attention.cu).
+// Stage 1 writes the same splits and partials as the 16-bit form (decode_attention.cu); the call that does both stages divides the
+// tokens itself (below).
 //
 // Bound by HBM: 2 * (128 + 4) bytes per token and kv head, each read once.  At that rate one SM has to take in a code every
 // 1/23 of a cycle and multiply it with up to 8 query heads, which is past what fp32 lanes do next to the conversion; so codes
@@ -14,9 +15,12 @@
 // (lane = 4g + c.)  A warp takes 16 tokens of one head tile per step.
 //
 // Precision.  q is scaled by a power of two per head so that its largest element is near 2^7 in f16: exact down to 2^-21 of
-// it.  Scores, maxima, sums and outputs are fp32.  The weights p * v_scale are rounded to f16 (11 bits) before the second
-// product, relative to 2^-8 * the largest v_scale seen by the warp: like the 16-bit P of the prefill kernels, one rounding of
-// 2^-12 relative per term.
+// it.  Scores, maxima, sums and outputs are fp32.  A weight p * v_scale, relative to 2^-8 * the largest v_scale seen by the warp,
+// enters the second product as its rounding to f16 and the rounding of what that left: 2^-22 relative.  (The rounding alone, 2^-12,
+// showed in f16 outputs: 3.3e-4 against 2.0e-4 for fp32 weights.)  With groups of up to four heads (GT = 4) the rests take the columns
+// of heads 4-7 and cost no product; larger groups (GT = 8) multiply V twice: 57 us for 64 requests x 8 q heads on 4 kv heads x 2500
+// tokens, 55 without.
+#include <algorithm>
 #include "quant_common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -42,12 +46,14 @@ struct DecodeQ8Args {
     const int32_t *b_req_idx, *b_seqlen;
     int batch, num_q_heads, num_kv_heads, group, seq_block_size;
     float scale_log2; int64_t pool_rows;
-    int num_blocks, compact;
-    int head_tiles, head_groups, scale_vec;      // tiles of up to 8 q heads of one kv head; CTAs that cover them all for one split
-    void* o; float* lse; int o_dtype; // with one split only: the results themselves instead of partials (o != nullptr)
+    int max_len, num_blocks, counted, ranges, min_units;  // ranges > 0: the tokens of all requests in that many equal pieces
+    int* parts;                                  // ranges: per request its first piece's partial and how many it has
+    int head_tiles, head_groups, scale_vec, q_bf16;      // tiles of up to 8 q heads of one kv head; CTAs that cover them all for one split
+    void* o; float* lse; int o_dtype, direct;    // results; direct: one split per request, whose results are written at once
 };
 
 constexpr int kQ8Warps = 4, kQ8HeadTile = 8;
+constexpr int kQ8Resident = 3 * kNumSMs, kQ8MinPiece = 128;     // CTAs the GPU holds; tokens below which a piece is not cut
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -79,11 +85,18 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 // pitches in shared memory are chosen so that the fragment reads (16 bytes per lane) have no bank conflicts: K rows an odd
 // multiple of 64 bytes apart, V rows an odd multiple of 16.
 //
-// CTAs are persistent: each walks over (split, request, heads) items, and the producer runs ahead into the next item, so that
-// neither the start of an item (length, slots, queries) nor its results stop the flow of copies.  Where a CTA has several items
-// and the batch is small enough, the splits that exist are counted first (a prefix sum over the lengths), so that ragged
-// batches divide evenly.
-constexpr int kQ8MaxCompact = 256;        // requests whose lengths are held in shared memory
+// CTAs are persistent: each walks over items (a request's tokens t0..t1, heads), and the producer runs ahead into the next item, so
+// that neither the start of an item (length, slots, queries) nor its results stop the flow of copies.  How the tokens are divided:
+//   ranges   the steps of all requests, laid end to end, are cut into as many equal pieces as there are CTAs for each group of heads;
+//            a piece that crosses requests has an item for each.  Pieces and requests both only grow along the way, so piece + request
+//            numbers a partial uniquely, and there are at most pieces + requests of them.  A request inside one piece gets its results
+//            at once.  Against splits of a fixed length every CTA has the same work and writes a partial or two instead of one per
+//            128 to 512 tokens: 185 us instead of 206 for 2 requests x 262144 tokens x 8 kv heads (group 4), 77 instead of 97 for
+//            64 requests x 4 kv heads (group 8), 474 instead of 509 for 32 requests x 1K-16K tokens x 32 kv heads.
+//   counted  splits of seq_block_size tokens, where a CTA has several and the batch is small enough: those that exist are counted
+//            first, so that ragged batches divide evenly.
+//   else     all splits up to the longest possible request; those behind a request's end are passed over.
+constexpr int kQ8MaxCounted = 384;        // requests whose lengths are held in shared memory
 struct WarpStateQ8 { float acc[32][32], m[32], l[32], v[32]; };      // [register][lane]
 template <int NH> struct RingQ8 {
     static constexpr int WT = kQ8Warps / NH, kTokens = 16 * WT;
@@ -96,7 +109,7 @@ template <int NH> struct RingQ8 {
     static constexpr int kOffAbort = kOffBar + 2 * kStages * 8;
     static constexpr int kOffMerge = kOffAbort + 16;                                            // states of the warps with wt > 0
     static constexpr int kOffLen = kOffMerge + (WT - 1) * NH * (int)sizeof(WarpStateQ8);        // lengths, first blocks
-    static constexpr int kSmem = kOffLen + (2 * kQ8MaxCompact + 1) * 4;
+    static constexpr int kSmem = kOffLen + (2 * kQ8MaxCounted + 1) * 4;
 };
 static_assert(3 * (RingQ8<4>::kSmem + 1024) <= 233472 && 3 * (RingQ8<2>::kSmem + 1024) <= 233472 && 3 * (RingQ8<1>::kSmem + 1024) <= 233472,
               "three CTAs to an SM");
@@ -156,9 +169,10 @@ __device__ __forceinline__ void store_row16(void* o, int64_t i, const float (&x)
     p[0] = make_uint4(u[0], u[1], u[2], u[3]); p[1] = make_uint4(u[4], u[5], u[6], u[7]);
 }
 
-struct ItemQ8 { int b, blk, hg, t0, t1, req, steps; bool write; };
+struct ItemQ8 { int b, hg, t0, t1, req, steps; int64_t row0; bool write, whole; };   // row0: of the partials, in rows of all heads
+struct CursorQ8 { int n, u, u1; };             // (piece, heads), its units from u to u1 are still to do
 
-template <typename T, int CODE, int NH>
+template <int CODE, int NH, int GT>
 __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel(DecodeQ8Args a) {
     using R = RingQ8<NH>;
     constexpr int WT = R::WT;
@@ -168,22 +182,23 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     auto empty = [sbase](int st) { return sbase + R::kOffBar + 8u * (R::kStages + st); };
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + R::kOffAbort);
     int* s_len = reinterpret_cast<int*>(smem + R::kOffLen);               // -1: the request's row is not in the table
-    int* s_first = s_len + kQ8MaxCompact;
+    int* s_first = s_len + kQ8MaxCounted;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool direct = a.o != nullptr;                                   // one split: results, also of empty requests
     if (threadIdx.x == 0) {
         *s_abort = *reinterpret_cast<volatile int*>(&g_decode_q8_status[0]) == ESP_ERR_DEVICE_TIMEOUT ? 1 : 0;
         for (int i = 0; i < R::kStages; ++i) { ptx::mbar_init(full(i), 33); ptx::mbar_init(empty(i), kQ8Warps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     auto blocks_of = [&](int len) { return len <= 0 ? 0 : min((len - 1) / a.seq_block_size + 1, a.num_blocks); };
-    if (a.compact) {
+    const int unit = a.ranges ? R::kTokens : a.seq_block_size;
+    if (a.counted) {
         for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
             const int len = a.b_seqlen[b], req = a.b_req_idx[b];
             const bool ok = req >= 0 && req < a.rtt_rows && len <= a.rtt_cols;
             if (!ok && len > 0) q8_report(1, req);
-            s_len[b] = ok ? len : -1;
-            s_first[b + 1] = blocks_of(len);
+            const int seen = min(len, a.max_len);
+            s_len[b] = ok ? (a.ranges ? seen : len) : -1;
+            s_first[b + 1] = a.ranges ? (seen <= 0 ? 0 : (seen - 1) / R::kTokens + 1) : blocks_of(len);
         }
         __syncthreads();
         if (warp == 0) {
@@ -199,34 +214,58 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         }
     }
     __syncthreads();
-    const int items = (a.compact ? s_first[a.batch] : a.num_blocks * a.batch) * a.head_groups;
-    // all head groups of a split are neighbouring items: their rows are neighbours in memory
-    auto item_at = [&](int n) -> ItemQ8 {
-        ItemQ8 it;
-        const int bi = n / a.head_groups;
-        it.hg = n - bi * a.head_groups;
+    const int units = a.counted ? s_first[a.batch] : a.num_blocks * a.batch;
+    const int per = a.ranges ? max(a.min_units, (units - 1) / a.ranges + 1) : 1;
+    const int items = (units == 0 ? 0 : (units - 1) / per + 1) * a.head_groups;
+    if (a.ranges && blockIdx.x == 0)
+        for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+            const int u0 = s_first[b], u1 = s_first[b + 1];
+            a.parts[2 * b] = u0 / per + b;
+            a.parts[2 * b + 1] = u1 > u0 ? (u1 - 1) / per - u0 / per + 1 : 0;
+        }
+    // The next item of a cursor.  All head groups of a piece are neighbouring CTAs' work: their rows are neighbours in memory.
+    CursorQ8 cur{(int)blockIdx.x - (int)gridDim.x, 0, 0};
+    auto next_item = [&](ItemQ8& it) -> bool {
+        if (cur.u >= cur.u1) {
+            cur.n += gridDim.x;
+            if (cur.n >= items) return false;
+            cur.u = cur.n / a.head_groups * per;
+            cur.u1 = min(cur.u + per, units);
+        }
+        const int piece = cur.n / a.head_groups;
+        it.hg = cur.n - piece * a.head_groups;
         int len;
-        if (a.compact) {
-            int lo = 0, hi = a.batch - 1;                                 // the last request whose first block is not behind bi
-            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_first[mid] <= bi) lo = mid; else hi = mid - 1; }
-            it.b = lo; it.blk = bi - s_first[lo];
+        if (a.counted) {
+            int lo = 0, hi = a.batch - 1;                                 // the last request whose first unit is not behind u
+            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_first[mid] <= cur.u) lo = mid; else hi = mid - 1; }
+            const int first = s_first[lo], behind = s_first[lo + 1], end = min(cur.u1, behind);
+            it.b = lo;
             len = s_len[lo];
             it.req = len > 0 ? a.b_req_idx[lo] : 0;
             it.write = true;
+            it.whole = a.ranges && cur.u == first && end == behind;
+            it.t0 = (cur.u - first) * unit;
+            it.t1 = min((end - first) * unit, len);
+            it.row0 = it.whole ? lo : (a.ranges ? piece + lo : (int64_t)(cur.u - first) * a.batch + lo);
+            cur.u = end;
         } else {
-            it.b = bi / a.num_blocks; it.blk = bi - it.b * a.num_blocks;
+            it.b = cur.u / a.num_blocks;
+            const int blk = cur.u - it.b * a.num_blocks;
             len = a.b_seqlen[it.b];
             it.req = a.b_req_idx[it.b];
-            it.write = direct || it.blk < blocks_of(len);
+            it.write = a.direct || blk < blocks_of(len);
+            it.whole = a.direct;
             if (len > 0 && (it.req < 0 || it.req >= a.rtt_rows || len > a.rtt_cols)) {
                 if (threadIdx.x == 0) q8_report(1, it.req);
                 len = 0;
             }
+            it.t0 = blk * unit;
+            it.t1 = min(it.t0 + unit, len);
+            it.row0 = (int64_t)blk * a.batch + it.b;
+            ++cur.u;
         }
-        it.t0 = it.blk * a.seq_block_size;
-        it.t1 = min(it.t0 + a.seq_block_size, len);
         it.steps = it.t1 > it.t0 ? (it.t1 - it.t0 + R::kTokens - 1) / R::kTokens : 0;
-        return it;
+        return true;
     };
     const int tiles_per_kv = (a.group + kQ8HeadTile - 1) / kQ8HeadTile;   // more than 1 only with NH = 1
 
@@ -237,8 +276,8 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         const int64_t ssrc_stride = isv ? a.vs_stride_t : a.ks_stride_t;
         bool ok = !*s_abort;
         int done = 0, st = 0, phase = 1;                                  // the first pass over the ring finds it empty
-        for (int n = blockIdx.x; n < items && ok; n += gridDim.x) {
-          const ItemQ8 it = item_at(n);
+        ItemQ8 it;
+        while (ok && next_item(it)) {
           const int kv0 = it.hg * NH / tiles_per_kv;
           const int32_t* rtt = a.req_to_tokens + (it.steps > 0 ? (int64_t)it.req * a.rtt_stride : 0);
           const uint8_t* ksrc = a.k + (int64_t)kv0 * a.k_stride_h + piece * 16;
@@ -302,8 +341,8 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     bool ok = !*s_abort;
     int st = 0, phase = 0, done = 0;
 
-    for (int n = blockIdx.x; n < items && ok; n += gridDim.x) {
-    const ItemQ8 it = item_at(n);
+    ItemQ8 it;
+    while (ok && next_item(it)) {
     if (!it.write) continue;                             // a split behind the request's end: no steps either
     // head tiles of this CTA: kv heads kv0 .. kv0 + NH - 1, or (a group of more than 8 q heads, NH = 1) tile `sub` of one
     const int kv0 = it.hg * NH / tiles_per_kv, sub = it.hg * NH - kv0 * tiles_per_kv;
@@ -315,15 +354,16 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     float qs;
     {
         float x[32], amax = 0.f;
-        const T* qp = reinterpret_cast<const T*>(a.q) + ((int64_t)it.b * a.num_q_heads + h0 + g) * 128 + c * 16;
+        const int j = g % GT;
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + ((int64_t)it.b * a.num_q_heads + h0 + j) * 128 + c * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint4 u = g < nheads ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
+            const uint4 u = j < nheads ? *reinterpret_cast<const uint4*>(qp + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = Cvt<T>::to_f2(w[j]);
-                x[8 * i + 2 * j] = f.x; x[8 * i + 2 * j + 1] = f.y;
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = a.q_bf16 ? Cvt<__nv_bfloat16>::to_f2(w[k]) : Cvt<__half>::to_f2(w[k]);
+                x[8 * i + 2 * k] = f.x; x[8 * i + 2 * k + 1] = f.y;
                 amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
         }
@@ -404,7 +444,11 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
             l_run += p;
             wgt[i] = p * (vs[i] * v_mul);
         }
-        const uint32_t b0 = Cvt<__half>::pack(wgt[0], wgt[1]), b1 = Cvt<__half>::pack(wgt[2], wgt[3]);
+        // a weight is its f16 rounding plus the f16 rounding of what that left
+        uint32_t b0 = Cvt<__half>::pack(wgt[0], wgt[1]), b1 = Cvt<__half>::pack(wgt[2], wgt[3]);
+        const float2 r0 = Cvt<__half>::to_f2(b0), r1 = Cvt<__half>::to_f2(b1);
+        const uint32_t e0 = Cvt<__half>::pack(wgt[0] - r0.x, wgt[1] - r0.y), e1 = Cvt<__half>::pack(wgt[2] - r1.x, wgt[3] - r1.y);
+        if (GT == 4 && g >= 4) { b0 = e0; b1 = e1; }
         uint32_t vw[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) { const uint4 x = *reinterpret_cast<const uint4*>(vrow + ((i & 1) + 8 * (i >> 1)) * R::kPitchV); vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w; }
@@ -417,6 +461,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
                 codes_to_f16<CODE>(__byte_perm(vw[0][w], vw[1][w], sel), x0, x1);
                 codes_to_f16<CODE>(__byte_perm(vw[2][w], vw[3][w], sel), y0, y1);
                 mma_f16(acc[2 * w + h], x0, x1, y0, y1, b0, b1);
+                if constexpr (GT == 8) mma_f16(acc[2 * w + h], x0, x1, y0, y1, e0, e1);
             }
         }
     };
@@ -468,8 +513,12 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     if (ok && wt == 0) {
         const float f = l_run == 0.f ? 0.f : (v_ref * (1.f / 4096.f)) / l_run;            // of head g; no token: zeros
         const float lse = l_run == 0.f ? -INFINITY : ((m_ref == -INFINITY ? 0.f : m_ref) + log2f(l_run)) * kLn2Q8;
-        const int64_t row0 = (direct ? (int64_t)it.b : (int64_t)it.blk * a.batch + it.b) * a.num_q_heads + h0;
-        if (c == 0 && g < nheads) (direct ? a.lse : a.mid_lse)[row0 + g] = lse;
+        const int64_t row0 = it.row0 * a.num_q_heads + h0;
+        if constexpr (GT == 4) {                                          // roundings and rests meet
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j >> 2][j & 3] += __shfl_xor_sync(0xffffffffu, acc[j >> 2][j & 3], 2);
+        }
+        if (c == 0 && g < nheads) (it.whole ? a.lse : a.mid_lse)[row0 + g] = lse;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const float fk = __shfl_sync(0xffffffffu, f, 8 * c + 4 * k);
@@ -477,7 +526,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
                 float x[16];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) { x[2 * j] = acc[j][k] * fk; x[2 * j + 1] = acc[j][2 + k] * fk; }
-                store_row16(direct ? a.o : a.mid_o, (row0 + 2 * c + k) * 128 + 16 * g, x, direct ? a.o_dtype : ESP_DTYPE_F32);
+                store_row16(it.whole ? a.o : a.mid_o, (row0 + 2 * c + k) * 128 + 16 * g, x, it.whole ? a.o_dtype : ESP_DTYPE_F32);
             }
         }
     }
@@ -490,17 +539,28 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
 template <int W>
 __global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float* __restrict__ lse, const int32_t* __restrict__ b_seqlen,
                                                                  const float* __restrict__ mid_o, const float* __restrict__ mid_lse,
+                                                                 const int* __restrict__ parts,
                                                                  int batch, int num_heads, int num_blocks, int block_seq, int o_dtype) {
     const int pair = blockIdx.x, b = pair / num_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int len = b_seqlen[b];
-    const int n = len <= 0 ? 0 : min((len - 1) / block_seq + 1, num_blocks);
-    const int64_t bh = (int64_t)batch * num_heads;
+    int n;
+    int64_t bh, row0;                                          // rows from one split to the next, row of the first
+    if (parts != nullptr) {
+        n = parts[2 * b + 1];
+        if (n == 1) return;                                    // stage 1 has written the results
+        bh = num_heads;
+        row0 = (int64_t)parts[2 * b] * num_heads + (pair - b * num_heads);
+    } else {
+        const int len = b_seqlen[b];
+        n = len <= 0 ? 0 : min((len - 1) / block_seq + 1, num_blocks);
+        bh = (int64_t)batch * num_heads;
+        row0 = pair;
+    }
     __shared__ float s_m[W], s_l[W], s_o[W][128];
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j0 = warp; j0 < n; j0 += W * 32) {                // up to 32 splits of this warp at a time, one lse per lane
         const int j = j0 + W * lane;
-        const float x = j < n ? mid_lse[j * bh + pair] : -INFINITY;
+        const float x = j < n ? mid_lse[j * bh + row0] : -INFINITY;
         float mx = x;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -513,7 +573,7 @@ __global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float*
 #pragma unroll 8
         for (int i = 0; i < cnt; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float4 v = *reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + W * i) * bh + pair) * 128 + lane * 4);
+            const float4 v = *reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + W * i) * bh + row0) * 128 + lane * 4);
             acc.x = fmaf(wi, v.x, acc.x); acc.y = fmaf(wi, v.y, acc.y); acc.z = fmaf(wi, v.z, acc.z); acc.w = fmaf(wi, v.w, acc.w);
         }
     }
@@ -558,24 +618,31 @@ using namespace esp;
 
 namespace esp {
 
-template <typename T, int CODE>
-static int launch_stage1_q8(DecodeQ8Args& a, int64_t nblk, cudaStream_t s) {
+template <int CODE, int GT>
+static int launch_stage1_q8(DecodeQ8Args& a, cudaStream_t s) {
     // neighbouring kv heads to a CTA, four or two where they divide evenly and lie next to each other, as long as every SM gets
     // two CTAs; else one, whose tokens the four warps share (one request of 513 tokens, 8 kv heads: see the measurements below)
     const bool dense = a.group <= kQ8HeadTile && a.k_stride_h == 128 && a.v_stride_h == 128;
-    const int64_t tiles = nblk * a.batch * a.head_tiles;
+    const int64_t tiles = (int64_t)a.num_blocks * a.batch * a.head_tiles;
     if (tiles > 2147483647LL - 65536) return ESP_ERR_TOO_LARGE;
     const int nh = dense && a.head_tiles % 4 == 0 && tiles >= 4 * 2 * kNumSMs ? 4 : (dense && a.head_tiles % 2 == 0 && tiles >= 2 * 2 * kNumSMs ? 2 : 1);
     a.head_groups = a.head_tiles / nh;
-    a.num_blocks = (int)nblk;
     a.scale_vec = aligned16(a.k_scale) && aligned16(a.v_scale) && a.ks_stride_t % 4 == 0 && a.vs_stride_t % 4 == 0;
-    const int64_t items = tiles / nh, resident = 3 * kNumSMs;
-    a.compact = items > resident && a.batch <= kQ8MaxCompact && a.o == nullptr;
+    const int64_t resident = kQ8Resident;
+    int64_t items = tiles / nh;
+    a.ranges = 0;
+    if (a.parts != nullptr) {
+        const int per_step = 16 * (kQ8Warps / nh);
+        a.min_units = kQ8MinPiece / per_step;
+        a.ranges = (int)std::max<int64_t>(1, std::min(resident / a.head_groups, (a.batch * (int64_t)a.max_len + kQ8MinPiece - 1) / kQ8MinPiece));
+        items = (int64_t)a.ranges * a.head_groups;
+    }
+    a.counted = a.ranges > 0 || (items > resident && a.batch <= kQ8MaxCounted && !a.direct);
     const dim3 grid((unsigned)(items < resident ? items : resident));
 #define ESP_S1Q(NH)                                                                                                               \
     {                                                                                                                            \
-        ESP_CUDA_TRY(cudaFuncSetAttribute(decode_stage1_q8_kernel<T, CODE, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, RingQ8<NH>::kSmem)); \
-        decode_stage1_q8_kernel<T, CODE, NH><<<grid, kQ8Warps * 32 + 32, RingQ8<NH>::kSmem, s>>>(a);                                              \
+        ESP_CUDA_TRY(cudaFuncSetAttribute(decode_stage1_q8_kernel<CODE, NH, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, RingQ8<NH>::kSmem)); \
+        decode_stage1_q8_kernel<CODE, NH, GT><<<grid, kQ8Warps * 32 + 32, RingQ8<NH>::kSmem, s>>>(a);                                              \
     }
     if (nh == 4) ESP_S1Q(4) else if (nh == 2) ESP_S1Q(2) else ESP_S1Q(1)
 #undef ESP_S1Q
@@ -585,7 +652,7 @@ static int launch_stage1_q8(DecodeQ8Args& a, int64_t nblk, cudaStream_t s) {
 
 static int stage1_q8(DecodeQ8Args& a, int head_dim, int max_len, int dtype, int code, float sm_scale, cudaStream_t s) {
     if (!a.q || !a.k || !a.v || !a.k_scale || !a.v_scale || !a.req_to_tokens || !a.b_req_idx || !a.b_seqlen || a.batch < 0 ||
-        a.num_q_heads <= 0 || a.num_kv_heads <= 0 || a.num_q_heads % a.num_kv_heads || a.seq_block_size <= 0 || a.rtt_rows <= 0 ||
+        a.num_q_heads <= 0 || a.num_kv_heads <= 0 || a.num_q_heads % a.num_kv_heads || (a.seq_block_size <= 0 && !a.parts) || a.rtt_rows <= 0 ||
         a.rtt_cols <= 0 || a.pool_rows <= 0)
         return ESP_ERR_BAD_ARG;
     if (dtype != ESP_DTYPE_F16 && dtype != ESP_DTYPE_BF16) return ESP_ERR_BAD_ARG;
@@ -596,14 +663,31 @@ static int stage1_q8(DecodeQ8Args& a, int head_dim, int max_len, int dtype, int 
         a.v_stride_h % 16 || ((uintptr_t)a.k_scale & 3u) || ((uintptr_t)a.v_scale & 3u))
         return ESP_ERR_ALIGNMENT;
     const int64_t nblk = (max_len + (int64_t)a.seq_block_size - 1) / a.seq_block_size;
+    if (a.parts && (a.batch > kQ8MaxCounted || (max_len / 16 + 1) * (int64_t)a.batch > 2147483647LL)) return ESP_ERR_TOO_LARGE;
+    a.num_blocks = (int)nblk;
+    a.max_len = max_len;
     if (nblk * a.seq_block_size > 2147483647LL - 65536) return ESP_ERR_TOO_LARGE;
     a.group = a.num_q_heads / a.num_kv_heads;
     a.head_tiles = a.num_kv_heads * ((a.group + kQ8HeadTile - 1) / kQ8HeadTile);
     a.scale_log2 = (sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)head_dim)) * kLog2eQ8;
-    if (dtype == ESP_DTYPE_F16)
-        return code == ESP_CODE_INT8 ? launch_stage1_q8<__half, ESP_CODE_INT8>(a, nblk, s) : launch_stage1_q8<__half, ESP_CODE_E4M3>(a, nblk, s);
-    return code == ESP_CODE_INT8 ? launch_stage1_q8<__nv_bfloat16, ESP_CODE_INT8>(a, nblk, s)
-                                 : launch_stage1_q8<__nv_bfloat16, ESP_CODE_E4M3>(a, nblk, s);
+    a.q_bf16 = dtype == ESP_DTYPE_BF16;
+    if (code == ESP_CODE_INT8) return a.group <= 4 ? launch_stage1_q8<ESP_CODE_INT8, 4>(a, s) : launch_stage1_q8<ESP_CODE_INT8, 8>(a, s);
+    return a.group <= 4 ? launch_stage1_q8<ESP_CODE_E4M3, 4>(a, s) : launch_stage1_q8<ESP_CODE_E4M3, 8>(a, s);
+}
+
+static DecodeQ8Args args_q8(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, int64_t k_stride_t,
+                            int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, int64_t k_scale_stride_t, int64_t v_scale_stride_t,
+                            const int32_t* req_to_tokens, int64_t req_to_tokens_stride, int32_t req_rows, int32_t req_cols,
+                            const int32_t* b_req_idx, const int32_t* b_seqlen, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                            int64_t pool_rows) {
+    DecodeQ8Args a{};
+    a.q = q; a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.k_scale = k_scale; a.v_scale = v_scale;
+    a.k_stride_t = k_stride_t; a.k_stride_h = k_stride_h; a.v_stride_t = v_stride_t; a.v_stride_h = v_stride_h;
+    a.ks_stride_t = k_scale_stride_t; a.vs_stride_t = v_scale_stride_t;
+    a.req_to_tokens = req_to_tokens; a.rtt_stride = req_to_tokens_stride; a.rtt_rows = req_rows; a.rtt_cols = req_cols;
+    a.b_req_idx = b_req_idx; a.b_seqlen = b_seqlen; a.batch = batch; a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads;
+    a.pool_rows = pool_rows;
+    return a;
 }
 
 }  // namespace esp
@@ -617,9 +701,10 @@ extern "C" int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q,
                                     int64_t pool_rows, void* stream) {
     if (batch == 0 || max_len_in_batch <= 0) return ESP_OK;
     if (!mid_o || !mid_lse) return ESP_ERR_BAD_ARG;
-    DecodeQ8Args a{mid_o, mid_lse, q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h,
-                   k_scale_stride_t, v_scale_stride_t, req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch,
-                   num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0, 0, 0, nullptr, nullptr, 0};
+    DecodeQ8Args a = args_q8(q, k, v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t,
+                             req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads,
+                             pool_rows);
+    a.mid_o = mid_o; a.mid_lse = mid_lse; a.seq_block_size = seq_block_size;
     return stage1_q8(a, head_dim, max_len_in_batch, dtype, code, sm_scale, (cudaStream_t)stream);
 }
 
@@ -631,25 +716,32 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
                                        int32_t num_kv_heads, int32_t head_dim, int32_t max_len_in_batch, int32_t seq_block_size,
                                        int32_t dtype, int32_t o_dtype, int32_t code, float sm_scale, int64_t pool_rows, void* stream) {
     if (batch == 0) return ESP_OK;
-    if (!o || !lse || max_len_in_batch < 0 || seq_block_size <= 0) return ESP_ERR_BAD_ARG;
+    if (!o || !lse || max_len_in_batch < 0 || seq_block_size < 0 || num_q_heads <= 0) return ESP_ERR_BAD_ARG;
     if (o_dtype != ESP_DTYPE_F16 && o_dtype != ESP_DTYPE_BF16 && o_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
     const int32_t max_len = max_len_in_batch > 0 ? max_len_in_batch : 1;
-    const int64_t nblk = (max_len + (int64_t)seq_block_size - 1) / seq_block_size;
+    // seq_block_size 0: equal pieces, or one split where a request has no more than a piece's least length
+    const bool even = seq_block_size == 0 && max_len > kQ8MinPiece;
+    const int32_t block = seq_block_size == 0 ? kQ8MinPiece : seq_block_size;
+    const int64_t nblk = (max_len + (int64_t)block - 1) / block;
     if (nblk > 1 && !workspace) return ESP_ERR_BAD_ARG;
     if (nblk > 1 && !aligned16(workspace)) return ESP_ERR_ALIGNMENT;
-    const int64_t rows = nblk * batch * num_q_heads;
-    DecodeQ8Args a{workspace, workspace + rows * 128, q, (const uint8_t*)k, (const uint8_t*)v, k_scale, v_scale, k_stride_t, k_stride_h,
-                   v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t, req_to_tokens, req_to_tokens_stride, req_rows, req_cols,
-                   b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads, 0, seq_block_size, 0.f, pool_rows, 0, 0, 0, 0, 0,
-                   nblk == 1 ? o : nullptr, nblk == 1 ? lse : nullptr, o_dtype};
+    DecodeQ8Args a = args_q8(q, k, v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t,
+                             req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads,
+                             pool_rows);
+    const int64_t rows = even ? (std::min<int64_t>(kQ8Resident, (batch * (int64_t)max_len + kQ8MinPiece - 1) / kQ8MinPiece) + batch) * num_q_heads
+                              : nblk * batch * num_q_heads;
+    a.mid_o = workspace; a.mid_lse = workspace + rows * 128; a.seq_block_size = block;
+    a.o = o; a.lse = lse; a.o_dtype = o_dtype; a.direct = nblk == 1;
+    if (even) a.parts = reinterpret_cast<int*>(workspace + rows * 129);
     cudaStream_t s = (cudaStream_t)stream;
     const int rc = stage1_q8(a, head_dim, max_len, dtype, code, sm_scale, s);
     if (rc || nblk == 1) return rc;
     const unsigned pairs = (unsigned)((int64_t)batch * num_q_heads);
-    if (nblk > 64)
-        decode_merge_q8_kernel<16><<<pairs, 512, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, batch, num_q_heads, (int)nblk, seq_block_size, o_dtype);
+    // splits of one request, on average
+    if ((even ? a.ranges / batch : nblk) > 64)
+        decode_merge_q8_kernel<16><<<pairs, 512, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, a.parts, batch, num_q_heads, (int)nblk, block, o_dtype);
     else
-        decode_merge_q8_kernel<4><<<pairs, 128, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, batch, num_q_heads, (int)nblk, seq_block_size, o_dtype);
+        decode_merge_q8_kernel<4><<<pairs, 128, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, a.parts, batch, num_q_heads, (int)nblk, block, o_dtype);
     ESP_LAUNCH_CHECK("decode_merge_q8_kernel");
     return ESP_OK;
 }

@@ -81,10 +81,13 @@ def flash_decoding_stage1_q8(mid_o, mid_o_logexpsum, q, k, k_scale, v, v_scale, 
         _lib.check(rc, "esp_decode_stage1_q8")
 
 
+Q8_MAX_EVEN = 384          # requests whose tokens one call divides evenly
+
+
 def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -> int:
-    """Tokens per split: eight times as many (split, heads) items as the GPU holds CTAs, within 128 and 512 tokens.  Shorter splits cost
-    partials, longer ones leave a tail: 32 requests x 1K-16K tokens x 32 heads take 476 / 401 / 405 / 427 / 475 us with 128 / 256 /
-    512 / 1024 / 2048."""
+    """Tokens per split, where splits have a fixed length: eight times as many (split, heads) items as the GPU holds CTAs, within 128
+    and 512 tokens.  Shorter splits cost partials, longer ones leave a tail: 32 requests x 1K-16K tokens x 32 heads take 473 / 430 /
+    404 / 427 / 467 us with 128 / 256 / 512 / 1024 / 2048."""
     tiles = batch * kv_heads * ((group + 7) // 8)
     splits = max(1, -(-148 * 3 * 8 * 4 // max(1, tiles)))
     return min(512, max(128, -(-max(int(max_len_in_batch), 1) // splits // 128) * 128))
@@ -93,7 +96,9 @@ def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -
 def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len,
                               max_len_in_batch: int, block_seq=None, out=None, out_logexpsum=None, sm_scale: float = 0.0):
     """Decode attention over a pool held in 8 bits, splits and merge in one call: (o like q unless ``out`` is given, lse fp32).
-    ``block_seq``: tokens per split, chosen from the sizes by default.  A request of length zero gets o = 0, lse = -inf."""
+    ``block_seq``: tokens per split; by default the tokens of up to 384 requests are divided evenly over the GPU (398 us for 32 requests
+    x 1K-16K tokens x 32 heads, 185 us for 2 x 262144 x 8; with the best fixed length 404 and 206).  A request of length zero gets
+    o = 0, lse = -inf."""
     dev = need_here(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len, out, out_logexpsum)
     args, slots = _q8_args(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len)
     batch, hq, hkv, dim = args[-4:]
@@ -109,9 +114,14 @@ def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_toke
         if out_logexpsum.dtype != torch.float32:
             raise TypeError("out_logexpsum is fp32")
     tags = dtype16_tag(q), dtype_tag(out), code_tag(cache_k)
-    block = int(block_seq) if block_seq is not None else q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len)
-    nblk = (max_len + block - 1) // block
-    work = k_scale.new_empty(nblk * batch * hq * (dim + 1)) if nblk > 1 else None
+    if block_seq is None and batch <= Q8_MAX_EVEN:
+        block = 0
+        floats = (min(444, (batch * max_len + 127) // 128) + batch) * hq * (dim + 1) + 2 * batch if max_len > 128 else 0
+    else:
+        block = int(block_seq) if block_seq is not None else q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len)
+        nblk = (max_len + block - 1) // block
+        floats = nblk * batch * hq * (dim + 1) if nblk > 1 else 0
+    work = k_scale.new_empty(floats) if floats else None
     rc = _lib.attn().esp_decode_attention_q8(out.data_ptr(), out_logexpsum.data_ptr(), ptr(work), *args, max_len, block, *tags, sm_scale,
                                              slots, stream_of(dev))
     if rc:

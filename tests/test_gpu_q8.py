@@ -175,13 +175,14 @@ def decode_case(lens, hq, hkv, dtype, code, seed, q_scale=1.5, pool_extra=3):
 
 
 def decode_exact(c, lens=None, sm_scale=None):
-    """(o, lse, sum p|v| / sum p, max over tokens of sum|q k| * sm_scale, tokens * largest v scale * top code) in 64 bits."""
+    """(o, lse, sum p|v| / sum p, max over tokens of sum|q k| * sm_scale, the same of max|q| * sum|k|, tokens * largest v scale * top
+    code) in 64 bits."""
     B, hq, _ = c["q"].shape
     hkv = c["hkv"]
     sm = sm_scale or D ** -0.5
     o = torch.zeros(B, hq, D, dtype=torch.float64); lse = torch.full((B, hq), -math.inf, dtype=torch.float64)
     wabs = torch.zeros_like(o); sabs = torch.zeros(B, hq, dtype=torch.float64)
-    floor = torch.zeros(B, hq, 1, dtype=torch.float64)
+    floor = torch.zeros(B, hq, 1, dtype=torch.float64); qabs = torch.zeros_like(sabs)
     for b, n in enumerate(lens if lens is not None else c["lens"].tolist()):
         if n == 0:
             continue
@@ -197,20 +198,22 @@ def decode_exact(c, lens=None, sm_scale=None):
         o[b] = (p[..., None] * v).sum(0).cpu(); wabs[b] = (p[..., None] * v.abs()).sum(0).cpu()
         lse[b] = torch.logsumexp(s, 0).cpu()
         sabs[b] = ((q[None] * k).abs().sum(-1) * sm).amax(0).cpu()
+        qabs[b] = (q.abs().amax(-1)[None] * k.abs().sum(-1) * sm).amax(0).cpu()
         top = c["scales"][slots, hkv:].double().amax(0).repeat_interleave(hq // hkv) * TOP[c["codes"].dtype]
         floor[b, :, 0] = len(slots) * top.cpu()
-    return o, lse, wabs, sabs, floor
+    return o, lse, wabs, sabs, qabs, floor
 
 
 def check_decode(o, lse, ref, n_max):
-    """Roundings: a score is a sum of 128 products and three factors (at most 131 * 2^-24 of sum|q k|); p carries the score's
-    error, one more of 2^-22 (ex2) and the rounding of p * v_scale to f16 before the second product (2^-11 relative; below f16's
-    normal range 2^-25 absolute of a number that is held as p * v_scale * 2^12 / v_ref with v_ref <= 4 * the largest v_scale, while
-    some p is 1 and so sum p >= 1: at most 2^-25 * 4 / 2^12 = 2^-35 of the largest v_scale * top code for each of n tokens); sums of
-    n terms in fp32 lose at most n * 2^-24 of the sum of magnitudes; the output is rounded once."""
-    ro, rl, wabs, sabs, floor = ref
-    ds = 131 * U32 * sabs
-    tol = ((2.0 ** -11 + 2.0 ** -20 + 2 * min(n_max, 4096) * U32) + 2 * ds)[..., None] * wabs
+    """Roundings.  A score is a sum of 128 products and three factors, at most 131 * 2^-24 of sum|q k|, of a query held in f16 with its
+    largest element scaled to [2^7, 2^8): exact, but for elements below f16's normal range, which are off by at most 2^-25 * 2^-7 of the
+    largest.  p carries the score's error and one more of 2^-22 (ex2).  The weight p * v_scale * 2^12 / v_ref with v_ref <= 4 * the
+    largest v_scale, while some p is 1 and so sum p >= 1, is held as the f16 rounding of itself and of what that left (2^-22 relative;
+    below f16's normal range 2^-25 absolute: at most 2^-25 * 4 / 2^12 = 2^-35 of the largest v_scale * top code for each of n tokens).
+    Sums of n terms in fp32 lose at most n * 2^-24 of the sum of magnitudes; the output is rounded once."""
+    ro, rl, wabs, sabs, qabs, floor = ref
+    ds = 131 * U32 * sabs + 2.0 ** -32 * qabs
+    tol = ((2.0 ** -22 + 2.0 ** -20 + 2 * min(n_max, 4096) * U32) + 2 * ds)[..., None] * wabs
     tol = tol + 2.0 ** -35 * floor + (half_step(o.dtype) if o.dtype != torch.float32 else U32) * ro.abs() * 1.01 + 1e-30
     if o.dtype == F16:
         tol = tol + 2.0 ** -25
@@ -260,6 +263,70 @@ def test_decode_partials_are_the_blocks_own_attention(code):
                 continue
             part = dict(c, table=c["table"][:, j * bs:], q=c["q"][b:b + 1], rows=c["rows"][b:b + 1])
             check_decode(mid_o[j, b:b + 1], mid_l[j, b:b + 1], decode_exact(part, [m]), m)
+
+
+@pytest.mark.parametrize("code,hq,hkv,lens", [
+    (INT8, 32, 32, [5000, 0, 1, 129, 700, 0, 2600]), (E4M3, 8, 1, [9000]), (INT8, 4, 4, [40] * 200 + [0, 0, 7] + [3000, 2999]),
+    (E4M3, 16, 2, [0] * 5 + [129] + [0] * 5), (INT8, 24, 8, [128 * (i % 5) + i for i in range(384)]), (INT8, 8, 8, [33 * (i % 9) for i in range(385)]),
+    (E4M3, 32, 4, [1] * 300 + [4096]), (INT8, 8, 2, [20000, 64, 20001])])
+def test_decode_pieces_across_requests(code, hq, hkv, lens):
+    """Divided evenly, a piece ends anywhere in a request and holds the ends of several."""
+    from loongserve_b200 import flash_decoding as fd
+    c = decode_case(lens, hq, hkv, BF16, code, seed=len(lens) + hq)
+    out = torch.full((len(lens), hq, D), 9.0, device=DEV); lse = torch.full((len(lens), hq), 9.0, device=DEV)
+    fd.token_decode_attention_q8(c["q"], c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"], c["rows"],
+                                 c["lens"], max(lens), None, out, lse)
+    check_decode(out, lse, decode_exact(c), max(lens))
+    assert fd.device_status()[0] == 0
+
+
+def test_decode_pieces_follow_the_lengths_of_a_replay():
+    """Captured once; lengths, rows and tokens are read when the graph runs.  Two graphs have a workspace each."""
+    from loongserve_b200 import flash_decoding as fd
+    hq, hkv = 8, 4
+    c = decode_case([900, 31, 1500, 2], hq, hkv, BF16, INT8, 77)
+    a = (c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"], c["rows"], c["lens"], 1500)
+    fd.token_decode_attention_q8(c["q"], *a)
+    torch.cuda.synchronize()
+    q2 = c["q"].flip(0).contiguous()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    res = []
+    for gr, q in zip(graphs, (c["q"], q2)):
+        with torch.cuda.graph(gr):
+            res.append(fd.token_decode_attention_q8(q, *a))
+    for lens in ([900, 31, 1500, 2], [1, 0, 1499, 2], [0, 0, 0, 0], [128, 31, 129, 1]):
+        c["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for (o, lse), q in zip(res, (c["q"], q2)):
+            check_decode(o, lse, decode_exact(dict(c, q=q)), 1500)
+
+
+def test_decode_pieces_stop_at_the_given_longest():
+    """No token behind max_len_in_batch is read; slots and rows outside are reported and left out, as with splits."""
+    from loongserve_b200 import flash_decoding as fd
+    fd.device_status()
+    c = decode_case([600, 400, 500], 8, 2, BF16, E4M3, 13)
+    r0 = int(c["rows"][0])
+    a = (c["codes"][:, :2], c["scales"][:, :2], c["codes"][:, 2:], c["scales"][:, 2:], c["table"])
+    out = torch.empty(3, 8, D, device=DEV); lse = torch.empty(3, 8, device=DEV)
+    fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 450, None, out, lse)
+    check_decode(out, lse, decode_exact(c, [450, 400, 450]), 450)
+    assert fd.device_status()[0] == 0
+    c["table"][r0, 5] = 2147483647; c["table"][r0, 400] = -3; c["table"][r0, 599] = c["codes"].shape[0]
+    fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 600, None, out, lse)
+    check_decode(out, lse, decode_exact(c), 600)
+    st = fd.device_status()
+    assert st[0] == -8 and st[2] == 0 and st[3] in (2147483647, -3, c["codes"].shape[0])
+    rows = c["rows"].clone(); rows[1] = 99; rows[2] = -1
+    lens = c["lens"].clone(); lens[0] = c["table"].shape[1] + 1                                # longer than the table is wide
+    fd.token_decode_attention_q8(c["q"], *a, rows, lens, 600, None, out, lse)
+    assert fd.device_status()[0] == -8
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
 def test_decode_scores_and_scales_of_every_size():

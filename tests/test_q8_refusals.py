@@ -73,6 +73,19 @@ def test_decode_stage1(lib, change, rc):
 
 
 @pytest.mark.parametrize("change,rc", [
+    (dict(batch=0), 0), (dict(o=None), BAD), (dict(lse=None), BAD), (dict(work=None), BAD), (dict(work=P + 4), ALIGN), (dict(block=-1), BAD),
+    (dict(max_len=-1), BAD), (dict(odt=3), BAD), (dict(batch=385), LARGE), (dict(batch=384, max_len=2147483647), LARGE), (dict(hq=0), BAD),
+    (dict(q=None), BAD), (dict(kst=520), ALIGN), (dict(dim=64), UNSUP), (dict(block=16, work=None), BAD)])
+def test_decode_attention(lib, change, rc):
+    """block 0: the tokens are divided evenly."""
+    base = dict(o=P, lse=P, work=P, **{k: v for k, v in DECODE.items() if k not in ("mid_o", "mid_lse")})
+    base.update(max_len=5000, block=0)
+    keys = list(base); at = keys.index("dtype") + 1
+    base = {**{k: base[k] for k in keys[:at]}, "odt": 1, **{k: base[k] for k in keys[at:]}}
+    assert call(lib.esp_decode_attention_q8, base, **change) == rc
+
+
+@pytest.mark.parametrize("change,rc", [
     (dict(tokens=0), 0), (dict(tokens=-1), BAD), (dict(hidden=0), BAD), (dict(hidden=60), ALIGN), (dict(hidden=65544), LARGE), (dict(dtype=2), BAD),
     (dict(inp=None), BAD), (dict(weight=None), BAD), (dict(residual=P + 4), ALIGN), (dict(inp=P + 2), ALIGN), (dict(weight=P + 8), ALIGN),
     (dict(tokens=1 << 31), LARGE)])
