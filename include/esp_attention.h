@@ -435,8 +435,8 @@ int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q, const void
  * workspace: ceil(max(max_len_in_batch, 1) / seq_block_size) * batch * Hq * (D + 1) floats, 16-byte aligned, used by this call
  * alone until it has run (may be NULL when there is one split: the results are then written at once).  seq_block_size 0: the
  * tokens of up to 384 requests are divided evenly over the GPU, none behind max_len_in_batch is read; workspace:
- * (min(444, ceil(batch * max_len_in_batch / 128)) + batch) * Hq * (D + 1) + 2 * batch floats, NULL up to a max_len_in_batch of
- * 128.  Other arguments as esp_decode_stage1_q8.  A request of length zero gets o = 0, lse = -inf. */
+ * (min(444, ceil(batch * max_len_in_batch / 64)) + batch) * Hq * (D + 1) + 2 * batch floats, NULL up to a max_len_in_batch of
+ * 256.  Other arguments as esp_decode_stage1_q8.  A request of length zero gets o = 0, lse = -inf. */
 int esp_decode_attention_q8(void* o, float* lse, float* workspace, const void* q, const void* k, const void* v,
                             const float* k_scale, const float* v_scale, int64_t k_stride_t, int64_t k_stride_h,
                             int64_t v_stride_t, int64_t v_stride_h, int64_t k_scale_stride_t,

@@ -53,11 +53,17 @@ struct DecodeQ8Args {
 };
 
 constexpr int kQ8Warps = 4, kQ8HeadTile = 8;
-constexpr int kQ8Resident = 3 * kNumSMs, kQ8MinPiece = 128;     // CTAs the GPU holds; tokens below which a piece is not cut
+constexpr int kQ8Resident = 3 * kNumSMs, kQ8MinPiece = 64;       // CTAs the GPU holds; tokens below which a piece is not cut
+constexpr int kQ8Whole = 256;                                    // requests up to this length are not cut at all
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Four codes of a word as two f16 pairs: codes 0, 1 and codes 2, 3.  int8: code + 128 placed under the exponent of 1024 is
@@ -349,11 +355,14 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     const int nheads = min(kQ8HeadTile, a.group - sub * kQ8HeadTile);
     const int h0 = (kv0 + hw) * a.group + sub * kQ8HeadTile;
 
-    // Q fragments: row g is head g of the tile (rows 8-15 of the MMA stay zero), dims in the order of the K words
-    uint32_t qf[8][2];
+    // Q fragments, dims in the order of the K words
+    constexpr bool kInt = CODE == ESP_CODE_INT8;
+    constexpr int kQExp = !kInt ? 7 : (GT == 4 ? 29 : 21);
+    uint32_t qf[8][kInt ? (GT == 4 ? 2 : 3) : 2];
     float qs;
     {
-        float x[32], amax = 0.f;
+        float x[32];
+        uint32_t amax = 0;
         const int j = g % GT;
         const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + ((int64_t)it.b * a.num_q_heads + h0 + j) * 128 + c * 16;
 #pragma unroll
@@ -364,20 +373,36 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
             for (int k = 0; k < 4; ++k) {
                 const float2 f = a.q_bf16 ? Cvt<__nv_bfloat16>::to_f2(w[k]) : Cvt<__half>::to_f2(w[k]);
                 x[8 * i + 2 * k] = f.x; x[8 * i + 2 * k + 1] = f.y;
-                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                amax = max(amax, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
             }
         }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^(7 - e) with 2^e <= amax; e held in [-100, 126] so that both powers are normal numbers
-        int e = (int)(__float_as_uint(amax) >> 23) - 127;
-        e = min(max(e, -100), 126);
-        const float up = __uint_as_float((uint32_t)(127 + 7 - e) << 23);
-        qs = a.scale_log2 * __uint_as_float((uint32_t)(127 - 7 + e) << 23);
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const bool finite = amax < 0x7f800000u;              // a query with inf or NaN: NaN
+        // 2^(kQExp - e) with 2^e <= max|q|; e held in [-90, 126] so that both powers are normal numbers
+        const int e = min(max((int)(amax >> 23) - 127, -90), 126);
+        const float up = __uint_as_float((uint32_t)(127 + kQExp - e) << 23);
+        qs = finite ? a.scale_log2 * __uint_as_float((uint32_t)(127 - kQExp + e) << 23) : __uint_as_float(0x7fc00000u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            qf[j][0] = Cvt<__half>::pack(x[4 * j] * up, x[4 * j + 1] * up);
-            qf[j][1] = Cvt<__half>::pack(x[4 * j + 2] * up, x[4 * j + 3] * up);
+        for (int k = 0; k < 8; ++k) {
+            if constexpr (kInt) {
+                uint32_t word[4] = {};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    int v = __float2int_rn(finite ? x[4 * k + i] * up : 0.f);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {            // balanced: digits from -128 to 127
+                        const int low = (int)(int8_t)v;
+                        word[d] |= ((uint32_t)v & 255u) << (8 * i);
+                        v = (v - low) >> 8;
+                    }
+                }
+                if constexpr (GT == 4) { qf[k][0] = g < 4 ? word[0] : word[1]; qf[k][1] = g < 4 ? word[2] : word[3]; }
+                else { qf[k][0] = word[0]; qf[k][1] = word[1]; qf[k][2] = word[2]; }
+            } else {
+                qf[k][0] = Cvt<__half>::pack(x[4 * k] * up, x[4 * k + 1] * up);
+                qf[k][1] = Cvt<__half>::pack(x[4 * k + 2] * up, x[4 * k + 3] * up);
+            }
         }
     }
 
@@ -390,24 +415,48 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         const uint8_t* vrow = d + R::kOffV + (wt * 16 + 2 * c) * R::kPitchV + hw * 128 + g * 16;
         const float* scl = reinterpret_cast<const float*>(d + R::kOffScale) + wt * 16 * NH + hw;
         const uint32_t present = *reinterpret_cast<const uint32_t*>(d + R::kOffPresent + 4 * wt);
-        float s[2][4] = {};
+        float sc[4], vs[4];               // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint4 x = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitchK);
             const uint4 y = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitchK + 64);
             const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            if constexpr (kInt) {
+                // a sum of 128 products of a digit and a code is below 2^21: counted in the last places of 1.5 * 2^23, it is a float
+                constexpr int kBase = 0x4b400000;
+                constexpr float kZero = 12582912.f;
+                int d[4] = {kBase, kBase, kBase, kBase}, d2[4] = {kBase, kBase, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t lo, hi;
-                codes_to_f16<CODE>(w[j], lo, hi);
-                mma_f16(s[i], qf[j][0], 0u, qf[j][1], 0u, lo, hi);
+                for (int j = 0; j < 4; ++j) {
+                    mma_s8(d, qf[2 * j][0], qf[2 * j][1], qf[2 * j + 1][0], qf[2 * j + 1][1], w[2 * j], w[2 * j + 1]);
+                    if constexpr (GT == 8) mma_s8(d2, qf[2 * j][2], 0u, qf[2 * j + 1][2], 0u, w[2 * j], w[2 * j + 1]);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float lo = __int_as_float(d[k]) - kZero, hi = __int_as_float(d[2 + k]) - kZero;
+                    if constexpr (GT == 4) {                  // digits 0 and 2 here, 1 and 3 in the lane of row g ^ 4
+                        float u = fmaf(hi, 65536.f, lo);
+                        u = g < 4 ? u : 256.f * u;
+                        sc[2 * i + k] = u + __shfl_xor_sync(0xffffffffu, u, 16);
+                    } else {
+                        sc[2 * i + k] = fmaf(__int_as_float(d2[k]) - kZero, 65536.f, fmaf(hi, 256.f, lo));
+                    }
+                }
+            } else {
+                float s[4] = {};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t lo, hi;
+                    codes_to_f16<CODE>(w[j], lo, hi);
+                    mma_f16(s, qf[j][0], 0u, qf[j][1], 0u, lo, hi);
+                }
+                sc[2 * i] = s[0]; sc[2 * i + 1] = s[1];
             }
         }
-        float sc[4], vs[4];               // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = 2 * c + (i & 1) + 8 * (i >> 1);
-            sc[i] = s[i >> 1][i & 1] * (scl[t * NH] * qs);
+            sc[i] *= scl[t * NH] * qs;
             vs[i] = scl[(R::kTokens + t) * NH];
         }
         if (present != 0xffffu) {         // zeros were copied for the others: only their scores need a word
@@ -620,12 +669,13 @@ namespace esp {
 
 template <int CODE, int GT>
 static int launch_stage1_q8(DecodeQ8Args& a, cudaStream_t s) {
-    // neighbouring kv heads to a CTA, four or two where they divide evenly and lie next to each other, as long as every SM gets
-    // two CTAs; else one, whose tokens the four warps share (one request of 513 tokens, 8 kv heads: see the measurements below)
+    // Neighbouring kv heads to a CTA, four or two where they divide evenly and lie next to each other, as long as every SM gets a CTA;
+    // else one, whose tokens the four warps share.  4 requests x 512 tokens x 32 kv heads: 11.9 us with four heads, 14.8 with one;
+    // 4 x 1000 x 8 kv heads: 14.2 and 12.0.
     const bool dense = a.group <= kQ8HeadTile && a.k_stride_h == 128 && a.v_stride_h == 128;
     const int64_t tiles = (int64_t)a.num_blocks * a.batch * a.head_tiles;
     if (tiles > 2147483647LL - 65536) return ESP_ERR_TOO_LARGE;
-    const int nh = dense && a.head_tiles % 4 == 0 && tiles >= 4 * 2 * kNumSMs ? 4 : (dense && a.head_tiles % 2 == 0 && tiles >= 2 * 2 * kNumSMs ? 2 : 1);
+    const int nh = dense && a.head_tiles % 4 == 0 && tiles >= 4 * kNumSMs ? 4 : (dense && a.head_tiles % 2 == 0 && tiles >= 2 * kNumSMs ? 2 : 1);
     a.head_groups = a.head_tiles / nh;
     a.scale_vec = aligned16(a.k_scale) && aligned16(a.v_scale) && a.ks_stride_t % 4 == 0 && a.vs_stride_t % 4 == 0;
     const int64_t resident = kQ8Resident;
@@ -719,9 +769,11 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     if (!o || !lse || max_len_in_batch < 0 || seq_block_size < 0 || num_q_heads <= 0) return ESP_ERR_BAD_ARG;
     if (o_dtype != ESP_DTYPE_F16 && o_dtype != ESP_DTYPE_BF16 && o_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
     const int32_t max_len = max_len_in_batch > 0 ? max_len_in_batch : 1;
-    // seq_block_size 0: equal pieces, or one split where a request has no more than a piece's least length
-    const bool even = seq_block_size == 0 && max_len > kQ8MinPiece;
-    const int32_t block = seq_block_size == 0 ? kQ8MinPiece : seq_block_size;
+    // seq_block_size 0: equal pieces, or one split where no request is longer than 256 tokens, which saves the merge (pieces / one
+    // split, 8 kv heads, group 4: one request of 256 tokens 10.3 / 9.5 us, of 512 10.9 / 13.2; 64 ragged ones of up to 256
+    // 18.2 / 12.2; 256 of them 36.7 / 30.4, of up to 512 53.1 / 61.2)
+    const bool even = seq_block_size == 0 && max_len > kQ8Whole;
+    const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : kQ8Whole) : seq_block_size;
     const int64_t nblk = (max_len + (int64_t)block - 1) / block;
     if (nblk > 1 && !workspace) return ESP_ERR_BAD_ARG;
     if (nblk > 1 && !aligned16(workspace)) return ESP_ERR_ALIGNMENT;

@@ -116,7 +116,7 @@ def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_toke
     tags = dtype16_tag(q), dtype_tag(out), code_tag(cache_k)
     if block_seq is None and batch <= Q8_MAX_EVEN:
         block = 0
-        floats = (min(444, (batch * max_len + 127) // 128) + batch) * hq * (dim + 1) + 2 * batch if max_len > 128 else 0
+        floats = (min(444, (batch * max_len + 63) // 64) + batch) * hq * (dim + 1) + 2 * batch if max_len > 256 else 0
     else:
         block = int(block_seq) if block_seq is not None else q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len)
         nblk = (max_len + block - 1) // block

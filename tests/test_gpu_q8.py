@@ -205,14 +205,14 @@ def decode_exact(c, lens=None, sm_scale=None):
 
 
 def check_decode(o, lse, ref, n_max):
-    """Roundings.  A score is a sum of 128 products and three factors, at most 131 * 2^-24 of sum|q k|, of a query held in f16 with its
-    largest element scaled to [2^7, 2^8): exact, but for elements below f16's normal range, which are off by at most 2^-25 * 2^-7 of the
-    largest.  p carries the score's error and one more of 2^-22 (ex2).  The weight p * v_scale * 2^12 / v_ref with v_ref <= 4 * the
+    """Roundings.  A score is a sum of 128 products and three factors, at most 131 * 2^-24 of sum|q k|, of a query whose
+    elements are held to 2^-22 of the largest (int8 codes: rounded to integers, the largest at least 2^21 of them; e4m3: f16, the largest
+    scaled to [2^7, 2^8), exact but below f16's normal range, 2^-25 * 2^-7).  p carries the score's error and one more of 2^-22 (ex2).  The weight p * v_scale * 2^12 / v_ref with v_ref <= 4 * the
     largest v_scale, while some p is 1 and so sum p >= 1, is held as the f16 rounding of itself and of what that left (2^-22 relative;
     below f16's normal range 2^-25 absolute: at most 2^-25 * 4 / 2^12 = 2^-35 of the largest v_scale * top code for each of n tokens).
     Sums of n terms in fp32 lose at most n * 2^-24 of the sum of magnitudes; the output is rounded once."""
     ro, rl, wabs, sabs, qabs, floor = ref
-    ds = 131 * U32 * sabs + 2.0 ** -32 * qabs
+    ds = 131 * U32 * sabs + 2.0 ** -22 * qabs
     tol = ((2.0 ** -22 + 2.0 ** -20 + 2 * min(n_max, 4096) * U32) + 2 * ds)[..., None] * wabs
     tol = tol + 2.0 ** -35 * floor + (half_step(o.dtype) if o.dtype != torch.float32 else U32) * ro.abs() * 1.01 + 1e-30
     if o.dtype == F16:
