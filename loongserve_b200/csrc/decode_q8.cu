@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     int* s_len = reinterpret_cast<int*>(smem + R::kOffLen);               // -1: the request's row is not in the table
     int* s_first = s_len + kQ8MaxCounted;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == kQ8Warps * 32) {                                   // not a thread that waits for the first lengths
         *s_abort = *reinterpret_cast<volatile int*>(&g_decode_q8_status[0]) == ESP_ERR_DEVICE_TIMEOUT ? 1 : 0;
         for (int i = 0; i < R::kStages; ++i) { ptx::mbar_init(full(i), 33); ptx::mbar_init(empty(i), kQ8Warps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -386,19 +386,19 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if constexpr (kInt) {
-                uint32_t word[4] = {};
+                // balanced digits, -128 to 127 each: with 128 added to every lower digit the bytes are digit + 128
+                uint32_t v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    int v = __float2int_rn(finite ? x[4 * k + i] * up : 0.f);
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {            // balanced: digits from -128 to 127
-                        const int low = (int)(int8_t)v;
-                        word[d] |= ((uint32_t)v & 255u) << (8 * i);
-                        v = (v - low) >> 8;
-                    }
+                for (int i = 0; i < 4; ++i) v[i] = ((uint32_t)__float2int_rn(finite ? x[4 * k + i] * up : 0.f) + 0x00808080u) ^ 0x00808080u;
+                if constexpr (GT == 4) {                     // lanes of rows 0-3: digits 0 and 2; of rows 4-7: 1 and 3
+                    const uint32_t sel = g < 4 ? 0x6240 : 0x7351;
+                    const uint32_t t0 = __byte_perm(v[0], v[1], sel), t1 = __byte_perm(v[2], v[3], sel);
+                    qf[k][0] = __byte_perm(t0, t1, 0x5410); qf[k][1] = __byte_perm(t0, t1, 0x7632);
+                } else {
+                    const uint32_t t0 = __byte_perm(v[0], v[1], 0x5140), t1 = __byte_perm(v[2], v[3], 0x5140);
+                    qf[k][0] = __byte_perm(t0, t1, 0x5410); qf[k][1] = __byte_perm(t0, t1, 0x7632);
+                    qf[k][2] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
                 }
-                if constexpr (GT == 4) { qf[k][0] = g < 4 ? word[0] : word[1]; qf[k][1] = g < 4 ? word[2] : word[3]; }
-                else { qf[k][0] = word[0]; qf[k][1] = word[1]; qf[k][2] = word[2]; }
             } else {
                 qf[k][0] = Cvt<__half>::pack(x[4 * k] * up, x[4 * k + 1] * up);
                 qf[k][1] = Cvt<__half>::pack(x[4 * k + 2] * up, x[4 * k + 3] * up);
