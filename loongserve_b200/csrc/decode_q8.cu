@@ -87,9 +87,10 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 // copies: one instruction takes the NH heads' K (or V) codes of WT tokens, 512 contiguous bytes for NH = 4, into a ring of
 // stages of 16 * WT tokens, counted on mbarriers.  Against fetches by the consumer warps themselves this takes address
 // arithmetic and slot lookups out of their instruction streams, and a scale's 32-byte sector is asked for once per CTA instead
-// of once per head.  (One bulk copy per token and operand instead: 81 cycles each from one warp, 3.3 TB/s at best.)  Row
-// pitches in shared memory are chosen so that the fragment reads (16 bytes per lane) have no bank conflicts: K rows an odd
-// multiple of 64 bytes apart, V rows an odd multiple of 16.
+// of once per head.  (One bulk copy per token and operand instead: 81 cycles each from one warp, 3.3 TB/s at best.)  A row lies
+// in shared memory as in the pool, a 128-byte line to a line, with its eight 16-byte pieces in another order (k_piece, v_piece),
+// so that the fragment reads (16 bytes per lane) have no bank conflicts.  Rows at odd pitches would do for the banks too, but a
+// copy whose line ends up across two lines of shared memory asks the L2 for the sectors on the border twice: half as many again.
 //
 // CTAs are persistent: each walks over items (a request's tokens t0..t1, heads), and the producer runs ahead into the next item, so
 // that neither the start of an item (length, slots, queries) nor its results stop the flow of copies.  How the tokens are divided:
@@ -106,11 +107,11 @@ constexpr int kQ8MaxCounted = 384;        // requests whose lengths are held in 
 struct WarpStateQ8 { float acc[32][32], m[32], l[32], v[32]; };      // [register][lane]
 template <int NH> struct RingQ8 {
     static constexpr int WT = kQ8Warps / NH, kTokens = 16 * WT;
-    static constexpr int kPitchK = NH * 128 + 64, kPitchV = NH * 128 + 16;
-    static constexpr int kOffV = kTokens * kPitchK, kOffScale = kOffV + kTokens * kPitchV;      // scales [K, V][token][NH]
+    static constexpr int kPitch = NH * 128, kOffV = kTokens * kPitch;
+    static constexpr int kOffScale = 2 * kOffV;                                                 // scales [K, V][token][NH]
     static constexpr int kOffPresent = kOffScale + 2 * kTokens * NH * 4;                        // WT masks of 16 tokens
-    static constexpr int kStageBytes = kOffPresent + 16;
-    static constexpr int kStages = NH == 4 ? 4 : (NH == 2 ? 3 : 2);
+    static constexpr int kStageBytes = kOffPresent + 128;
+    static constexpr int kStages = NH == 4 ? 4 : 3;
     static constexpr int kOffBar = kStages * kStageBytes;                                       // full [kStages], empty [kStages]
     static constexpr int kOffAbort = kOffBar + 2 * kStages * 8;
     static constexpr int kOffMerge = kOffAbort + 16;                                            // states of the warps with wt > 0
@@ -174,6 +175,10 @@ __device__ __forceinline__ void store_row16(void* o, int64_t i, const float (&x)
     uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(o) + i);
     p[0] = make_uint4(u[0], u[1], u[2], u[3]); p[1] = make_uint4(u[4], u[5], u[6], u[7]);
 }
+
+// where piece i of 16 bytes of a head's row lies, by the row's token
+__device__ __forceinline__ int k_piece(int i, int token) { return i ^ (token & 1) << 2; }
+__device__ __forceinline__ int v_piece(int i, int token) { return i ^ (token & 6); }
 
 struct ItemQ8 { int b, hg, t0, t1, req, steps; int64_t row0; bool write, whole; };   // row0: of the partials, in rows of all heads
 struct CursorQ8 { int n, u, u1; };             // (piece, heads), its units from u to u1 are still to do
@@ -317,8 +322,9 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
                 const int slot = __shfl_sync(0xffffffffu, s[j * WT / 16], j * WT % 16 + share);
                 const int64_t row = max(slot, 0);
                 const uint32_t at = j * WT + share;
-                cp_async16(stage + at * R::kPitchK + piece * 16, ksrc + row * a.k_stride_t, slot >= 0);
-                cp_async16(stage + R::kOffV + at * R::kPitchV + piece * 16, vsrc + row * a.v_stride_t, slot >= 0);
+                const uint32_t line = stage + at * R::kPitch + (piece >> 3) * 128;
+                cp_async16(line + k_piece(piece & 7, at) * 16, ksrc + row * a.k_stride_t, slot >= 0);
+                cp_async16(line + R::kOffV + v_piece(piece & 7, at) * 16, vsrc + row * a.v_stride_t, slot >= 0);
             }
 #pragma unroll
             for (int u = 0; u < WT; ++u) {                            // scales: lanes 0-15 K, lanes 16-31 V of 16 tokens
@@ -411,15 +417,15 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     float v_ref = 0.f, v_mul = 0.f;       // weights are held as p * v_scale * v_mul, v_mul = 2^12 / v_ref, v_ref >= every v_scale so far
 
     auto compute = [&](const uint8_t* d) {
-        const uint8_t* krow = d + (wt * 16 + g) * R::kPitchK + hw * 128 + c * 16;
-        const uint8_t* vrow = d + R::kOffV + (wt * 16 + 2 * c) * R::kPitchV + hw * 128 + g * 16;
+        const uint8_t* krow = d + (wt * 16 + g) * R::kPitch + hw * 128 + k_piece(c, g) * 16;
+        const uint8_t* vrow = d + R::kOffV + (wt * 16 + 2 * c) * R::kPitch + hw * 128 + v_piece(g, 2 * c) * 16;
         const float* scl = reinterpret_cast<const float*>(d + R::kOffScale) + wt * 16 * NH + hw;
         const uint32_t present = *reinterpret_cast<const uint32_t*>(d + R::kOffPresent + 4 * wt);
         float sc[4], vs[4];               // of tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitchK);
-            const uint4 y = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitchK + 64);
+            const uint4 x = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitch);
+            const uint4 y = *reinterpret_cast<const uint4*>(krow + 8 * i * R::kPitch + (g & 1 ? -64 : 64));
             const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
             if constexpr (kInt) {
                 // a sum of 128 products of a digit and a code is below 2^21: counted in the last places of 1.5 * 2^23, it is a float
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         if (GT == 4 && g >= 4) { b0 = e0; b1 = e1; }
         uint32_t vw[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const uint4 x = *reinterpret_cast<const uint4*>(vrow + ((i & 1) + 8 * (i >> 1)) * R::kPitchV); vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w; }
+        for (int i = 0; i < 4; ++i) { const uint4 x = *reinterpret_cast<const uint4*>(vrow + ((i & 1) + 8 * (i >> 1)) * R::kPitch); vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w; }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
 #pragma unroll
