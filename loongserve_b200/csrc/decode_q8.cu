@@ -294,17 +294,23 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
           const uint8_t* ksrc = a.k + (int64_t)kv0 * a.k_stride_h + piece * 16;
           const uint8_t* vsrc = a.v + (int64_t)kv0 * a.v_stride_h + piece * 16;
           const float* ssrc = isv ? a.v_scale + kv0 : a.k_scale + kv0;
-          // slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u; -1: no such token
-          auto load_slots = [&](int i, int u) -> int {
-            const int t = it.t0 + ((i + isv) * WT + u) * 16 + tok;
-            if (i + isv >= it.steps || t >= it.t1) return -1;
-            const int s = rtt[t];
+          // Slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u.  They are asked for two steps before they
+          // are looked at: a check at once made the producer wait for every load, two thirds of its time.
+          auto token_of = [&](int i, int u) { return it.t0 + ((i + isv) * WT + u) * 16 + tok; };
+          auto ask = [&](int i, int u) -> int {
+            const int t = token_of(i, u);
+            return i + isv < it.steps && t < it.t1 ? rtt[t] : 0;
+          };
+          auto check = [&](int i, int u, int s) -> int {                  // -1: no such token
+            if (i + isv >= it.steps || token_of(i, u) >= it.t1) return -1;
             if (s < 0 || s >= a.pool_rows) { q8_report(0, s); return -1; }
             return s;
           };
           int slots[WT], slots_next[WT];
 #pragma unroll
-          for (int u = 0; u < WT; ++u) { slots[u] = load_slots(0, u); slots_next[u] = load_slots(2, u); }
+          for (int u = 0; u < WT; ++u) { slots[u] = ask(0, u); slots_next[u] = ask(2, u); }
+#pragma unroll
+          for (int u = 0; u < WT; ++u) slots[u] = check(0, u, slots[u]);
           for (int i = 0; i < it.steps; ++i, ++done) {
             ok = __all_sync(0xffffffffu, q8_wait(empty(st), phase, s_abort, 8, done));
             if (!ok) break;
@@ -338,7 +344,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
             cp_async_arrive(full(st));
             if (i & 1) {
 #pragma unroll
-                for (int u = 0; u < WT; ++u) { slots[u] = slots_next[u]; slots_next[u] = load_slots(i + 3, u); }
+                for (int u = 0; u < WT; ++u) { slots[u] = check(i + 1, u, slots_next[u]); slots_next[u] = ask(i + 3, u); }
             }
             if (++st == R::kStages) { st = 0; phase ^= 1; }
           }
