@@ -54,7 +54,8 @@ struct DecodeQ8Args {
 
 constexpr int kQ8Warps = 4, kQ8HeadTile = 8;
 constexpr int kQ8Resident = 3 * kNumSMs, kQ8MinPiece = 64;       // CTAs the GPU holds; tokens below which a piece is not cut
-constexpr int kQ8Whole = 256;                                    // requests up to this length are not cut at all
+// requests up to this length are not cut at all
+inline int q8_whole(int batch) { return batch < 8 ? 256 : 512; }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -294,8 +295,9 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
           const uint8_t* ksrc = a.k + (int64_t)kv0 * a.k_stride_h + piece * 16;
           const uint8_t* vsrc = a.v + (int64_t)kv0 * a.v_stride_h + piece * 16;
           const float* ssrc = isv ? a.v_scale + kv0 : a.k_scale + kv0;
-          // Slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u.  They are asked for two steps before they
-          // are looked at: a check at once made the producer wait for every load, two thirds of its time.
+          // Slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u.  They are asked for eight steps at a time (four
+          // with NH < 4), as many before they are looked at: they queue behind the copies, and the producer waits for all it has asked for.  (A check
+          // at once: two thirds of its time; two steps at a time, two steps before: half of it.)
           auto token_of = [&](int i, int u) { return it.t0 + ((i + isv) * WT + u) * 16 + tok; };
           auto ask = [&](int i, int u) -> int {
             const int t = token_of(i, u);
@@ -306,19 +308,30 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
             if (s < 0 || s >= a.pool_rows) { q8_report(0, s); return -1; }
             return s;
           };
-          int slots[WT], slots_next[WT];
+          constexpr int kPairs = NH == 4 ? 4 : 2;
+          int slots[kPairs][WT], later[kPairs][WT];
 #pragma unroll
-          for (int u = 0; u < WT; ++u) { slots[u] = ask(0, u); slots_next[u] = ask(2, u); }
+          for (int k = 0; k < kPairs; ++k)
 #pragma unroll
-          for (int u = 0; u < WT; ++u) slots[u] = check(0, u, slots[u]);
+              for (int u = 0; u < WT; ++u) later[k][u] = ask(2 * k, u);
           for (int i = 0; i < it.steps; ++i, ++done) {
             ok = __all_sync(0xffffffffu, q8_wait(empty(st), phase, s_abort, 8, done));
             if (!ok) break;
             const uint32_t stage = sbase + st * R::kStageBytes;
+            if (i % (2 * kPairs) == 0) {
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k)
+#pragma unroll
+                    for (int u = 0; u < WT; ++u) slots[k][u] = check(i + 2 * k, u, later[k][u]);
+            }
+            const int pair = i / 2 % kPairs;
             int s[WT];
 #pragma unroll
             for (int u = 0; u < WT; ++u) {
-                s[u] = __shfl_sync(0xffffffffu, slots[u], (i & 1) * 16 + tok);
+                int mine = slots[0][u];
+#pragma unroll
+                for (int k = 1; k < kPairs; ++k) mine = pair == k ? slots[k][u] : mine;
+                s[u] = __shfl_sync(0xffffffffu, mine, (i & 1) * 16 + tok);
                 const uint32_t present = __ballot_sync(0xffffffffu, s[u] >= 0) & 0xffffu;
                 if (lane == 0) *reinterpret_cast<uint32_t*>(smem + st * R::kStageBytes + R::kOffPresent + 4 * u) = present;
             }
@@ -342,9 +355,11 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
                     for (int h = 0; h < NH; ++h) cp_async4(sd + 4 * h, sp + h, s[u] >= 0);
             }
             cp_async_arrive(full(st));
-            if (i & 1) {
+            if (i % (2 * kPairs) == 0) {
 #pragma unroll
-                for (int u = 0; u < WT; ++u) { slots[u] = check(i + 1, u, slots_next[u]); slots_next[u] = ask(i + 3, u); }
+                for (int k = 0; k < kPairs; ++k)
+#pragma unroll
+                    for (int u = 0; u < WT; ++u) later[k][u] = ask(i + 2 * kPairs + 2 * k, u);
             }
             if (++st == R::kStages) { st = 0; phase ^= 1; }
           }
@@ -781,11 +796,11 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     if (!o || !lse || max_len_in_batch < 0 || seq_block_size < 0 || num_q_heads <= 0) return ESP_ERR_BAD_ARG;
     if (o_dtype != ESP_DTYPE_F16 && o_dtype != ESP_DTYPE_BF16 && o_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
     const int32_t max_len = max_len_in_batch > 0 ? max_len_in_batch : 1;
-    // seq_block_size 0: equal pieces, or one split where no request is longer than 256 tokens, which saves the merge (pieces / one
-    // split, 8 kv heads, group 4: one request of 256 tokens 10.3 / 9.5 us, of 512 10.9 / 13.2; 64 ragged ones of up to 256
-    // 18.2 / 12.2; 256 of them 36.7 / 30.4, of up to 512 53.1 / 61.2)
-    const bool even = seq_block_size == 0 && max_len > kQ8Whole;
-    const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : kQ8Whole) : seq_block_size;
+    // seq_block_size 0: equal pieces, or one split where no request is longer than 256 tokens (512 from 8 requests on), which saves
+    // the merge.  Pieces / one split in us, 8 kv heads, group 4: one request of 256 tokens 8.2 / 8.3, of 512 9.9 / 11.3; 16 ragged ones
+    // of up to 512 13.4 / 11.1, 64 of them 19.5 / 18.3, 256 50.3 / 51.0.
+    const bool even = seq_block_size == 0 && max_len > q8_whole(batch);
+    const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : q8_whole(batch)) : seq_block_size;
     const int64_t nblk = (max_len + (int64_t)block - 1) / block;
     if (nblk > 1 && !workspace) return ESP_ERR_BAD_ARG;
     if (nblk > 1 && !aligned16(workspace)) return ESP_ERR_ALIGNMENT;
