@@ -12,6 +12,10 @@ The modules mirror the call surface of the reference's model layer for this path
   rnccl               get_nccl_unique_id, RNCCLComm               (raw NCCL point-to-point)
   ring                ring prefill loop and multi-master decode orchestration
 
+Next to it, the 8-bit serving path: a KV pool of int8 or e4m3 codes (kv_ops.destindex_copy_quantize_kv, gather_dequantize_kv,
+flash_decoding.token_decode_attention_q8, mem_manager.QuantizedKVMemoryManager) and int8 projections with the row kernels that
+feed them (layer_ops.mm_w8a8, add_rms_norm_quant, silu_and_mul_quant, quantize_rows, dequantize_rows).
+
 All compute goes through the C ABI in include/esp_attention.h; there is no CPU or PyTorch fallback.
 """
 from . import _lib  # noqa: F401

@@ -3,23 +3,29 @@
 // Stage 1 writes the same splits and partials as the 16-bit form (decode_attention.cu); the call that does both stages divides the
 // tokens itself (below).
 //
-// Bound by HBM: 2 * (128 + 4) bytes per token and kv head, each read once.  At that rate one SM has to take in a code every
-// 1/23 of a cycle and multiply it with up to 8 query heads, which is past what fp32 lanes do next to the conversion; so codes
-// become f16 (exactly: 8 bits fit) and the products run on the tensor cores (mma.sync m16n8k16, fp32 sums), which are far
-// from their limit here.  A lane reads 16-byte pieces of the rows and its pieces ARE operand fragments, because the order of
-// the summed index (head dims for S, tokens for O) is free:
-//   S [heads 16 x tokens 8] = Q K^T   B fragment of lane (g, c): token g, dims {16c..16c+15, 64+16c..64+16c+15}, one word of
-//                                     four codes per MMA; Q fragments are loaded once in the same dim order.
+// Bound by HBM: 2 * (128 + 4) bytes per token and kv head, each read once (64 requests x 4096-65536 tokens x 32 kv heads, 17.9 GB:
+// 2.74 ms, 6.5 TB/s; the 16-bit pool of the same requests 5.13 ms), and next to that by power: a GPU that runs it without a pause
+// lowers its clocks (32 requests x 1K-16K tokens x 32 kv heads: 338 us in a burst, 390 in a loop at 980 W), so instructions per
+// byte count.  At that rate one SM has to take in a code every 1/23 of a cycle and multiply it with up to 8 query heads, which is
+// past what fp32 lanes do next to the conversion; the products run on the tensor cores (mma.sync), which are far from their limit
+// here.  A lane reads 16-byte pieces of the rows and its pieces ARE operand fragments, because the order of the summed index
+// (head dims for S, tokens for O) is free:
+//   S [rows 16 x tokens 8] = Q K^T    B fragment of lane (g, c): token g, dims {16c..16c+15, 64+16c..64+16c+15}; Q fragments are
+//                                     loaded once in the same dim order.
 //   O^T [dims 16 x heads 8] += V^T P^T  A fragment of lane (g, c): dims 16g..16g+15, tokens 2c, 2c+1, 2c+8, 2c+9 (words of two
 //                                     tokens interleaved byte by byte); P^T's fragment is what the lane holds of S.
 // (lane = 4g + c.)  A warp takes 16 tokens of one head tile per step.
 //
-// Precision.  q is scaled by a power of two per head so that its largest element is near 2^7 in f16: exact down to 2^-21 of
-// it.  Scores, maxima, sums and outputs are fp32.  A weight p * v_scale, relative to 2^-8 * the largest v_scale seen by the warp,
-// enters the second product as its rounding to f16 and the rounding of what that left: 2^-22 relative.  (The rounding alone, 2^-12,
-// showed in f16 outputs: 3.3e-4 against 2.0e-4 for fp32 weights.)  With groups of up to four heads (GT = 4) the rests take the columns
-// of heads 4-7 and cost no product; larger groups (GT = 8) multiply V twice: 57 us for 64 requests x 8 q heads on 4 kv heads x 2500
-// tokens, 55 without.
+// Precision.  Scores, maxima, sums and outputs are fp32.
+//   S, int8 codes: they are operands as they lie in the pool (m16n8k32, 32-bit integer sums); q, scaled by a power of two per head, is
+//   an integer of 30 bits in four balanced base-256 digits, rows j, j + 4, j + 8, j + 12 of A (groups of up to four heads, GT = 4), or
+//   of 22 bits in three (GT = 8: rows j, j + 8, and a second product).  Against codes brought to f16 this saves a third of the
+//   instructions: 477 us instead of 499 for the 32 requests above, in a loop, before the copies were what they are now.
+//   S, e4m3 codes: brought to f16 (exactly; two instructions a word), q scaled to 2^7 in f16, exact down to 2^-21 of its largest.
+//   O: codes become f16 (exactly: 8 bits fit).  A weight p * v_scale, relative to 2^-8 * the largest v_scale seen by the warp, enters as
+//   its rounding to f16 and the rounding of what that left: 2^-22 relative.  (The rounding alone, 2^-12, showed in f16 outputs: 3.3e-4
+//   against 2.0e-4 for fp32 weights.)  With GT = 4 the rests take the columns of heads 4-7 and cost no product; GT = 8 multiplies V
+//   twice.
 #include <algorithm>
 #include "quant_common.cuh"
 #include "sm100_ptx.cuh"
@@ -99,8 +105,9 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 //            a piece that crosses requests has an item for each.  Pieces and requests both only grow along the way, so piece + request
 //            numbers a partial uniquely, and there are at most pieces + requests of them.  A request inside one piece gets its results
 //            at once.  Against splits of a fixed length every CTA has the same work and writes a partial or two instead of one per
-//            128 to 512 tokens: 185 us instead of 206 for 2 requests x 262144 tokens x 8 kv heads (group 4), 77 instead of 97 for
-//            64 requests x 4 kv heads (group 8), 474 instead of 509 for 32 requests x 1K-16K tokens x 32 kv heads.
+//            128 to 512 tokens: 180 us instead of 186 (the best length) to 222 for 2 requests x 200K-262K tokens x 8 kv heads (group 4), 76
+//            instead of 87 to 126 for 64 requests x 4 kv heads (group 8), 338 instead of 347 to 409 for 32 requests x 1K-16K tokens x
+//            32 kv heads.
 //   counted  splits of seq_block_size tokens, where a CTA has several and the batch is small enough: those that exist are counted
 //            first, so that ragged batches divide evenly.
 //   else     all splits up to the longest possible request; those behind a request's end are passed over.

@@ -7,9 +7,10 @@
 // The norm is taken of the unrounded sum, so the output is rounded once; what is kept for the next layer is the rounded one.
 //
 // HBM bound: every element is read once, held in registers in fp32 (up to 8 * VPT per thread) across the row's reduction,
-// and written once.  Rows of up to 512 elements: a warp per row, eight rows to a CTA (60000 rows of 256: a CTA of one warp per row
-// took 33 us, this form 9-20 us).  Wider rows: a CTA per row; CTAs walk over the rows and load the next one before they reduce the
-// one in hand, which keeps copies in flight through the reduction (norm into codes, 16384 x 4096: 44.9 -> 37 us).
+// and written once.  Rows of up to 512 elements: a warp per row, eight rows to a CTA, the next row asked for before the one in hand
+// is reduced (60000 rows of 256 into codes: a CTA of one warp per row took 33 us, this form 10).  Wider rows: a CTA per row; asking for
+// the next row there cost more in registers than it gained.  Measured (B200): add + norm into codes 16384 x 4096 72 us for 470 MB,
+// SiLU * mul into codes 8192 x 11008 74 us for 451 MB, codes back into rows 16384 x 4096 35 us for 201 MB.
 #include "quant_common.cuh"
 
 namespace esp {
