@@ -303,8 +303,8 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
           const uint8_t* vsrc = a.v + (int64_t)kv0 * a.v_stride_h + piece * 16;
           const float* ssrc = isv ? a.v_scale + kv0 : a.k_scale + kv0;
           // Slots of steps i (lanes 0-15) and i + 1 (lanes 16-31), 16 tokens of share u.  They are asked for eight steps at a time (four
-          // with NH < 4), as many before they are looked at: they queue behind the copies, and the producer waits for all it has asked for.  (A check
-          // at once: two thirds of its time; two steps at a time, two steps before: half of it.)
+          // with NH < 4), as many steps before they are looked at: they queue behind the copies, and looking at one waits for all that
+          // have been asked for.  (Looked at when asked for: two thirds of the producer's time; two steps at a time: half of it.)
           auto token_of = [&](int i, int u) { return it.t0 + ((i + isv) * WT + u) * 16 + tok; };
           auto ask = [&](int i, int u) -> int {
             const int t = token_of(i, u);
@@ -747,7 +747,7 @@ static int stage1_q8(DecodeQ8Args& a, int head_dim, int max_len, int dtype, int 
         a.v_stride_h % 16 || ((uintptr_t)a.k_scale & 3u) || ((uintptr_t)a.v_scale & 3u))
         return ESP_ERR_ALIGNMENT;
     const int64_t nblk = (max_len + (int64_t)a.seq_block_size - 1) / a.seq_block_size;
-    if (a.parts && (a.batch > kQ8MaxCounted || (max_len / 16 + 1) * (int64_t)a.batch > 2147483647LL)) return ESP_ERR_TOO_LARGE;
+    if (a.parts && (a.batch > kQ8MaxCounted || (max_len / 16 + 1) * (int64_t)a.batch > 2147483647LL - 65536)) return ESP_ERR_TOO_LARGE;
     a.num_blocks = (int)nblk;
     a.max_len = max_len;
     if (nblk * a.seq_block_size > 2147483647LL - 65536) return ESP_ERR_TOO_LARGE;
@@ -785,6 +785,7 @@ extern "C" int esp_decode_stage1_q8(float* mid_o, float* mid_lse, const void* q,
                                     int64_t pool_rows, void* stream) {
     if (batch == 0 || max_len_in_batch <= 0) return ESP_OK;
     if (!mid_o || !mid_lse) return ESP_ERR_BAD_ARG;
+    if (!aligned16(mid_o) || ((uintptr_t)mid_lse & 3u)) return ESP_ERR_ALIGNMENT;
     DecodeQ8Args a = args_q8(q, k, v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t,
                              req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads,
                              pool_rows);
@@ -807,10 +808,10 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     // the merge.  Pieces / one split in us, 8 kv heads, group 4: one request of 256 tokens 8.2 / 8.3, of 512 9.9 / 11.3; 16 ragged ones
     // of up to 512 13.4 / 11.1, 64 of them 19.5 / 18.3, 256 50.3 / 51.0.
     const bool even = seq_block_size == 0 && max_len > q8_whole(batch);
-    const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : q8_whole(batch)) : seq_block_size;
+    const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : max_len) : seq_block_size;
     const int64_t nblk = (max_len + (int64_t)block - 1) / block;
     if (nblk > 1 && !workspace) return ESP_ERR_BAD_ARG;
-    if (nblk > 1 && !aligned16(workspace)) return ESP_ERR_ALIGNMENT;
+    if (!aligned16(o) || ((uintptr_t)lse & 3u) || (nblk > 1 && !aligned16(workspace))) return ESP_ERR_ALIGNMENT;
     DecodeQ8Args a = args_q8(q, k, v, k_scale, v_scale, k_stride_t, k_stride_h, v_stride_t, v_stride_h, k_scale_stride_t, v_scale_stride_t,
                              req_to_tokens, req_to_tokens_stride, req_rows, req_cols, b_req_idx, b_seqlen, batch, num_q_heads, num_kv_heads,
                              pool_rows);

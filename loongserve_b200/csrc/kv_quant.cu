@@ -318,7 +318,7 @@ extern "C" int esp_kv_scatter_register_q8(
     const PoolQ8 p{(uint8_t*)codes, codes_row_stride, codes_head_stride, scales, scales_row_stride, pool_rows};
     const int lpr = lanes_per_row(head_dim);
     RegisterArgs a{new_len, range_begin, range_end, new_len_cumsum, kv_b_start_loc, cur_kv_cache_index, mem_index, idx64, req_to_token,
-                   req_to_token_stride, b_req_idx, num_used_mem_index, ((max_len_in_batch + 255) / 256) * 256, should_register, dim3(1)};
+                   req_to_token_stride, b_req_idx, num_used_mem_index, max_len_in_batch > 2147483392 ? 2147483647 : (max_len_in_batch + 255) / 256 * 256, should_register, dim3(1)};
     // the 16-bit form's row cap: rows past max_len_in_batch rounded up to 256 are not copied
     const int64_t per = ((int64_t)kNumSMs * 32 + batch - 1) / batch;
     int64_t gx = q8_grid(max_len_in_batch, (kQ8Threads / lpr) >> head_shift(heads2, lpr));

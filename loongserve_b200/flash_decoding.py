@@ -114,11 +114,12 @@ def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_toke
         if out_logexpsum.dtype != torch.float32:
             raise TypeError("out_logexpsum is fp32")
     tags = dtype16_tag(q), dtype_tag(out), code_tag(cache_k)
-    if block_seq is None and batch <= Q8_MAX_EVEN:
+    if block_seq is None and (batch <= Q8_MAX_EVEN or max_len <= 512):
         block = 0
-        floats = (min(444, (batch * max_len + 63) // 64) + batch) * hq * (dim + 1) + 2 * batch if max_len > 256 else 0
+        floats = (min(444, (batch * max_len + 63) // 64) + batch) * hq * (dim + 1) + 2 * batch if 256 < max_len and batch <= Q8_MAX_EVEN else 0
     else:
         block = int(block_seq) if block_seq is not None else q8_block_seq(batch, hkv, hq // max(hkv, 1), max_len)
+        assert block > 0
         nblk = (max_len + block - 1) // block
         floats = nblk * batch * hq * (dim + 1) if nblk > 1 else 0
     work = k_scale.new_empty(floats) if floats else None

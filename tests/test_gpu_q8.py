@@ -268,7 +268,7 @@ def test_decode_partials_are_the_blocks_own_attention(code):
 @pytest.mark.parametrize("code,hq,hkv,lens", [
     (INT8, 32, 32, [5000, 0, 1, 129, 700, 0, 2600]), (E4M3, 8, 1, [9000]), (INT8, 4, 4, [40] * 200 + [0, 0, 7] + [3000, 2999]),
     (E4M3, 16, 2, [0] * 5 + [129] + [0] * 5), (INT8, 24, 8, [128 * (i % 5) + i for i in range(384)]), (INT8, 8, 8, [33 * (i % 9) for i in range(385)]),
-    (E4M3, 32, 4, [1] * 300 + [4096]), (INT8, 8, 2, [20000, 64, 20001])])
+    (E4M3, 32, 4, [1] * 300 + [4096]), (INT8, 8, 2, [20000, 64, 20001]), (INT8, 449, 449, [600, 70]), (E4M3, 4, 4, [500] * 390)])
 def test_decode_pieces_across_requests(code, hq, hkv, lens):
     """Divided evenly, a piece ends anywhere in a request and holds the ends of several."""
     from loongserve_b200 import flash_decoding as fd
@@ -317,6 +317,13 @@ def test_decode_pieces_stop_at_the_given_longest():
     fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 450, None, out, lse)
     check_decode(out, lse, decode_exact(c, [450, 400, 450]), 450)
     assert fd.device_status()[0] == 0
+    fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 100, None, out, lse)
+    check_decode(out, lse, decode_exact(c, [100, 100, 100]), 100)
+    buf = torch.zeros(3 * 8 * D + 1, dtype=BF16, device=DEV)
+    with pytest.raises(RuntimeError):                                                          # rows are written 16 bytes at a time
+        fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 100, None, buf[1:].view(3, 8, D), lse)
+    with pytest.raises(AssertionError):
+        fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 600, 0, out, lse)
     c["table"][r0, 5] = 2147483647; c["table"][r0, 400] = -3; c["table"][r0, 599] = c["codes"].shape[0]
     fd.token_decode_attention_q8(c["q"], *a, c["rows"], c["lens"], 600, None, out, lse)
     check_decode(out, lse, decode_exact(c), 600)

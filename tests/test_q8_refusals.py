@@ -67,13 +67,14 @@ DECODE = dict(mid_o=P, mid_lse=P, q=P, k=P, v=P, ks=P, vs=P, kst=528, ksh=128, v
     (dict(batch=0), 0), (dict(max_len=0), 0), (dict(batch=-2), BAD), (dict(mid_o=None), BAD), (dict(q=None), BAD), (dict(k=None), BAD), (dict(vs=None), BAD),
     (dict(table=None), BAD), (dict(b_len=None), BAD), (dict(hq=9), BAD), (dict(hkv=0), BAD), (dict(block=0), BAD), (dict(rows=0), BAD), (dict(cols=0), BAD),
     (dict(pool=0), BAD), (dict(dtype=2), BAD), (dict(code=2), BAD), (dict(dim=64), UNSUP), (dict(batch=65536), LARGE), (dict(hq=65536, hkv=1), LARGE),
-    (dict(q=P + 8), ALIGN), (dict(k=P + 8), ALIGN), (dict(kst=520), ALIGN), (dict(vsh=8), ALIGN), (dict(ks=P + 1), ALIGN)])
+    (dict(q=P + 8), ALIGN), (dict(k=P + 8), ALIGN), (dict(kst=520), ALIGN), (dict(vsh=8), ALIGN), (dict(ks=P + 1), ALIGN),
+    (dict(mid_o=P + 4), ALIGN), (dict(mid_lse=P + 2), ALIGN)])
 def test_decode_stage1(lib, change, rc):
     assert call(lib.esp_decode_stage1_q8, DECODE, **change) == rc
 
 
 @pytest.mark.parametrize("change,rc", [
-    (dict(batch=0), 0), (dict(o=None), BAD), (dict(lse=None), BAD), (dict(work=None), BAD), (dict(work=P + 4), ALIGN), (dict(block=-1), BAD),
+    (dict(batch=0), 0), (dict(o=None), BAD), (dict(lse=None), BAD), (dict(work=None), BAD), (dict(work=P + 4), ALIGN), (dict(o=P + 8), ALIGN), (dict(lse=P + 1), ALIGN), (dict(block=-1), BAD),
     (dict(max_len=-1), BAD), (dict(odt=3), BAD), (dict(batch=385), LARGE), (dict(batch=384, max_len=2147483647), LARGE), (dict(hq=0), BAD),
     (dict(q=None), BAD), (dict(kst=520), ALIGN), (dict(dim=64), UNSUP), (dict(block=16, work=None), BAD)])
 def test_decode_attention(lib, change, rc):
