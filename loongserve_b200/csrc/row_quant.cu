@@ -143,25 +143,20 @@ __global__ void __launch_bounds__(WARP ? 256 : (VPT == 2 ? 512 : (VPT == 4 ? 512
     }
 }
 
-// V codes per lane and step, U steps in flight
-template <typename OT, int V, int U>
+// eight codes per lane and step, four steps in flight
+template <typename OT>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(OT* __restrict__ out, const int8_t* __restrict__ codes,
                                                               const float* __restrict__ scale, int64_t rows, int vecs) {
+    constexpr int U = 4;
     const int64_t total = rows * vecs, stride = (int64_t)gridDim.x * 256;
     for (int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += U * stride) {
-        uint32_t w[U][V / 4];
+        uint2 w[U];
         float s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t i = i0 + u * stride;
             if (i < total) {
-                if constexpr (V == 16) {
-                    const uint4 x = __ldcs(reinterpret_cast<const uint4*>(codes) + i);
-                    w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
-                } else {
-                    const uint2 x = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
-                    w[u][0] = x.x; w[u][1] = x.y;
-                }
+                w[u] = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
                 s[u] = scale[i / vecs];
             }
         }
@@ -169,24 +164,18 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(OT* __restrict__ o
         for (int u = 0; u < U; ++u) {
             const int64_t i = i0 + u * stride;
             if (i >= total) continue;
-            float f[V];
+            float lo[4], hi[4], f[8];
+            unpack_codes4<ESP_CODE_INT8>(w[u].x, lo);
+            unpack_codes4<ESP_CODE_INT8>(w[u].y, hi);
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) {
-                float x[4];
-                unpack_codes4<ESP_CODE_INT8>(w[u][j], x);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) f[4 * j + k] = x[k] * s[u];
-            }
+            for (int k = 0; k < 4; ++k) { f[k] = lo[k] * s[u]; f[4 + k] = hi[k] * s[u]; }
             if constexpr (sizeof(OT) == 4) {
-                float4* o = reinterpret_cast<float4*>(out + i * V);
-#pragma unroll
-                for (int j = 0; j < V / 4; ++j) o[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                float4* o = reinterpret_cast<float4*>(out + i * 8);
+                o[0] = make_float4(f[0], f[1], f[2], f[3]);
+                o[1] = make_float4(f[4], f[5], f[6], f[7]);
             } else {
-                uint4* o = reinterpret_cast<uint4*>(out + i * V);
-#pragma unroll
-                for (int j = 0; j < V / 8; ++j)
-                    o[j] = make_uint4(Cvt<OT>::pack(f[8 * j], f[8 * j + 1]), Cvt<OT>::pack(f[8 * j + 2], f[8 * j + 3]),
-                                      Cvt<OT>::pack(f[8 * j + 4], f[8 * j + 5]), Cvt<OT>::pack(f[8 * j + 6], f[8 * j + 7]));
+                *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(Cvt<OT>::pack(f[0], f[1]), Cvt<OT>::pack(f[2], f[3]),
+                                                                    Cvt<OT>::pack(f[4], f[5]), Cvt<OT>::pack(f[6], f[7]));
             }
         }
     }
@@ -287,7 +276,7 @@ extern "C" int esp_dequantize_rows(void* out, const int8_t* codes, const float* 
     const int64_t want = (rows * (cols / 8) + 1023) / 1024, cap = (int64_t)kNumSMs * 32;
     const unsigned grid = (unsigned)(want < cap ? want : cap);
     cudaStream_t s = (cudaStream_t)stream;
-#define ESP_DQ(OT) dequantize_rows_kernel<OT, 8, 4><<<grid, 256, 0, s>>>((OT*)out, codes, scale, rows, cols / 8);
+#define ESP_DQ(OT) dequantize_rows_kernel<OT><<<grid, 256, 0, s>>>((OT*)out, codes, scale, rows, cols / 8);
     if (dtype == ESP_DTYPE_F16) ESP_DQ(__half)
     else if (dtype == ESP_DTYPE_BF16) ESP_DQ(__nv_bfloat16)
     else if (dtype == ESP_DTYPE_F32) ESP_DQ(float)
