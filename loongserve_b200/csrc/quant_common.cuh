@@ -21,6 +21,12 @@ template <> struct CodeTop<ESP_CODE_E4M3> { static constexpr float v = kE4m3Top;
 // so a NaN is not lost on the way (fmaxf would drop it).
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// Programmatic launch.  A kernel launched with the attribute may start before the one ahead of it in the stream has ended; it waits
+// for that kernel's end and results here (every thread, before anything else that kernel may write or read).
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// From here on (once every CTA has passed or left) a kernel behind this one that was launched so may start.
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 struct RowScale { float inv, scale; bool finite; };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits, float top) {
     RowScale r;

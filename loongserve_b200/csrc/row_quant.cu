@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(WARP ? 256 : (VPT == 2 ? 512 : (VPT == 4 ? 512
     const int tid = WARP ? lane : threadIdx.x, nt = WARP ? 32 : blockDim.x;
     const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : a.rows;      // a CTA takes one row
+    if (QUANT) grid_dependents_launch();              // a product of the codes is what comes next
     const uint4* wv = reinterpret_cast<const uint4*>(a.weight);
     __shared__ float s_ss[32];
     __shared__ uint32_t s_mx[32];

@@ -246,6 +246,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
 // Few tokens: the weights are what is read, so channels take the 128 rows of the MMA and TN tokens its columns.  A cluster of S
 // CTAs splits K of one tile; the integer partials are summed through distributed shared memory (each CTA sums and writes TN / S
 // of the tokens).  Warps: 0 producer, 1 issuer, 2-5 epilogue (one channel per thread).
+//
+// Some 6 us of such a call are not its bytes, so its start (barriers, tensor memory, descriptors) runs under the kernel before it
+// where that one allows it (the row kernels, this one): nothing of that kernel's results is touched before grid_dependency_wait, and
+// after it only by loads that pass the L1; the scales wait in shared memory for the sums.  One after the other (us, tokens x
+// channels x K): 64 x 4096 x 4096 10.6 -> 8.9, 1 x 22016 x 4096 19.5 -> 17.6, 64 x 4096 x 11008 14.5 -> 13.4; norm, product, SiLU and
+// product of a layer of 4096 and 11008: 37.5 -> 33.9 for one token, 46.2 -> 43.0 for 64.
 constexpr int kSkinnyThreads = 192;
 template <int TN> struct Skinny {
     static_assert(TN == 16 || TN == 32 || TN == 64 || TN == 128, "tokens of a tile");
@@ -255,7 +261,8 @@ template <int TN> struct Skinny {
     static constexpr int kBody = kStages * kStageBytes > kDump ? kStages * kStageBytes : kDump;
     static constexpr int kOffBar = kBody;
     static constexpr int kOffMisc = kOffBar + (2 * kStages + 1) * 8;
-    static constexpr int kSmem = kOffMisc + 16 + 1024;
+    static constexpr int kOffScale = kOffMisc + 16;                 // of the tile's tokens, of its channels
+    static constexpr int kSmem = kOffScale + (TN + 128) * 4 + 1024;
     static constexpr int kCols = TN < 32 ? 32 : TN;
 };
 
@@ -286,6 +293,8 @@ __global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
+    grid_dependency_wait();
+    grid_dependents_launch();
     bool ok = !*s_abort;
 
     if (warp == 0) {
@@ -320,7 +329,12 @@ __global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __
         }
     }
     int32_t* dump = reinterpret_cast<int32_t*>(gen);                      // [TN][128]
+    float* s_scale = reinterpret_cast<float*>(gen + C::kOffScale);
     if (warp >= 2) {
+        for (int i = threadIdx.x - 64; i < TN + 128; i += 128) {          // while the MMAs run
+            const int64_t at = i < TN ? m0 + i : n0 + (i - TN);
+            s_scale[i] = at < (i < TN ? p.M : p.N) ? __ldcg((i < TN ? p.a_scale : p.w_scale) + at) : 0.f;
+        }
         const int q = warp & 3;                                           // the quarter of the tensor-memory lanes this warp may read
         if (ok) ok = mm_wait(bar(2 * C::kStages), 0, s_abort, MW_DRAIN, nk);
         ok = __all_sync(0xffffffffu, ok);
@@ -357,11 +371,11 @@ __global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __
                 asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v0), "=r"(v1) : "r"(at));
                 s0 += v0; s1 += v1;
             }
-            const float sa = p.a_scale[m];
-            const float x0 = __int2float_rn(s0) * sa * p.w_scale[n];
+            const float sa = s_scale[t];
+            const float x0 = __int2float_rn(s0) * sa * s_scale[TN + ch];
             OT* o = out + m * p.ldo + n;
             if (n + 1 < N) {
-                const float x1 = __int2float_rn(s1) * sa * p.w_scale[n + 1];
+                const float x1 = __int2float_rn(s1) * sa * s_scale[TN + ch + 1];
                 if (p.vec_out) {
                     if constexpr (sizeof(OT) == 2) *reinterpret_cast<uint32_t*>(o) = Cvt<OT>::pack(x0, x1);
                     else *reinterpret_cast<float2*>(o) = make_float2(x0, x1);
@@ -463,10 +477,12 @@ static int launch_skinny(const int8_t* a, int64_t lda, const int8_t* w, int64_t 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(nt * splits), (unsigned)mt); cfg.blockDim = dim3(kSkinnyThreads);
     cfg.dynamicSmemBytes = C::kSmem; cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = splits; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
     ESP_CUDA_TRY(cudaFuncSetAttribute(mm_w8a8_skinny_kernel<OT, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     ESP_CUDA_TRY(cudaLaunchKernelEx(&cfg, mm_w8a8_skinny_kernel<OT, TN>, ta, tw, g, splits));
     return ESP_OK;
@@ -478,7 +494,8 @@ static int launch_mm(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw,
     g.vec_out = ((uintptr_t)g.out % 16 == 0 && (g.ldo * (int64_t)sizeof(OT)) % 16 == 0) ? 1 : 0;
     // The variant with the least estimated time (us).  A skinny CTA costs about 6 us around its stages; a stage costs less while
     // every SM has one CTA than with two (which then share the SM's intake).  A pair costs 5.4 or 6.5 us and 0.29 or 0.31 us per
-    // stage and wave of tiles.  Measured against these estimates (B200, tokens x channels x K, us):
+    // stage and wave of tiles.  Measured against these estimates (B200, tokens x channels x K, us,
+    // each call by itself; with its start under the kernel before it a skinny one takes 1 to 2 us less):
     //   64 x 4096 x 11008: TN 64 in 8 splits 13.8, 4 splits 15.2, 1 split 29.2, pairs 31.0      256 x 4096 x 11008: TN 128 in 4 splits 20.1, pairs 31.0
     //   256 x 22016 x 4096: TN 64 50.8, TN 128 54.3, pairs of 256 29.7                          512 x 4096 x 1280: TN 64 12.9, pairs of 128 8.3, of 256 9.6
     //   600 x 600 x 8000: TN 64 in 4 splits 12.4, TN 128 in 8 splits 12.5, pairs of 128 24.6    400 x 8000 x 2992: pairs of 256 17.2, of 128 21.0, TN 128 36.7

@@ -632,3 +632,44 @@ def test_empty_batches_do_nothing():
                                           torch.zeros(2, 8, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV),
                                           torch.zeros(2, dtype=torch.int32, device=DEV), 0)
     assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 64])
+def test_row_kernels_and_products_in_a_chain(tokens):
+    """A layer's norm, product, SiLU and product, three layers in one graph over shared buffers: every product waits for its rows, and
+    every row kernel for the product before it."""
+    from loongserve_b200 import layer_ops as ops
+    H, Fn = 1024, 2816
+    g = torch.Generator().manual_seed(tokens)
+    w1 = ops.quantize_rows((torch.randn(2 * Fn, H, generator=g) * H ** -0.5).to(BF16).to(DEV))
+    w2 = ops.quantize_rows((torch.randn(H, Fn, generator=g) * Fn ** -0.5).to(BF16).to(DEV))
+    nw = torch.rand(H, generator=g).to(BF16).to(DEV)
+    x = torch.empty(tokens, H, dtype=BF16, device=DEV); res = torch.empty_like(x)
+    codes, scale = torch.empty(tokens, H, dtype=INT8, device=DEV), torch.empty(tokens, device=DEV)
+    gu = torch.empty(tokens, 2 * Fn, dtype=BF16, device=DEV)
+    codes2, scale2 = torch.empty(tokens, Fn, dtype=INT8, device=DEV), torch.empty(tokens, device=DEV)
+
+    def layers(sync):
+        for _ in range(3):
+            for f in (lambda: ops.add_rms_norm_quant(x, res, nw, 1e-5, codes, scale), lambda: ops.mm_w8a8(codes, scale, *w1, out=gu),
+                      lambda: ops.silu_and_mul_quant(gu, codes2, scale2), lambda: ops.mm_w8a8(codes2, scale2, *w2, out=x)):
+                f()
+                if sync:
+                    torch.cuda.synchronize()
+
+    x.normal_(); res.normal_()
+    layers(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layers(False)
+    for seed in range(4):
+        g.manual_seed(seed)
+        a, b = torch.randn(tokens, H, generator=g).to(BF16).to(DEV), torch.randn(tokens, H, generator=g).to(BF16).to(DEV)
+        x.copy_(a); res.copy_(b)
+        layers(True)
+        want = x.clone(), res.clone(), codes2.clone(), scale2.clone()
+        for run in (graph.replay, lambda: layers(False)):
+            x.copy_(a); res.copy_(b)
+            run()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(want, (x, res, codes2, scale2)))
