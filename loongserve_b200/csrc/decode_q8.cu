@@ -208,6 +208,10 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         for (int i = 0; i < R::kStages; ++i) { ptx::mbar_init(full(i), 33); ptx::mbar_init(empty(i), kQ8Warps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // The queries, the pool and the lengths are there from here on; what is above may run while the kernel ahead ends (one request of
+    // 512 tokens 10.1 -> 9.3 us, 64 of up to 512 18.1 -> 17.5).  Neither this kernel nor the merge lets the next one start earlier than
+    // that: CTAs placed while some SMs are still busy end up uneven (that 19.5 us; two requests in splits of 4096 tokens 237 -> 320).
+    grid_dependency_wait();
     auto blocks_of = [&](int len) { return len <= 0 ? 0 : min((len - 1) / a.seq_block_size + 1, a.num_blocks); };
     const int unit = a.ranges ? R::kTokens : a.seq_block_size;
     if (a.counted) {
@@ -620,20 +624,20 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
 // one warp per row leaves most of the GPU idle (130 us; four warps 31 us).  Warp w takes splits w, w + W, ...; lanes hold four
 // dims each.
 template <int W>
-__global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float* __restrict__ lse, const int32_t* __restrict__ b_seqlen,
-                                                                 const float* __restrict__ mid_o, const float* __restrict__ mid_lse,
-                                                                 const int* __restrict__ parts,
+__global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float* lse, const int32_t* b_seqlen,
+                                                                 const float* mid_o, const float* mid_lse, const int* parts,
                                                                  int batch, int num_heads, int num_blocks, int block_seq, int o_dtype) {
     const int pair = blockIdx.x, b = pair / num_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dependency_wait();                                    // its loads pass the L1: it may have started before stage 1 ended
     int n;
     int64_t bh, row0;                                          // rows from one split to the next, row of the first
     if (parts != nullptr) {
-        n = parts[2 * b + 1];
+        n = __ldcg(parts + 2 * b + 1);
         if (n == 1) return;                                    // stage 1 has written the results
         bh = num_heads;
-        row0 = (int64_t)parts[2 * b] * num_heads + (pair - b * num_heads);
+        row0 = (int64_t)__ldcg(parts + 2 * b) * num_heads + (pair - b * num_heads);
     } else {
-        const int len = b_seqlen[b];
+        const int len = __ldcg(b_seqlen + b);
         n = len <= 0 ? 0 : min((len - 1) / block_seq + 1, num_blocks);
         bh = (int64_t)batch * num_heads;
         row0 = pair;
@@ -643,7 +647,7 @@ __global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float*
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j0 = warp; j0 < n; j0 += W * 32) {                // up to 32 splits of this warp at a time, one lse per lane
         const int j = j0 + W * lane;
-        const float x = j < n ? mid_lse[j * bh + row0] : -INFINITY;
+        const float x = j < n ? __ldcg(mid_lse + j * bh + row0) : -INFINITY;
         float mx = x;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float*
 #pragma unroll 8
         for (int i = 0; i < cnt; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float4 v = *reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + W * i) * bh + row0) * 128 + lane * 4);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(mid_o + ((int64_t)(j0 + W * i) * bh + row0) * 128 + lane * 4));
             acc.x = fmaf(wi, v.x, acc.x); acc.y = fmaf(wi, v.y, acc.y); acc.z = fmaf(wi, v.z, acc.z); acc.w = fmaf(wi, v.w, acc.w);
         }
     }
@@ -726,11 +730,10 @@ static int launch_stage1_q8(DecodeQ8Args& a, cudaStream_t s) {
 #define ESP_S1Q(NH)                                                                                                               \
     {                                                                                                                            \
         ESP_CUDA_TRY(cudaFuncSetAttribute(decode_stage1_q8_kernel<CODE, NH, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, RingQ8<NH>::kSmem)); \
-        decode_stage1_q8_kernel<CODE, NH, GT><<<grid, kQ8Warps * 32 + 32, RingQ8<NH>::kSmem, s>>>(a);                                              \
+        ESP_CUDA_TRY(launch_early(decode_stage1_q8_kernel<CODE, NH, GT>, grid, kQ8Warps * 32 + 32, RingQ8<NH>::kSmem, s, a));                     \
     }
     if (nh == 4) ESP_S1Q(4) else if (nh == 2) ESP_S1Q(2) else ESP_S1Q(1)
 #undef ESP_S1Q
-    ESP_LAUNCH_CHECK("decode_stage1_q8_kernel");
     return ESP_OK;
 }
 
@@ -805,7 +808,7 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     if (o_dtype != ESP_DTYPE_F16 && o_dtype != ESP_DTYPE_BF16 && o_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
     const int32_t max_len = max_len_in_batch > 0 ? max_len_in_batch : 1;
     // seq_block_size 0: equal pieces, or one split where no request is longer than 256 tokens (512 from 8 requests on), which saves
-    // the merge.  Pieces / one split in us, 8 kv heads, group 4: one request of 256 tokens 8.2 / 8.3, of 512 9.9 / 11.3; 16 ragged ones
+    // the merge.  Pieces / one split in us (both 0.6 more than they are now), 8 kv heads, group 4: one request of 256 tokens 8.2 / 8.3, of 512 9.9 / 11.3; 16 ragged ones
     // of up to 512 13.4 / 11.1, 64 of them 19.5 / 18.3, 256 50.3 / 51.0.
     const bool even = seq_block_size == 0 && max_len > q8_whole(batch);
     const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : max_len) : seq_block_size;
@@ -825,10 +828,8 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     if (rc || nblk == 1) return rc;
     const unsigned pairs = (unsigned)((int64_t)batch * num_q_heads);
     // splits of one request, on average
-    if ((even ? a.ranges / batch : nblk) > 64)
-        decode_merge_q8_kernel<16><<<pairs, 512, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, a.parts, batch, num_q_heads, (int)nblk, block, o_dtype);
-    else
-        decode_merge_q8_kernel<4><<<pairs, 128, 0, s>>>(o, lse, b_seqlen, a.mid_o, a.mid_lse, a.parts, batch, num_q_heads, (int)nblk, block, o_dtype);
-    ESP_LAUNCH_CHECK("decode_merge_q8_kernel");
+    const bool wide = (even ? a.ranges / batch : nblk) > 64;
+    ESP_CUDA_TRY(launch_early(wide ? decode_merge_q8_kernel<16> : decode_merge_q8_kernel<4>, dim3(pairs), wide ? 512 : 128, 0, s, o, lse, b_seqlen,
+                              a.mid_o, a.mid_lse, a.parts, batch, num_q_heads, (int)nblk, block, o_dtype));
     return ESP_OK;
 }

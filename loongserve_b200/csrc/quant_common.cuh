@@ -26,6 +26,18 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // From here on (once every CTA has passed or left) a kernel behind this one that was launched so may start.
 __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Launch of a kernel that begins with grid_dependency_wait.
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.attrs = &at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 
 struct RowScale { float inv, scale; bool finite; };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits, float top) {

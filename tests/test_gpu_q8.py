@@ -673,3 +673,44 @@ def test_row_kernels_and_products_in_a_chain(tokens):
             run()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(want, (x, res, codes2, scale2)))
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("lens", [[40, 9], [3000, 1200, 1, 700]])
+def test_pool_writes_and_decode_in_a_chain(code, lens):
+    """A step's rows are written, attended to with a query that the step before made, three times in one graph: each kernel waits for the
+    one ahead of it, and calls that take turns on one workspace do not meet."""
+    from loongserve_b200 import flash_decoding as fd, kv_ops
+    hq, hkv = 8, 4
+    B = len(lens)
+    c = decode_case(lens, hq, hkv, BF16, code, 31)
+    a = (c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"], c["rows"], c["lens"], max(lens))
+    last = torch.stack([c["table"][int(c["rows"][b]), n - 1] for b, n in enumerate(lens)]).to(torch.int64)
+    kv = torch.empty(B, 2 * hkv, D, dtype=BF16, device=DEV); q = torch.empty(B, hq, D, dtype=BF16, device=DEV)
+    lse = torch.empty(B, hq, device=DEV)
+
+    def steps(sync):
+        for _ in range(3):
+            for f in (lambda: kv_ops.destindex_copy_quantize_kv(kv, last, c["codes"], c["scales"]),
+                      lambda: fd.token_decode_attention_q8(q, *a, out=q, out_logexpsum=lse), lambda: kv.copy_(q[:, :2 * hkv])):
+                f()
+                if sync:
+                    torch.cuda.synchronize()
+
+    kv.normal_(); q.normal_()
+    steps(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps(False)
+    g = torch.Generator()
+    for seed in range(4):
+        g.manual_seed(seed)
+        x, y = torch.randn(B, 2 * hkv, D, generator=g).to(BF16).to(DEV), torch.randn(B, hq, D, generator=g).to(BF16).to(DEV)
+        kv.copy_(x); q.copy_(y)
+        steps(True)
+        want = q.clone(), lse.clone(), kv.clone()
+        for run in (graph.replay, lambda: steps(False)):
+            kv.copy_(x); q.copy_(y)
+            run()
+            torch.cuda.synchronize()
+            assert all(torch.equal(m, n) for m, n in zip(want, (q, lse, kv)))
