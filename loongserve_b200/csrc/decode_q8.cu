@@ -417,8 +417,9 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const bool finite = amax < 0x7f800000u;              // a query with inf or NaN: NaN
-        // 2^(kQExp - e) with 2^e <= max|q|; e held in [-90, 126] so that both powers are normal numbers
-        const int e = min(max((int)(amax >> 23) - 127, -90), 126);
+        // 2^(kQExp - e) with 2^e <= max|q| < 2^(e + 1): the scaled query lies below 2^(kQExp + 1), which the digits below hold.  e is at
+        // least -90, so that both powers are normal numbers, and at most 127 (the largest exponent of bf16), where they are normal too.
+        const int e = max((int)(min(amax, 0x7f7fffffu) >> 23) - 127, -90);
         const float up = __uint_as_float((uint32_t)(127 + kQExp - e) << 23);
         qs = finite ? a.scale_log2 * __uint_as_float((uint32_t)(127 - kQExp + e) << 23) : __uint_as_float(0x7fc00000u);
 #pragma unroll

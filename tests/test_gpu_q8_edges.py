@@ -1,0 +1,28 @@
+"""Edges of the 8-bit operators beside those of tests/test_gpu_q8.py, with its definitions, inputs and tolerances unless a test derives
+its own."""
+import pytest
+import torch
+
+from test_gpu_q8 import BF16, D, DEV, E4M3, INT8, check_decode, decode_case, decode_exact
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 2), (10, 2), (16, 2)])
+def test_decode_with_the_largest_queries(code, hq, hkv):
+    """+-finfo(bf16).max in a query, K scales of 2^-126 that bring the scores back to about a hundred: signs and sizes hold, in the
+    digits of groups of up to four heads and of more."""
+    from loongserve_b200 import flash_decoding as fd
+    c = decode_case([40, 300], hq, hkv, BF16, code, 17)
+    top = torch.finfo(BF16).max
+    c["scales"][:, :hkv] = 2.0 ** -126
+    c["q"][0, 0, 3] = top
+    c["q"][0, -1, 0] = -top; c["q"][0, -1, 127] = top
+    c["q"][1, 0, 64] = -top
+    c["q"][1, -1] = top
+    out = torch.empty(2, hq, D, device=DEV); lse = torch.empty(2, hq, device=DEV)
+    for block in (None, 64):
+        fd.token_decode_attention_q8(c["q"], c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"],
+                                     c["rows"], c["lens"], 300, block, out, lse)
+        check_decode(out, lse, decode_exact(c), 300)
