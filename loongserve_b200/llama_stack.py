@@ -98,7 +98,9 @@ class LlamaESPStack:
     def _w8a8_rest(self, x, o, lw):
         """Output projection, x += it, and the FFN; the FFN's output is left for the next norm to add."""
         cfg = self.cfg
-        att = layer_ops.mm_w8a8(*layer_ops.quantize_rows(o.view(x.shape[0], -1)), *lw["o"], out_dtype=x.dtype)
+        # the width is spelled out: an instance may hold no token of a prefill, and view(0, -1) is refused
+        o = o.view(x.shape[0], cfg.num_q_heads * cfg.head_dim)
+        att = layer_ops.mm_w8a8(*layer_ops.quantize_rows(o), *lw["o"], out_dtype=x.dtype)
         h, hs = layer_ops.add_rms_norm_quant(att, x, lw["ffn_norm"], cfg.rms_eps)
         gu = layer_ops.mm_w8a8(h, hs, *lw["gate_up"], out_dtype=x.dtype)
         return layer_ops.mm_w8a8(*layer_ops.silu_and_mul_quant(gu), *lw["down"], out_dtype=x.dtype)

@@ -26,3 +26,16 @@ def test_decode_with_the_largest_queries(code, hq, hkv):
         fd.token_decode_attention_q8(c["q"], c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"],
                                      c["rows"], c["lens"], 300, block, out, lse)
         check_decode(out, lse, decode_exact(c), 300)
+
+
+def test_a_layer_of_no_tokens():
+    """The 8-bit layer of an instance that holds no token of a prefill: every operator takes zero rows."""
+    from types import SimpleNamespace
+    from loongserve_b200.llama_stack import LlamaConfig, LlamaESPStack, LlamaW8A8Weights, LlamaWeights
+    cfg = LlamaConfig(num_layers=2, hidden=256, num_q_heads=4, num_kv_heads=2, head_dim=128, ffn=320, vocab=50)
+    scratch = torch.zeros(1, 4, D, dtype=BF16, device=DEV)
+    rt = SimpleNamespace(pre_cache_kv=lambda st, li: scratch, context_attention=lambda q, st, li: torch.empty_like(q))
+    stack = LlamaESPStack(cfg, LlamaW8A8Weights(cfg, LlamaWeights(cfg, BF16, DEV, seed=1)), rt)
+    none = torch.empty(0, dtype=torch.int64, device=DEV)
+    assert stack.prefill(none, none, None).shape == (0, 256) and stack.prefill(none, none, None, last_token_rows=none).shape == (0, 50)
+    torch.cuda.synchronize()

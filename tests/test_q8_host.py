@@ -1,0 +1,61 @@
+"""Host side of the 8-bit serving path: the Llama stack's glue around the operators, on stand-ins of their shapes (no GPU needed)."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from loongserve_b200 import llama_stack
+
+
+class Ops:
+    """The layer operators by their shapes."""
+
+    @staticmethod
+    def add_rms_norm_quant(x, residual, weight, eps):
+        assert residual is None or residual.shape == x.shape
+        return torch.zeros(x.shape, dtype=torch.int8), torch.ones(x.shape[0])
+
+    @staticmethod
+    def add_rms_norm(x, residual, weight, eps):
+        assert residual.shape == x.shape
+        return torch.zeros_like(x)
+
+    @staticmethod
+    def mm_w8a8(a, a_scale, w, w_scale, out_dtype=torch.bfloat16, out=None):
+        assert a.shape[1] == w.shape[1] and a_scale.shape == a.shape[:1]
+        if out is None:
+            return torch.zeros(a.shape[0], w.shape[0], dtype=out_dtype)
+        assert out.shape == (a.shape[0], w.shape[0])
+        return out.zero_()
+
+    @staticmethod
+    def quantize_rows(x):
+        return torch.zeros(x.shape, dtype=torch.int8), torch.ones(x.shape[0])
+
+    @staticmethod
+    def silu_and_mul_quant(io):
+        return torch.zeros(io.shape[0], io.shape[1] // 2, dtype=torch.int8), torch.ones(io.shape[0])
+
+    @staticmethod
+    def rotary_emb(q, k, cos, sin):
+        assert q.shape[0] == k.shape[0] == cos.shape[0]
+
+
+def stack_on_stand_ins(monkeypatch, max_tokens):
+    monkeypatch.setattr(llama_stack, "layer_ops", Ops)
+    cfg = llama_stack.LlamaConfig(num_layers=2, hidden=64, num_q_heads=4, num_kv_heads=2, head_dim=128, ffn=96, vocab=10)
+    q8 = lambda n, k: (torch.zeros(n, k, dtype=torch.int8), torch.ones(n))
+    layer = dict(att_norm=torch.ones(64), ffn_norm=torch.ones(64), q=q8(512, 64), kv=q8(512, 64), o=q8(64, 512), gate_up=q8(192, 64), down=q8(64, 96))
+    weights = SimpleNamespace(w8a8=True, embed=torch.zeros(10, 64), final_norm=torch.ones(64), lm_head=torch.zeros(64, 10), layers=[layer, layer])
+    scratch = torch.zeros(max_tokens, 4, 128)
+    rt = SimpleNamespace(pre_cache_kv=lambda st, li: scratch, context_attention=lambda q, st, li: torch.empty_like(q))
+    return llama_stack.LlamaESPStack(cfg, weights, rt)
+
+
+@pytest.mark.parametrize("n", [0, 1, 3])
+def test_a_prefill_of_which_an_instance_holds_few_tokens_or_none(monkeypatch, n):
+    """Striped placement leaves the higher instances without tokens where all prompts are shorter than the ring."""
+    stack = stack_on_stand_ins(monkeypatch, 4)
+    hidden = stack.prefill(torch.zeros(n, dtype=torch.long), torch.arange(n), None)
+    assert hidden.shape == (n, 64)
+    assert stack.prefill(torch.zeros(n, dtype=torch.long), torch.arange(n), None, last_token_rows=torch.arange(n)).shape == (n, 10)
