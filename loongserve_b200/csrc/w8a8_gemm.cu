@@ -81,7 +81,7 @@ template <int PN> struct Pair {
     static constexpr int kOffBar = kOffEpi + 4 * kEpiWarp;
     static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = 2 * kStages + 2, kDrain = 2 * kStages + 4, kBars = 2 * kStages + 5;
     static constexpr int kOffMisc = kOffBar + kBars * 8;
-    static constexpr int kSmem = kOffMisc + 16 + 1024;
+    static constexpr int kSmem = kOffMisc + 32 + 1024;
 };
 static_assert(Pair<256>::kSmem <= 232448 && Pair<128>::kSmem <= 232448, "shared memory of one CTA");
 
@@ -92,6 +92,25 @@ __device__ __forceinline__ void tile_of(int t, int m_tiles, int n_tiles, int& m,
     const int rows = min(kBand, m_tiles - band * kBand);
     n = in_band / rows;
     m = band * kBand + (in_band - n * rows);
+}
+
+// After a wait ran out: neither CTA may leave while MMAs or copies of either are under way, because copies write the CTA that started
+// them and count on the even CTA's barriers.  The two may have come a different number of steps far (issued, peer_issued): a step
+// that one of them alone has started is made to expect that CTA's bytes alone.  The issuing thread has committed kDrain.
+template <int PN>
+__device__ __noinline__ void pair_drain(uint32_t base, uint32_t cta, int issued, int peer_issued) {
+    using C = Pair<PN>;
+    auto bar = [base](int i) { return base + C::kOffBar + 8u * i; };
+    if (threadIdx.x == 32) mm_drain(bar(C::kDrain), 0);
+    if (cta == 0 && threadIdx.x == 0) {
+        const int hi = max(issued, peer_issued);
+        for (int i = max(hi - C::kStages, 0); i < hi; ++i) {
+            const uint32_t b = bar(C::kFull + i % C::kStages);
+            if (i >= issued) mbar_expect_tx(b, C::kStageBytes);
+            else if (i >= peer_issued) mbar_complete_tx(b, C::kStageBytes);
+            mm_drain(b, (i / C::kStages) & 1);
+        }
+    }
 }
 
 template <typename OT, int PN>
@@ -105,6 +124,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
     auto lbar = [&bar](int i) { return map_to_cta(bar(i), 0u); };               // the even CTA's barrier
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + C::kOffMisc);
     volatile int* s_abort = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 4);
+    volatile int* s_issued = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 8);     // steps whose copies this CTA has started
+    volatile int* s_peer = reinterpret_cast<volatile int*>(gen + C::kOffMisc + 16);      // the other CTA's s_abort and s_issued, at the end
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = cluster_ctarank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -112,6 +133,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
 
     if (threadIdx.x == 0) {
         *s_abort = (*reinterpret_cast<volatile int*>(&g_mm_status[0]) != 0) ? 1 : 0;    // after a reported timeout nothing is started
+        *s_issued = 0;
         for (int i = 0; i < C::kBars; ++i) mbar_init(bar(i), (i == C::kAccEmpty || i == C::kAccEmpty + 1) ? 8 : 1);
         fence_barrier_init();
         prefetch_tensormap(&tm_a); prefetch_tensormap(&tm_w);
@@ -141,8 +163,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
                     tma_load_2d_pair(dst + kPairM * kBK, &tm_w, lbar(C::kFull + st), k * kBK, n0);
                 }
             }
-            if (!ok && cta == 0)                               // copies of both CTAs count on the even CTA's barriers
-                for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) mm_drain(bar(C::kFull + i % C::kStages), (i / C::kStages) & 1);
+            // A look at the last steps, a millisecond each at most; what is still under way then is waited for at the end.  (Measured: with
+            // the loop above alone the compiler makes something of it that takes 1002 us instead of 995 for 16384 x 22016 x 4096.)
+            if (!ok && cta == 0)
+                for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) mbar_try_wait(bar(C::kFull + i % C::kStages), (i / C::kStages) & 1);
+            *s_issued = it;
         }
     } else if (warp == 1) {
         if (cta == 0 && lane == 0 && !*s_abort) {
@@ -165,7 +190,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
                 }
                 if (ok) umma_pair_commit(bar(C::kAccFull + buf));
             }
-            if (!ok) { umma_pair_commit(bar(C::kDrain)); mm_drain(bar(C::kDrain), 0); }
         }
     } else if (warp >= 4) {
         const int w = warp - 4;
@@ -238,7 +262,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) mm_w8a8_pair_kernel(const __g
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) {
+        st_cluster_u32(map_to_cta(base + C::kOffMisc + 16, cta ^ 1u), (uint32_t)*s_abort);
+        st_cluster_u32(map_to_cta(base + C::kOffMisc + 20, cta ^ 1u), (uint32_t)*s_issued);
+    }
     cluster_sync_all();                  // neither CTA frees tensor memory while the peer's MMAs may still use it
+    if (*s_abort | s_peer[0]) {          // a wait ran out in one of the CTAs: both see it here
+        if (threadIdx.x == 32 && cta == 0) umma_pair_commit(bar(C::kDrain));
+        pair_drain<PN>(base, cta, *s_issued, s_peer[1]);
+        __syncthreads();
+        cluster_sync_all();
+    }
     if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 2 * PN); }
 }
 
