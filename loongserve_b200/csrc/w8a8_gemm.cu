@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __
                 tma_load_2d(dst, &tm_w, bar(st), (k0 + it) * kBK, n0);
                 tma_load_2d(dst + 128 * kBK, &tm_a, bar(st), (k0 + it) * kBK, m0);
             }
-            if (!ok)
-                for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) mm_drain(bar(i % C::kStages), (i / C::kStages) & 1);
+            // whichever warp gives up, the CTA does not leave before the copies have landed
+            for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i) mm_drain(bar(i % C::kStages), (i / C::kStages) & 1);
         }
     } else if (warp == 1) {
         if (lane == 0 && ok) {

@@ -1,7 +1,7 @@
 """How a kernel of the 8-bit path ends after one of its bounded waits has run out, executed on the CPU.
 
 Copies go to shared memory on their own and are counted on mbarriers; a CTA that leaves while one is under way lets it write into
-whatever block comes next.  The model has the parts of the kernels in csrc/w8a8_gemm.cu: producers that start copies into a ring of
+whatever block comes next.  The model has the parts of the kernels in csrc/w8a8_gemm.cu and of stage 1 in csrc/decode_q8.cu: producers that start copies into a ring of
 stages, an issuer that consumes full stages and whose products hand them back later, waits that may run out at any moment, and the
 clean-up at the end.  They are run in many random orders that keep only what the machine guarantees.  Whatever the order: nothing may
 be under way when the CTAs leave, and the clean-up's own waits must end by themselves.  With a rule of the clean-up taken away the
@@ -41,7 +41,7 @@ ALL = frozenset({"every end", "both CTAs", "level"})
 
 
 class Kernel:
-    """`ctas` 1: the kernel for few tokens (copies and products of one CTA); 2: the pair kernel (each CTA copies its share, counted on
+    """`ctas` 1: the kernel for few tokens and decode stage 1 (copies and products of one CTA); 2: the pair kernel (each CTA copies its share, counted on
     the even CTA's barriers, whose issuer consumes both)."""
 
     def __init__(self, ctas, stages, steps, rules, rng):
@@ -160,3 +160,8 @@ def test_the_harness_notices_a_missing_rule(without):
     """every end: cleaned up whoever gave up, not only where the producer did; both CTAs: the odd CTA's copies too; level: a step that
     one CTA alone has started expects that CTA's bytes alone."""
     assert outcomes(2, ALL - {without}) != (True, True)
+
+
+def test_a_cta_leaves_nothing_under_way():
+    assert outcomes(1, ALL) == (True, True)
+    assert outcomes(1, ALL - {"every end"}) != (True, True)
