@@ -112,7 +112,9 @@ int esp_prefill_lse(const float* m, const float* l, float* lse, int64_t n, void*
 int esp_device_status(int32_t out[4], int32_t clear);
 
 /* Limit, in SM cycles, of every bounded in-kernel wait of this library on the CURRENT device (the mbarrier waits of the
- * prefill kernels and of esp_mm_w8a8, the flag waits of the gated decode kernels and of esp_flag_wait).  Default 2e9 (about a second).
+ * prefill kernels, of esp_mm_w8a8 and of the 8-bit decode, the flag waits of the gated decode kernels and of esp_flag_wait).  Default
+ * 2e9 (about a second).  Once a wait has run out, esp_mm_w8a8 and the 8-bit decode wait for their own copies by the default, whatever
+ * is set here.
  * The reference has no counterpart: its kernels never wait on one another, and its NCCL calls wait without a limit. */
 int esp_set_wait_limit_cycles(int64_t cycles);
 

@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         }
         // whichever warp gives up, the CTA does not leave before the copies have landed (bounded)
         for (int j = done > R::kStages ? done - R::kStages : 0; j < done; ++j)
-            ptx::mbar_wait_bounded(full(j % R::kStages), (j / R::kStages) & 1, &g_decode_q8_wait_limit_cycles, nullptr);
+            ptx::mbar_wait_bounded(full(j % R::kStages), (j / R::kStages) & 1, &kDrainLimitCycles, nullptr);
         return;
     }
     const int g = lane >> 2, c = lane & 3;

@@ -39,6 +39,10 @@ inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, in
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+// Limit, in SM cycles, of the waits for work of one's own that is still in flight after a wait has run out.  It is not the limit that
+// esp_set_wait_limit_cycles sets: a short one ends waits for others early, but not those for copies that write this CTA's memory.
+static __device__ const long long kDrainLimitCycles = 2000000000LL;
+
 struct RowScale { float inv, scale; bool finite; };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits, float top) {
     RowScale r;

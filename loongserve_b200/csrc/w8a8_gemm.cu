@@ -37,7 +37,7 @@ __device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, volatile 
 }
 // after an abort: wait (bounded, whatever the abort flag says) for work of one's own that is still in flight
 __device__ __forceinline__ void mm_drain(uint32_t bar, uint32_t parity) {
-    mbar_wait_bounded(bar, parity, &g_mm_wait_limit_cycles, nullptr);
+    mbar_wait_bounded(bar, parity, &kDrainLimitCycles, nullptr);
 }
 
 template <typename OT> __device__ __forceinline__ OT from_f32(float x);

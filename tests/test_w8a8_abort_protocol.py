@@ -37,7 +37,7 @@ class Bar:
         return self.phase != parity
 
 
-ALL = frozenset({"every end", "both CTAs", "level"})
+ALL = frozenset({"every end", "both CTAs", "level", "limit of its own"})
 
 
 class Kernel:
@@ -116,7 +116,7 @@ class Kernel:
         """The bounded wait for step i's stage; False where only its limit would end it."""
         bar, parity = self.full[i % self.S], (i // self.S) & 1
         while not bar.done(parity):
-            if not self.flight:
+            if not self.flight or "limit of its own" not in self.rules and self.rng.random() < 0.1:
                 return False
             self.land()
         return True
@@ -158,10 +158,11 @@ def test_a_pair_leaves_nothing_under_way():
 @pytest.mark.parametrize("without", sorted(ALL))
 def test_the_harness_notices_a_missing_rule(without):
     """every end: cleaned up whoever gave up, not only where the producer did; both CTAs: the odd CTA's copies too; level: a step that
-    one CTA alone has started expects that CTA's bytes alone."""
+    one CTA alone has started expects that CTA's bytes alone; limit of its own: a short limit of the waits does not end the clean-up's."""
     assert outcomes(2, ALL - {without}) != (True, True)
 
 
 def test_a_cta_leaves_nothing_under_way():
     assert outcomes(1, ALL) == (True, True)
-    assert outcomes(1, ALL - {"every end"}) != (True, True)
+    for rule in ("every end", "limit of its own"):
+        assert outcomes(1, ALL - {rule}) != (True, True)
