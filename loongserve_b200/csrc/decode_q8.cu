@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     int* s_first = s_len + kQ8MaxCounted;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == kQ8Warps * 32) {                                   // not a thread that waits for the first lengths
-        *s_abort = *reinterpret_cast<volatile int*>(&g_decode_q8_status[0]) == ESP_ERR_DEVICE_TIMEOUT ? 1 : 0;
+        s_abort[0] = s_abort[1] = *reinterpret_cast<volatile int*>(&g_decode_q8_status[0]) == ESP_ERR_DEVICE_TIMEOUT ? 1 : 0;
         for (int i = 0; i < R::kStages; ++i) { ptx::mbar_init(full(i), 33); ptx::mbar_init(empty(i), kQ8Warps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
         const int tok = lane & 15, isv = lane >> 4;
         const int piece = lane % (NH * 8), share = lane / (NH * 8);         // 16 bytes of a row; which of an instruction's WT tokens
         const int64_t ssrc_stride = isv ? a.vs_stride_t : a.ks_stride_t;
-        bool ok = !*s_abort;
+        bool ok = !s_abort[1];
         int done = 0, st = 0, phase = 1;                                  // the first pass over the ring finds it empty
         ItemQ8 it;
         while (ok && next_item(it)) {
@@ -382,7 +382,9 @@ __global__ void __launch_bounds__(kQ8Warps * 32 + 32, 3) decode_stage1_q8_kernel
     }
     const int g = lane >> 2, c = lane & 3;
     const int hw = warp % NH, wt = warp / NH;            // kv head within the CTA, share of its tokens
-    bool ok = !*s_abort;
+    // s_abort[1] keeps its first value: the four warps meet at barriers inside the loop, so all of them enter it or none does, also where
+    // one has given up before another has come this far
+    bool ok = !s_abort[1];
     int st = 0, phase = 0, done = 0;
 
     ItemQ8 it;

@@ -166,3 +166,25 @@ def test_a_cta_leaves_nothing_under_way():
     assert outcomes(1, ALL) == (True, True)
     for rule in ("every end", "limit of its own"):
         assert outcomes(1, ALL - {rule}) != (True, True)
+
+
+def consumers(first_value_kept, rng):
+    """The four consumer warps of decode stage 1 over one item: each looks whether to start, waits for its stage (and may give up, which
+    sets the CTA's flag), and meets the others at a barrier.  True when all of them got past it."""
+    flag, at = [False, False], ["start"] * 4                       # the flag that moves, and the one that keeps its first value
+    while True:
+        able = [w for w in range(4) if at[w] in ("start", "wait")]
+        if not able:
+            return "barrier" not in at or at.count("barrier") == 4
+        w = rng.choice(able)
+        if at[w] == "start":
+            at[w] = "left" if flag[1 if first_value_kept else 0] else "wait"
+        else:
+            flag[0] = flag[0] or rng.random() < 0.3
+            at[w] = "barrier"
+
+
+def test_consumer_warps_all_start_or_none_does():
+    rng = random.Random(1)
+    assert all(consumers(True, rng) for _ in range(2000))
+    assert not all(consumers(False, rng) for _ in range(2000))
