@@ -6,8 +6,9 @@ Produces, next to this file:
   libesp_attention.so  -- kernels + C ABI declared in include/esp_attention.h
   libesp_rnccl.so      -- raw NCCL point-to-point layer declared in include/esp_rnccl.h
 Both link the shared CUDA runtime, so they use the same runtime instance as PyTorch in one process.
-`build_selftest()` builds the test-suite's own kernels (tests/csrc/selftest_kernels.cu) into tests/libesp_selftest.so;
-they are not part of the product library.
+`build_selftest()` builds the test-suite's own kernels (tests/csrc/selftest_kernels.cu) into tests/libesp_selftest.so,
+`build_short_waits()` builds the 8-bit kernels with waits that can run out at once into tests/libesp_short_waits.so.  Neither is part
+of the product library.
 """
 from __future__ import annotations
 
@@ -86,6 +87,18 @@ def build_selftest(force: bool = False) -> str:
     return SELFTEST_LIB
 
 
+SHORT_WAITS_SRC = os.path.join(ROOT, "tests", "csrc", "short_waits.cu")
+SHORT_WAITS_LIB = os.path.join(ROOT, "tests", "libesp_short_waits.so")
+
+
+def build_short_waits(force: bool = False) -> str:
+    deps = [SHORT_WAITS_SRC] + [os.path.join(CSRC, f) for f in ("esp_common.cuh", "sm100_ptx.cuh", "quant_common.cuh", "w8a8_gemm.cu", "decode_q8.cu")] + \
+        [os.path.join(ROOT, "include", "esp_attention.h")]
+    if force or _newer(SHORT_WAITS_LIB, deps):
+        _run([_nvcc()] + NVCC_FLAGS + ["-shared", SHORT_WAITS_SRC, "-o", SHORT_WAITS_LIB])
+    return SHORT_WAITS_LIB
+
+
 def build_rnccl(force: bool = False) -> str:
     src = os.path.join(CSRC, "rnccl.cpp")
     deps = [src, os.path.join(ROOT, "include", "esp_rnccl.h")]
@@ -101,6 +114,8 @@ def build_all(force: bool = False) -> None:
     build_rnccl(force)
     if os.path.exists(SELFTEST_SRC):
         build_selftest(force)
+    if os.path.exists(SHORT_WAITS_SRC):
+        build_short_waits(force)
 
 
 if __name__ == "__main__":

@@ -19,6 +19,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 #ifndef ESP_MBAR_SUSPEND_HINT_NS
 #define ESP_MBAR_SUSPEND_HINT_NS 1000000u
 #endif
+// Polls between two looks at the abort flag and the clock in a bounded wait.
+#ifndef ESP_MBAR_POLLS_PER_LOOK
+#define ESP_MBAR_POLLS_PER_LOOK 64u
+#endif
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -40,11 +44,19 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
+#ifdef ESP_MBAR_NEVER_SUSPEND           // the test-suite's kernels with short waits
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+#else
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok) : "r"(bar), "r"(parity), "r"(ESP_MBAR_SUSPEND_HINT_NS) : "memory");
+#endif
     return ok != 0;
 }
 
@@ -56,7 +68,7 @@ __device__ __forceinline__ int mbar_wait_bounded(uint32_t bar, uint32_t parity, 
     const long long t0 = clock64();
     uint32_t spins = 0;
     while (!mbar_try_wait(bar, parity)) {
-        if ((++spins & 63u) == 0) {
+        if (++spins % ESP_MBAR_POLLS_PER_LOOK == 0) {
             if (abort != nullptr && *abort) return 1;
             if (clock64() - t0 > *reinterpret_cast<const volatile long long*>(limit_cycles)) return 2;
         }
@@ -199,6 +211,8 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

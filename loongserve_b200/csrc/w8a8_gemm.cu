@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __
     if (warp == 1) { tmem_alloc(base + C::kOffMisc, C::kCols); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
+    if (splits > 1) cluster_arrive();                                     // s_abort is set up: the other CTAs may write it
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
     grid_dependency_wait();
@@ -385,10 +386,14 @@ __global__ void __launch_bounds__(kSkinnyThreads) mm_w8a8_skinny_kernel(const __
             tc_fence_before();
         }
     }
-    // every CTA of the cluster passes here, also one whose waits ran out (its partials are then not there: the status says so)
+    // Every CTA of the cluster passes here.  One whose waits ran out has no partials: it tells the others, and nothing is written.
     __syncthreads();
-    if (splits > 1) cluster_sync_all();
-    {
+    if (splits > 1) {
+        cluster_wait();
+        if (threadIdx.x < splits && *s_abort) st_cluster_u32(map_to_cta(base + C::kOffMisc + 4, threadIdx.x), 1u);
+        cluster_sync_all();
+    }
+    if (!*s_abort) {
         OT* out = reinterpret_cast<OT*>(p.out);
         const int t_lo = TN * split / splits, t_hi = TN * (split + 1) / splits;
         const int64_t M = p.M, N = p.N;

@@ -1,0 +1,80 @@
+"""What the 8-bit product kernels do once a bounded wait has run out, on their own code with waits that can be made short
+(tests/csrc/short_waits.cu): they return, the status names the wait, what they write is right or not written at all, a later call
+writes nothing until the status has been read, and after that everything works.  Nothing hangs or faults: every wait is bounded, and
+the kernels wait for their own copies and products before they leave."""
+import ctypes as C
+
+import pytest
+import torch
+
+from test_gpu_q8 import DEV
+
+pytestmark = pytest.mark.gpu
+FULL = 2_000_000_000
+TIMEOUT = -4
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from loongserve_b200 import _lib, build
+    short = C.CDLL(build.build_short_waits())
+    for name in ("esp_mm_w8a8", "esp_decode_attention_q8", "esp_decode_stage1_q8"):
+        getattr(short, name).argtypes = _lib.ATTN_SIGNATURES[name]
+        getattr(short, name).restype = C.c_int32
+    short.esp_short_limit.argtypes = [C.c_int64]
+    yield short
+    short.esp_short_limit(FULL)
+
+
+def status(lib):
+    buf = (C.c_int32 * 8)()
+    assert lib.esp_short_status(buf) == 0
+    return tuple(buf[:4]), tuple(buf[4:])
+
+
+def run_out(lib, call, results, want, which):
+    """call() with limits from one cycle to some twenty thousand; results: what it writes, want: what it should."""
+    status(lib)
+    ran_out = 0
+    for limit in (1, 300, 1000, 2000, 4000, 8000, 20000, 1):
+        for r in results:
+            r.fill_(7.0)
+        assert lib.esp_short_limit(limit) == 0
+        call()
+        torch.cuda.synchronize()
+        for r, w in zip(results, want):
+            assert bool(((r == 7.0) | (r == w)).all())                # what is written is right
+        again = [r.clone() for r in results]
+        call()                                                         # once the status is set nothing is started
+        st = status(lib)
+        if st[which][0]:
+            assert st[which][0] == TIMEOUT
+            ran_out += 1
+        else:
+            assert all(torch.equal(r, w) for r, w in zip(results, want))
+        if limit == 1:
+            assert st[which][0] == TIMEOUT
+            assert all(torch.equal(r, a) for r, a in zip(results, again))
+        assert lib.esp_short_limit(FULL) == 0
+        call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(r, w) for r, w in zip(results, want)) and status(lib)[which][0] == 0
+    assert ran_out >= 2
+
+
+# few tokens: 1, 2 and 8 splits of K, tiles of 16 to 128 tokens; pairs over 256 and 128 channels, one tile each and several
+@pytest.mark.parametrize("m,n,k", [(1, 100, 112), (16, 4096, 4096), (33, 300, 11008), (64, 4096, 11008), (200, 600, 8000), (512, 4096, 1280),
+                                   (300, 22016, 4096), (5000, 333, 512), (2049, 5000, 400)])
+def test_products(lib, m, n, k):
+    from loongserve_b200 import layer_ops as ops
+    g = torch.Generator(device=DEV).manual_seed(m + n)
+    a = torch.randint(-128, 128, (m, k), generator=g, device=DEV, dtype=torch.int8)
+    w = torch.randint(-128, 128, (n, k), generator=g, device=DEV, dtype=torch.int8)
+    sa, sw = torch.rand(m, generator=g, device=DEV) + 0.1, torch.rand(n, generator=g, device=DEV) + 0.1
+    want = ops.mm_w8a8(a, sa, w, sw, out_dtype=torch.float32)
+    out = torch.empty_like(want)
+    s = torch.cuda.current_stream().cuda_stream
+
+    def call():
+        assert lib.esp_mm_w8a8(out.data_ptr(), n, a.data_ptr(), k, sa.data_ptr(), w.data_ptr(), k, sw.data_ptr(), m, n, k, 2, s) == 0
+    run_out(lib, call, [out], [want], 0)
