@@ -667,12 +667,13 @@ __global__ void __launch_bounds__(W * 32) decode_merge_q8_kernel(void* o, float*
             acc.x = fmaf(wi, v.x, acc.x); acc.y = fmaf(wi, v.y, acc.y); acc.z = fmaf(wi, v.z, acc.z); acc.w = fmaf(wi, v.w, acc.w);
         }
     }
+    const int status = __ldcg(&g_decode_q8_status[0]);         // looked at before the results are written
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
     *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
     __syncthreads();
-    if (threadIdx.x >= 128) return;
+    if (threadIdx.x >= 128 || status == ESP_ERR_DEVICE_TIMEOUT) return;       // of a stage 1 that gave up, partials are missing
     float M = s_m[0];
 #pragma unroll
     for (int w = 1; w < W; ++w) M = fmaxf(M, s_m[w]);

@@ -1,4 +1,4 @@
-"""What the 8-bit product kernels do once a bounded wait has run out, on their own code with waits that can be made short
+"""What the 8-bit product and decode kernels do once a bounded wait has run out, on their own code with waits that can be made short
 (tests/csrc/short_waits.cu): they return, the status names the wait, what they write is right or not written at all, a later call
 writes nothing until the status has been read, and after that everything works.  Nothing hangs or faults: every wait is bounded, and
 the kernels wait for their own copies and products before they leave."""
@@ -7,7 +7,7 @@ import ctypes as C
 import pytest
 import torch
 
-from test_gpu_q8 import DEV
+from test_gpu_q8 import BF16, DEV, E4M3, INT8, decode_case
 
 pytestmark = pytest.mark.gpu
 FULL = 2_000_000_000
@@ -78,3 +78,19 @@ def test_products(lib, m, n, k):
     def call():
         assert lib.esp_mm_w8a8(out.data_ptr(), n, a.data_ptr(), k, sa.data_ptr(), w.data_ptr(), k, sw.data_ptr(), m, n, k, 2, s) == 0
     run_out(lib, call, [out], [want], 0)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("lens,hq,hkv", [([300], 8, 2), ([5000, 0, 1, 700], 8, 2), ([40] * 100 + [3000], 16, 16), ([200] * 40, 20, 2)])
+def test_decode(lib, code, lens, hq, hkv):
+    from loongserve_b200 import _lib, flash_decoding as fd
+    c = decode_case(lens, hq, hkv, BF16, code, 3)
+    a = (c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"], c["rows"], c["lens"], max(lens))
+    out, lse = torch.empty(len(lens), hq, 128, dtype=torch.float32, device=DEV), torch.empty(len(lens), hq, device=DEV)
+    want = [t.clone() for t in fd.token_decode_attention_q8(c["q"], *a, None, out, lse)]
+    real = _lib.attn
+    try:
+        _lib.attn = lambda: lib
+        run_out(lib, lambda: fd.token_decode_attention_q8(c["q"], *a, None, out, lse), [out, lse], want, 1)
+    finally:
+        _lib.attn = real
