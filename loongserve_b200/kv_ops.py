@@ -174,8 +174,10 @@ def destindex_copy_quantize_and_register_kv(batch_size, new_kv_cache_len, kv_ran
                                             req_to_token_indexs, b_req_idx, num_used_mem_index: int, max_len_in_batch: int,
                                             should_register_kv: bool):
     """``destindex_copy_and_register_kv`` into a pool held in 8 bits (``total_kv_cache`` codes, ``total_kv_scale`` scales)."""
-    need_here(kv, total_kv_cache, total_kv_scale, mem_index, req_to_token_indexs, new_kv_cache_len_sum)
-    need_i32(new_kv_cache_len, kv_range_begin, kv_range_end, kv_b_start_loc, cur_kv_cache_index, b_req_idx)
+    vectors = (new_kv_cache_len, kv_range_begin, kv_range_end, kv_b_start_loc, cur_kv_cache_index, b_req_idx)
+    need_here(kv, total_kv_cache, total_kv_scale, mem_index, req_to_token_indexs, new_kv_cache_len_sum, *vectors)
+    need_i32(*vectors)
+    assert all(v.numel() >= batch_size for v in (new_kv_cache_len_sum, *vectors)), "expected an entry for every request"
     assert new_kv_cache_len_sum.dtype == torch.int64 and new_kv_cache_len_sum.is_contiguous()
     heads, dim, _ = _rows(kv)
     slots, h, d, code, row, head, srow = _q8_pool(total_kv_cache, total_kv_scale)

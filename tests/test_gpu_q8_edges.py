@@ -39,3 +39,21 @@ def test_a_layer_of_no_tokens():
     none = torch.empty(0, dtype=torch.int64, device=DEV)
     assert stack.prefill(none, none, None).shape == (0, 256) and stack.prefill(none, none, None, last_token_rows=none).shape == (0, 50)
     torch.cuda.synchronize()
+
+
+def test_keep_range_write_refuses_vectors_of_the_host():
+    from loongserve_b200 import kv_ops
+    from test_gpu_q8 import pool
+    dev = lambda *x, dtype=torch.int32: torch.tensor(x, dtype=dtype, device=DEV)
+    raw, codes, scales = pool(8, 2, INT8)
+    before = raw.clone()
+    a = [1, dev(2), dev(0), dev(2), dev(2, dtype=torch.int64), torch.randn(4, 2, D, device=DEV).to(BF16), dev(0), dev(0), dev(3, 1, dtype=torch.int64),
+         codes, scales, torch.zeros(2, 8, dtype=torch.int32, device=DEV), dev(0), 0, 2, True]
+    for i in (1, 2, 3, 4, 6, 7, 8, 11, 12):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            kv_ops.destindex_copy_quantize_and_register_kv(*a[:i], a[i].cpu(), *a[i + 1:])
+    with pytest.raises(AssertionError):
+        kv_ops.destindex_copy_quantize_and_register_kv(2, *a[1:])
+    assert torch.equal(raw, before)
+    kv_ops.destindex_copy_quantize_and_register_kv(*a)
+    assert not torch.equal(raw[[1, 3]], before[[1, 3]]) and a[11][0, :2].tolist() == [3, 1]

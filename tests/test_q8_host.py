@@ -1,4 +1,5 @@
-"""Host side of the 8-bit serving path: the Llama stack's glue around the operators, on stand-ins of their shapes (no GPU needed)."""
+"""Host side of the 8-bit serving path: the Llama stack's glue around the operators, on stand-ins of their shapes, and checks that are
+made before a launch (no GPU needed)."""
 from types import SimpleNamespace
 
 import pytest
@@ -59,3 +60,41 @@ def test_a_prefill_of_which_an_instance_holds_few_tokens_or_none(monkeypatch, n)
     hidden = stack.prefill(torch.zeros(n, dtype=torch.long), torch.arange(n), None)
     assert hidden.shape == (n, 64)
     assert stack.prefill(torch.zeros(n, dtype=torch.long), torch.arange(n), None, last_token_rows=torch.arange(n)).shape == (n, 10)
+
+
+def keep_range_args(batch):
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)
+    lay = dict(codes=torch.zeros(9, 2, 128, dtype=torch.int8), scales=torch.zeros(9, 2))
+    vectors = dict(new_len=i32(batch), begin=i32(batch), end=i32(batch), start=i32(batch), cur=i32(batch), b_req=i32(batch))
+    rest = dict(cumsum=torch.zeros(batch, dtype=torch.int64), kv=torch.zeros(4, 2, 128, dtype=torch.bfloat16), mem=torch.zeros(4, dtype=torch.int64),
+                table=torch.zeros(3, 8, dtype=torch.int32))
+    return {**lay, **vectors, **rest}
+
+
+def keep_range(a, batch):
+    from loongserve_b200 import kv_ops
+    kv_ops.destindex_copy_quantize_and_register_kv(batch, a["new_len"], a["begin"], a["end"], a["cumsum"], a["kv"], a["start"], a["cur"], a["mem"],
+                                                   a["codes"], a["scales"], a["table"], a["b_req"], 0, 4, True)
+
+
+def test_the_keep_range_write_looks_where_every_tensor_lies(monkeypatch):
+    """The kernel reads all of them: a vector left on the host must not get as far as the launch."""
+    from loongserve_b200 import kv_ops
+    a = keep_range_args(2)
+    seen = []
+    monkeypatch.setattr(kv_ops, "need_here", lambda *ts: seen.extend(id(t) for t in ts))
+    monkeypatch.setattr(kv_ops, "need_i32", lambda *ts: (_ for _ in ()).throw(InterruptedError))
+    with pytest.raises(InterruptedError):
+        keep_range(a, 2)
+    assert {k for k, t in a.items() if id(t) not in seen} == set()
+
+
+@pytest.mark.parametrize("short", ["new_len", "begin", "end", "start", "cur", "b_req", "cumsum"])
+def test_the_keep_range_write_wants_an_entry_for_every_request(monkeypatch, short):
+    from loongserve_b200 import kv_ops
+    a = keep_range_args(3)
+    a[short] = a[short][:2]
+    monkeypatch.setattr(kv_ops, "need_here", lambda *ts: 0)
+    monkeypatch.setattr(kv_ops._lib, "attn", lambda: pytest.fail("a launch"))
+    with pytest.raises(AssertionError, match="every request"):
+        keep_range(a, 3)
