@@ -48,7 +48,9 @@ class ESPAttentionRuntime:
     ``total_rank`` is this instance's SP rank.  ``dtype`` is the KV / activation dtype (fp16 or bf16).
     ``kv_dtype`` torch.int8 or torch.float8_e4m3fn holds the pool in 8 bits (all instances alike): K/V rows are computed and
     attended to in ``dtype`` during prefill, quantised as they are written to the pool, and read as codes by decode and
-    migration.  The peer-memory decode exchange is not available then (the message exchange is)."""
+    migration.  The peer-memory decode exchange is not available then (the message exchange is).
+    ``decode_block_seq``: tokens per split of decode attention; by default up to 256, or, where a batch lives on one instance with an
+    8-bit pool, the tokens of all its requests divided evenly."""
 
     def __init__(self, *, layers_num: int, q_head_num: int, kv_head_num: int, head_dim: int, max_total_token_num: int,
                  max_req_num: int, max_seq_length: int, sp_world_size: int = 1, total_rank: int = 0, sp_comm=None,
@@ -422,7 +424,7 @@ class ESPAttentionRuntime:
             if self.kv_quantized:
                 k, v = pool_layer[:, :Hkv, :], pool_layer[:, Hkv:, :]
                 o, _ = fd.token_decode_attention_q8(qv.contiguous(), k.codes, k.scales, v.codes, v.scales, self.req_manager.req_to_token_indexs,
-                                                    mp.b_req_idx, mp.b_seq_len, mp.max_len_in_batch,
+                                                    mp.b_req_idx, mp.b_seq_len, mp.max_len_in_batch, block_seq=self.decode_block_seq,
                                                     out=None if out is None else out.view_as(qv), out_logexpsum=mp.global_out_lse)
                 return o if out is None else out
             fd.flash_decoding_stage1(mp.global_mid_o, mp.global_mid_lse, qv, pool_layer[:, :Hkv, :], pool_layer[:, Hkv:, :],

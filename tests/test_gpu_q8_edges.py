@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from test_gpu_q8 import BF16, D, DEV, E4M3, INT8, check_decode, decode_case, decode_exact
+from test_gpu_q8_runtime import exact_over_pool, i32, make_runtime, prefill, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +58,19 @@ def test_keep_range_write_refuses_vectors_of_the_host():
     assert torch.equal(raw, before)
     kv_ops.destindex_copy_quantize_and_register_kv(*a)
     assert not torch.equal(raw[[1, 3]], before[[1, 3]]) and a[11][0, :2].tolist() == [3, 1]
+
+
+@pytest.mark.parametrize("block", [None, 32, 100])
+def test_a_decode_step_with_splits_of_its_own(block):
+    g = torch.Generator().manual_seed(3)
+    lens = [300, 7, 130]
+    rt = make_runtime(INT8, decode_block_seq=block)
+    b_req, _, _ = prefill(rt, lens, rows(437, 2, 8, g), rows(437, 2, 4, g))
+    lens = [n + 1 for n in lens]
+    st = rt.prepare_decode(3, 3, max(lens), b_req, i32(lens), i32([n - 1 for n in lens]), 0, [0], 0)
+    q, kv = torch.randn(3, 8, D, generator=g).to(BF16).to(DEV), torch.randn(3, 4, D, generator=g).to(BF16).to(DEV)
+    for layer in range(2):
+        rt.decode_cache_kv(st, layer).copy_(kv)
+        rt.post_decode_cache_kv(st, layer)
+        check_decode(rt.token_attention(q, st, layer), st.global_out_logexpsum, exact_over_pool(rt, layer, q, b_req, lens), max(lens))
+    rt.check_device_status()

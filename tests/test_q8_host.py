@@ -98,3 +98,25 @@ def test_the_keep_range_write_wants_an_entry_for_every_request(monkeypatch, shor
     monkeypatch.setattr(kv_ops._lib, "attn", lambda: pytest.fail("a launch"))
     with pytest.raises(AssertionError, match="every request"):
         keep_range(a, 3)
+
+
+def decode_step(monkeypatch, peers, **kw):
+    """A decode step of two requests on an 8-bit pool, without its kernels: (state, arguments that attention got)."""
+    from loongserve_b200 import attention_runtime as ar
+    monkeypatch.setattr(ar.kv_ops, "copy_kv_index_to_req", lambda *a: None)
+    got = []
+    monkeypatch.setattr(ar.fd, "token_decode_attention_q8", lambda q, *a, **k: (got.append((a, k)), (q, None))[1])
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    rt = ar.ESPAttentionRuntime(layers_num=1, q_head_num=4, kv_head_num=2, head_dim=128, max_total_token_num=2048, max_req_num=4, max_seq_length=1024,
+                                device="cpu", kv_dtype=torch.int8, **kw)
+    st = rt.prepare_decode(2, 2, 700, i32(0, 1), i32(700, 30), i32(699, 29), 0, peers, 0)
+    if len(peers) == 1:
+        rt.token_attention(torch.zeros(2, 4, 128, dtype=torch.bfloat16), st, 0)
+    return st, got
+
+
+@pytest.mark.parametrize("block", [None, 64, 100])
+def test_splits_asked_for_reach_attention_over_an_8_bit_pool(monkeypatch, block):
+    st, got = decode_step(monkeypatch, [0], decode_block_seq=block)
+    (args, kw), = got
+    assert kw["block_seq"] == block and args[-1] == 700 and kw["out_logexpsum"] is st.global_out_logexpsum
