@@ -366,8 +366,10 @@ class ESPAttentionRuntime:
         if is_master:
             nblk = (max_len_in_batch + st.BLOCK_SEQ - 1) // st.BLOCK_SEQ
             st.num_seq_block = nblk
-            st.global_mid_o = torch.empty((P - 1 + nblk, batch_size, Hq, D), **f32)
-            st.global_mid_o_logexpsum = torch.empty((P - 1 + nblk, batch_size, Hq), **f32)
+            # attention over an 8-bit pool of this instance alone keeps its partials itself (``token_attention``)
+            parts = not (self.kv_quantized and P == 1 and peer_sp_master_rank_list is None)
+            st.global_mid_o = torch.empty((P - 1 + nblk, batch_size, Hq, D), **f32) if parts else None
+            st.global_mid_o_logexpsum = torch.empty((P - 1 + nblk, batch_size, Hq), **f32) if parts else None
             st.global_merge_len = ((P - 1) + (b_seq_len + (st.BLOCK_SEQ - 1)) // st.BLOCK_SEQ).view((batch_size,)).to(torch.int32).contiguous().clone()
             st.global_out_logexpsum = torch.empty((batch_size, Hq), **f32)
             st.master_plan = ringmod.MasterPlan(peers=list(logical_sp_peer_ranks), b_req_idx=b_req_idx, b_seq_len=b_seq_len,

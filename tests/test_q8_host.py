@@ -120,3 +120,10 @@ def test_splits_asked_for_reach_attention_over_an_8_bit_pool(monkeypatch, block)
     st, got = decode_step(monkeypatch, [0], decode_block_seq=block)
     (args, kw), = got
     assert kw["block_seq"] == block and args[-1] == 700 and kw["out_logexpsum"] is st.global_out_logexpsum
+
+
+def test_a_step_of_one_instance_holds_no_partials_that_nothing_reads(monkeypatch):
+    st, _ = decode_step(monkeypatch, [0])
+    assert st.global_mid_o is None and st.global_mid_o_logexpsum is None and st.global_out_logexpsum.shape == (2, 4)
+    st, _ = decode_step(monkeypatch, [0, 1], sp_world_size=2)
+    assert st.global_mid_o.shape == (1 + 3, 2, 4, 128) and st.master_plan.global_mid_lse.shape == (1 + 3, 2, 4)
