@@ -108,7 +108,9 @@ int esp_prefill_lse(const float* m, const float* l, float* lse, int64_t n, void*
 
 /* Device-side status of the bounded waits inside the prefill kernels and esp_mm_w8a8 on the current device:
  * out[0] = 0 or ESP_ERR_DEVICE_TIMEOUT, out[1] = block index, out[2] = which wait (100 and above: esp_mm_w8a8), out[3] = detail.
- * Synchronises the device.  `clear` != 0 resets it. */
+ * Synchronises the device.  `clear` != 0 resets it.  The prefill kernels and esp_mm_w8a8 have a word each: with both set this shows
+ * (and clears) that of the prefill kernels, the next call the other.  The same goes for the 16-bit and the 8-bit kernels behind
+ * esp_decode_device_status and esp_kv_device_status. */
 int esp_device_status(int32_t out[4], int32_t clear);
 
 /* Limit, in SM cycles, of every bounded in-kernel wait of this library on the CURRENT device (the mbarrier waits of the
@@ -229,8 +231,8 @@ int esp_decode_merge_gated(void* o, float* out_lse, const int32_t* b_seqlen, con
                            void* stream);
 /* Status of the decode kernels and flag waits on the current device, like esp_device_status: out[0] = 0,
  * ESP_ERR_DEVICE_TIMEOUT (out[2] = which wait: 1 stage-1 gate, 2 merge gate, >= 16 esp_flag_wait ids; out[3] = awaited
- * value) or ESP_ERR_BAD_SLOT (out[3] = the slot id stage 1 refused).  After a timeout every later gated kernel on the
- * device returns at once until the status is cleared. */
+ * value; 8 and 9 the copies of the 8-bit stage 1, out[3] = the step) or ESP_ERR_BAD_SLOT (out[3] = the slot id stage 1 refused).  After
+ * a timeout every later gated kernel on the device returns at once until the status is cleared, and so do the 8-bit ones. */
 int esp_decode_device_status(int32_t out[4], int32_t clear);
 
 /* ------------------------------------------------------------------------------------------------
@@ -243,7 +245,8 @@ int esp_decode_device_status(int32_t out[4], int32_t clear);
  */
 
 /* out[0] = 0 or ESP_ERR_BAD_SLOT, out[1] = kernel (1 scatter, 2 scatter+register, 3 migration gather, 4 migration
- * scatter), out[2] = position of the id in its index array, out[3] = the id.  Synchronises the device. */
+ * scatter; 8-bit pool: 5 scatter, 6 scatter+register, 7 read-back), out[2] = position of the id in its index array, out[3] = the id.
+ * Synchronises the device. */
 int esp_kv_device_status(int32_t out[4], int32_t clear);
 
 /* out[dest[i]] = src[i], i < n.  Replaces destindex_copy_kv

@@ -169,12 +169,17 @@ class ESPAttentionRuntime:
         the last check.  Synchronises the device: call it where the caller synchronises anyway (``token_attention`` does
         every ``status_check_interval`` decode layers calls).  After a timed-out wait the gated kernels of the device
         return at once and publish nothing until the status has been read here."""
-        st = ca.device_status()
-        dst = fd.device_status(clear=True)
-        kst = kv_ops.device_status(clear=True)
-        for name, v in (("prefill kernel", st), ("decode kernels / flag waits", dst), ("KV pool kernels", kst)):
-            if v[0] != 0:
-                raise RuntimeError(f"ESP attention device status, {name}: code {v[0]} ({tuple(v)})")
+        found = []
+        for read, name in ((ca.device_status, lambda v: "8-bit product" if v[2] >= 100 else "prefill kernel"),
+                           (fd.device_status, lambda v: "8-bit decode kernel" if v[0] == -4 and v[2] in (8, 9) else "decode kernels / flag waits"),
+                           (kv_ops.device_status, lambda v: "8-bit KV pool kernels" if v[1] >= 5 else "KV pool kernels")):
+            for _ in range(2):                  # the 16-bit kernels' word, then the 8-bit kernels'
+                v = read(clear=True)
+                if v[0] == 0:
+                    break
+                found.append(f"{name(v)}: code {v[0]} ({tuple(v)})")
+        if found:
+            raise RuntimeError("ESP attention device status, " + "; ".join(found))
 
     # ------------------------------------------------------------------------------------------ prefill
     @torch.no_grad()

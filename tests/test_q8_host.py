@@ -127,3 +127,20 @@ def test_a_step_of_one_instance_holds_no_partials_that_nothing_reads(monkeypatch
     assert st.global_mid_o is None and st.global_mid_o_logexpsum is None and st.global_out_logexpsum.shape == (2, 4)
     st, _ = decode_step(monkeypatch, [0, 1], sp_world_size=2)
     assert st.global_mid_o.shape == (1 + 3, 2, 4, 128) and st.master_plan.global_mid_lse.shape == (1 + 3, 2, 4)
+
+
+@pytest.mark.parametrize("words,names", [
+    ([[(-4, 3, 101, 7)], [], []], ["8-bit product"]), ([[(-4, 3, 6, 7)], [], []], ["prefill kernel"]),
+    ([[(-4, 3, 6, 7), (-4, 0, 104, 1)], [(-4, 1, 2, 5), (-4, 1, 9, 5)], [(-8, 1, 0, 3), (-8, 6, 0, 3)]],
+     ["prefill kernel", "8-bit product", "decode kernels / flag waits", "8-bit decode kernel", "KV pool kernels", "8-bit KV pool kernels"]),
+    ([[], [(-8, 0, 0, 99)], [(-8, 7, 2, -1)]], ["decode kernels / flag waits", "8-bit KV pool kernels"]), ([[], [], []], [])])
+def test_the_device_status_names_every_kernel_that_reported(monkeypatch, words, names):
+    from loongserve_b200 import attention_runtime as ar
+    for mod, left in zip((ar.ca, ar.fd, ar.kv_ops), words):
+        monkeypatch.setattr(mod, "device_status", lambda clear=True, left=list(left): left.pop(0) if left else (0, 0, 0, 0))
+    check = lambda: ar.ESPAttentionRuntime.check_device_status(SimpleNamespace())
+    if names:
+        with pytest.raises(RuntimeError) as e:
+            check()
+        assert [part.split(":")[0] for part in str(e.value).removeprefix("ESP attention device status, ").split("; ")] == names
+    check()                                     # all of it has been read
