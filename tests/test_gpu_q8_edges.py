@@ -3,7 +3,7 @@ its own."""
 import pytest
 import torch
 
-from test_gpu_q8 import BF16, D, DEV, E4M3, INT8, check_decode, decode_case, decode_exact
+from test_gpu_q8 import BF16, D, DEV, E4M3, F16, INT8, U32, check_decode, decode_case, decode_exact
 from test_gpu_q8_runtime import exact_over_pool, i32, make_runtime, prefill, rows
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +74,68 @@ def test_a_decode_step_with_splits_of_its_own(block):
         rt.post_decode_cache_kv(st, layer)
         check_decode(rt.token_attention(q, st, layer), st.global_out_logexpsum, exact_over_pool(rt, layer, q, b_req, lens), max(lens))
     rt.check_device_status()
+
+
+def launch_shapes(test):
+    """Groups of up to four heads (rests in the columns of heads 4 to 7) and of more (a second product), one, two and four kv heads to
+    a CTA."""
+    return pytest.mark.parametrize("code", [INT8, E4M3])(pytest.mark.parametrize("hq,hkv,batch", [
+        (8, 2, 4), (32, 32, 10), (32, 32, 20), (10, 2, 4), (16, 2, 4), (160, 32, 10), (256, 32, 20), (20, 1, 4)])(test))
+
+
+@launch_shapes
+def test_decode_weights_keep_both_their_f16_numbers(code, hq, hkv, batch):
+    """K scales of zero make every score 0 and every p exactly 1, so nothing covers the weights' own error.
+
+    Roundings, relative to the mean of |v|: a weight is vs * (4096 / v_ref), 2; held as an f16 number and the f16 rounding of its rest,
+    2^-22 (and 2^-25 absolute next to weights of 128 at least); 2n terms (both numbers of n weights) are added up, at most 2^-23
+    each where the sum is cut instead of rounded; moving the reference, twice 1; the shares of four warps, three times 4; the two
+    halves, the factor and its product, 4."""
+    from loongserve_b200 import flash_decoding as fd
+    lens = [17, 1, 3, 16] * (batch // 4) + [5] * (batch % 4)
+    c = decode_case(lens, hq, hkv, BF16, code, hq + batch)
+    g = torch.Generator().manual_seed(batch)
+    c["scales"][:, :hkv] = 0.0
+    c["scales"][:, hkv:] = (1 + 7 * torch.rand(c["scales"].shape[0], hkv, generator=g)).to(DEV)
+    out = torch.empty(batch, hq, D, device=DEV); lse = torch.empty(batch, hq, device=DEV)
+    fd.token_decode_attention_q8(c["q"], c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"], c["rows"],
+                                 c["lens"], 17, None, out, lse)
+    n = torch.tensor(lens, dtype=torch.float64)[:, None]
+    ro, _, wabs, _, _, _ = decode_exact(c)
+    tol = (2.0 ** -22 + 2.0 ** -32 + 2 * n * 2.0 ** -23 + 20 * U32)[..., None] * wabs
+    assert bool(((out.double().cpu() - ro).abs() <= tol).all()), ((out.double().cpu() - ro).abs() / tol).max()
+    assert bool(((lse.double().cpu() - n.log()).abs() <= 4 * U32 * n.log() + 2.0 ** -30).all())
+    # the bound is of use: weights without their rests do not keep it
+    worst = 0.0
+    for b, m in enumerate(lens):
+        slots = c["table"][int(c["rows"][b]), :m].long()
+        vs = c["scales"][slots, hkv:].double().cpu()                                             # [m, hkv]
+        w = (vs * (1024 / vs.amax(0))).to(F16).double() * vs.amax(0) / 1024
+        v = c["codes"].view(torch.uint8)[slots].view(code)[:, hkv:].double().cpu() * w[..., None]
+        off = (v.mean(0).repeat_interleave(hq // hkv, 0) - ro[b]).abs() / tol[b]
+        worst = max(worst, float(off.max()))
+    assert worst > 4
+
+
+@launch_shapes
+def test_decode_scores_of_single_tokens(code, hq, hkv, batch):
+    """A request of one token: p is exactly 1, and lse is the score itself.
+
+    Roundings.  The factor sm_scale * log2(e), its two constants and the way back to natural logarithms: 6, and 2 of the K scale's
+    products, relative to the score.  int8: the sum over the query's integer is exact; its digits meet in 3 roundings of sums
+    below sum|q k| and what a lower digit can have more than its place (2^-6 of the largest element); the integer is off by half
+    of 2^-29 (groups of up to four) or 2^-21 of the largest.  e4m3: 128 exact products are added up, at most 2^-23 each; elements below
+    2^-21 of the largest are rounded by 2^-32 of it."""
+    from loongserve_b200 import flash_decoding as fd
+    c = decode_case([1] * batch, hq, hkv, BF16, code, hq - batch)
+    out = torch.empty(batch, hq, D, device=DEV); lse = torch.empty(batch, hq, device=DEV)
+    fd.token_decode_attention_q8(c["q"], c["codes"][:, :hkv], c["scales"][:, :hkv], c["codes"][:, hkv:], c["scales"][:, hkv:], c["table"], c["rows"],
+                                 c["lens"], 1, None, out, lse)
+    ro, rl, wabs, sabs, qabs, _ = decode_exact(c)
+    if code is INT8:
+        ds = 3 * U32 * (sabs + 2.0 ** -6 * qabs) + (2.0 ** -30 if hq // hkv <= 4 else 2.0 ** -22) * qabs
+    else:
+        ds = 128 * 2.0 ** -23 * sabs + 2.0 ** -32 * qabs
+    tol = 8 * U32 * rl.abs() + ds
+    assert bool(((lse.double().cpu() - rl).abs() <= tol).all()), ((lse.double().cpu() - rl).abs() / tol).max()
+    assert bool(((out.double().cpu() - ro).abs() <= (2.0 ** -22 + 12 * U32) * wabs).all())
