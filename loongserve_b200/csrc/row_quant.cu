@@ -12,6 +12,7 @@
 // the next row there cost more in registers than it gained.  Measured (B200): add + norm into codes 16384 x 4096 72 us for 470 MB,
 // SiLU * mul into codes 8192 x 11008 74 us for 451 MB, codes back into rows 16384 x 4096 35 us for 201 MB.
 #include "quant_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace esp {
 
@@ -25,6 +26,15 @@ struct RowArgs {
     float eps, inv_cols;
     int64_t rows;
 };
+
+// silu(g) * u.  1 + exp(-g) reaches 2^128 before it overflows, and its reciprocal is subnormal from 2^126 on, where g / (1 + exp(-g)) is
+// still a normal number: both are taken 2^16 apart, which is given back by u (exactly: a 16-bit number times 2^-16 is an fp32 number).
+__device__ __forceinline__ float silu_mul(float g, float u) {
+    constexpr float kDown = 1.f / 65536.f;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(ptx::ex2(g * -1.4426950408889634f), kDown, kDown)));
+    return g * (r * (u * kDown));
+}
 
 template <int VPT> struct RowData { uint4 a[VPT], b[VPT]; };
 
@@ -73,8 +83,8 @@ __global__ void __launch_bounds__(WARP ? 256 : (VPT == 2 ? 512 : (VPT == 4 ? 512
                     if (MODE == ROW_ADD_NORM) { const float2 g = Cvt<T>::to_f2(q[k]); f.x += g.x; f.y += g.y; }
                     if (MODE == ROW_SILU) {
                         const float2 g = Cvt<T>::to_f2(q[k]);
-                        f.x = __fdividef(f.x, 1.f + __expf(-f.x)) * g.x;
-                        f.y = __fdividef(f.y, 1.f + __expf(-f.y)) * g.y;
+                        f.x = silu_mul(f.x, g.x);
+                        f.y = silu_mul(f.y, g.y);
                     }
                     if (kNorm) { ss = fmaf(f.x, f.x, ss); ss = fmaf(f.y, f.y, ss); }
                     t[c][2 * k] = f.x; t[c][2 * k + 1] = f.y;

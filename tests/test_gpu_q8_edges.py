@@ -139,3 +139,19 @@ def test_decode_scores_of_single_tokens(code, hq, hkv, batch):
     tol = 8 * U32 * rl.abs() + ds
     assert bool(((lse.double().cpu() - rl).abs() <= tol).all()), ((lse.double().cpu() - rl).abs() / tol).max()
     assert bool(((out.double().cpu() - ro).abs() <= (2.0 ** -22 + 12 * U32) * wabs).all())
+
+
+def test_silu_where_the_denominator_nears_the_end_of_the_range():
+    """Gates from -88.5 to -87 give 1 + exp(-g) of 2^125 to 2^128; next to up values of 1e36 and more the products are ordinary
+    numbers.  exp(-g) is off by 2 + 1.173 * 88.5 ulp, its reciprocal by one; then two products: within 2^-16 relative."""
+    from loongserve_b200 import layer_ops as ops
+    g = torch.Generator().manual_seed(2)
+    gate = torch.linspace(-88.5, -87.0, 256).to(BF16)
+    up = (torch.randn(3, 256, generator=g) * torch.tensor([[1e36], [1e37], [3e37]])).to(BF16)
+    io = torch.cat([gate.expand(3, -1), up], 1).contiguous()
+    codes, scale = ops.silu_and_mul_quant(io.to(DEV))
+    y = gate.double() * torch.sigmoid(gate.double()) * up.double()
+    s = y.abs().amax(-1) / 127
+    assert bool(((scale.double().cpu() - s).abs() <= (2.0 ** -16 + 2 * U32) * s).all())
+    v = codes.double().cpu() * scale.double().cpu()[:, None]
+    assert bool(((v - y).abs() <= (0.5 + 127 * 2.0 ** -15) * s[:, None]).all())
