@@ -468,7 +468,7 @@ int esp_dequantize_rows(void* out, const int8_t* codes, const float* scale, int6
                         int32_t dtype, void* stream);
 
 /* out[m, n] = (sum_k a[m, k] * w[n, k]) * a_scale[m] * w_scale[n]: int8 operands with K contiguous, exact 32-bit integer
- * sums, one rounding to out_dtype (F16/BF16/F32).  Row strides in elements; k and the int8 row strides multiples of 16,
+ * sums, then fp32 (the sum, two products) and the rounding to out_dtype (F16/BF16/F32).  Row strides in elements; k and the int8 row strides multiples of 16,
  * k <= 131071 (the sums stay inside 32 bits). */
 int esp_mm_w8a8(void* out, int64_t out_row_stride, const int8_t* a, int64_t a_row_stride, const float* a_scale,
                 const int8_t* w, int64_t w_row_stride, const float* w_scale, int64_t m, int64_t n, int64_t k,

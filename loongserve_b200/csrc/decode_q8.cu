@@ -5,8 +5,8 @@
 //
 // Bound by HBM: 2 * (128 + 4) bytes per token and kv head, each read once (64 requests x 4096-65536 tokens x 32 kv heads, 17.9 GB:
 // 2.74 ms, 6.5 TB/s; the 16-bit pool of the same requests 5.13 ms), and next to that by power: a GPU that runs it without a pause
-// lowers its clocks (32 requests x 1K-16K tokens x 32 kv heads: 338 us in a burst, 390 in a loop at 980 W), so instructions per
-// byte count.  At that rate one SM has to take in a code every 1/23 of a cycle and multiply it with up to 8 query heads, which is
+// lowers its clocks (at 980 W a call of 32 requests x 1K-16K tokens x 32 kv heads takes 15 % longer in a loop than in a burst), so
+// instructions per byte count.  At that rate one SM has to take in a code every 1/23 of a cycle and multiply it with up to 8 query heads, which is
 // past what fp32 lanes do next to the conversion; the products run on the tensor cores (mma.sync), which are far from their limit
 // here.  A lane reads 16-byte pieces of the rows and its pieces ARE operand fragments, because the order of the summed index
 // (head dims for S, tokens for O) is free:
@@ -22,8 +22,9 @@
 //   of 22 bits in three (GT = 8: rows j, j + 8, and a second product).  Against codes brought to f16 this saves a third of the
 //   instructions: 477 us instead of 499 for the 32 requests above, in a loop, before the copies were what they are now.
 //   S, e4m3 codes: brought to f16 (exactly; two instructions a word), q scaled to 2^7 in f16, exact down to 2^-21 of its largest.
-//   O: codes become f16 (exactly: 8 bits fit).  A weight p * v_scale, relative to 2^-8 * the largest v_scale seen by the warp, enters as
-//   its rounding to f16 and the rounding of what that left: 2^-22 relative.  (The rounding alone, 2^-12, showed in f16 outputs: 3.3e-4
+//   O: codes become f16 (exactly: 8 bits fit).  A weight p * v_scale enters in units of 2^-12 * v_ref, v_ref 1 to 4 times the largest v_scale
+//   that the warp has seen, as its rounding to f16 and the rounding of what that left: 2^-22 relative, and at least 2^-37 of v_ref (below f16's
+//   normal range), so that a token whose v_scale is far below the largest has fewer bits.  (The rounding alone, 2^-12, showed in f16 outputs: 3.3e-4
 //   against 2.0e-4 for fp32 weights.)  With GT = 4 the rests take the columns of heads 4-7 and cost no product; GT = 8 multiplies V
 //   twice.
 #include <algorithm>
@@ -60,7 +61,7 @@ struct DecodeQ8Args {
 
 constexpr int kQ8Warps = 4, kQ8HeadTile = 8;
 constexpr int kQ8Resident = 3 * kNumSMs, kQ8MinPiece = 64;       // CTAs the GPU holds; tokens below which a piece is not cut
-// requests up to this length are not cut at all
+// requests up to this length are not cut at all (measured at the call that uses it)
 inline int q8_whole(int batch) { return batch < 8 ? 256 : 512; }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -105,9 +106,9 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 //            a piece that crosses requests has an item for each.  Pieces and requests both only grow along the way, so piece + request
 //            numbers a partial uniquely, and there are at most pieces + requests of them.  A request inside one piece gets its results
 //            at once.  Against splits of a fixed length every CTA has the same work and writes a partial or two instead of one per
-//            128 to 512 tokens: 180 us instead of 186 (the best length) to 222 for 2 requests x 200K-262K tokens x 8 kv heads (group 4), 76
-//            instead of 87 to 126 for 64 requests x 4 kv heads (group 8), 338 instead of 347 to 409 for 32 requests x 1K-16K tokens x
-//            32 kv heads.
+//            128 to 512 tokens: 185 us instead of 195 (the best length) to 241 for 2 requests x 8 kv heads (group 4), 501702 tokens; 66
+//            instead of 76 to 80 for 64 requests x 4096 tokens x 4 kv heads (group 8); 392 instead of 389 (splits of 512) to 467 (of 128)
+//            for 32 requests x 32 kv heads, 287567 tokens.
 //   counted  splits of seq_block_size tokens, where a CTA has several and the batch is small enough: those that exist are counted
 //            first, so that ragged batches divide evenly.
 //   else     all splits up to the longest possible request; those behind a request's end are passed over.
@@ -812,8 +813,9 @@ extern "C" int esp_decode_attention_q8(void* o, float* lse, float* workspace, co
     if (o_dtype != ESP_DTYPE_F16 && o_dtype != ESP_DTYPE_BF16 && o_dtype != ESP_DTYPE_F32) return ESP_ERR_BAD_ARG;
     const int32_t max_len = max_len_in_batch > 0 ? max_len_in_batch : 1;
     // seq_block_size 0: equal pieces, or one split where no request is longer than 256 tokens (512 from 8 requests on), which saves
-    // the merge.  Pieces / one split in us (both 0.6 more than they are now), 8 kv heads, group 4: one request of 256 tokens 8.2 / 8.3, of 512 9.9 / 11.3; 16 ragged ones
-    // of up to 512 13.4 / 11.1, 64 of them 19.5 / 18.3, 256 50.3 / 51.0.
+    // the merge.  Pieces / one split in us, 8 kv heads, group 4: one request of 256 tokens 8.7 / 7.4; 16 of 512 11.7 / 11.2, 64 of
+    // them 25.6 / 20.5, 256 71.4 / 65.3; 32 kv heads, 8 of 512 16.4 / 14.3.  The rule does not count heads: with a single kv head there are
+    // too few CTAs in one split (8 requests of 512 tokens 9.4 / 10.8, 32 of them 10.1 / 11.1).
     const bool even = seq_block_size == 0 && max_len > q8_whole(batch);
     const int32_t block = seq_block_size == 0 ? (even ? kQ8MinPiece : max_len) : seq_block_size;
     const int64_t nblk = (max_len + (int64_t)block - 1) / block;

@@ -8,7 +8,8 @@
 // head row with 16 elements each: two 16-byte loads, the row's maximum by shuffles over its lanes, a 16-byte store of codes; the
 // data is read once and stays in registers.  A lane group's token and head come from shifts, not from a division of the row
 // number: with the division, and with 8 elements per lane, the instructions were the bound (16384 tokens x 64 heads: 82 and
-// 108 us; as it is 71 us for 407 MB, the way back 69).
+// 108 us; as it is 71 us for 407 MB, the way back 68).  The keep-range form has one row of a lane group in flight and takes 82 us for the same
+// rows from 8 requests.
 #include "quant_common.cuh"
 
 namespace esp {

@@ -6,11 +6,14 @@
 //   codes        int8, scale = max|y| / 127 (quant_common.cuh)
 // The norm is taken of the unrounded sum, so the output is rounded once; what is kept for the next layer is the rounded one.
 //
-// HBM bound: every element is read once, held in registers in fp32 (up to 8 * VPT per thread) across the row's reduction,
+// HBM bound: every element is read once, held in fp32 (8 * VPT per thread; in registers up to 16384 wide) across the row's reduction,
 // and written once.  Rows of up to 512 elements: a warp per row, eight rows to a CTA, the next row asked for before the one in hand
 // is reduced (60000 rows of 256 into codes: a CTA of one warp per row took 33 us, this form 10).  Wider rows: a CTA per row; asking for
-// the next row there cost more in registers than it gained.  Measured (B200): add + norm into codes 16384 x 4096 72 us for 470 MB,
-// SiLU * mul into codes 8192 x 11008 74 us for 451 MB, codes back into rows 16384 x 4096 35 us for 201 MB.
+// the next row there cost more in registers than it gained.  Measured (B200): add + norm into codes 16384 x 4096 70.5 us for 470 MB,
+// SiLU * mul into codes 8192 x 11008 71.7 us for 451 MB, plain rows into codes 16384 x 4096 38.8 us and back 34.0 us for 201 MB.
+// Rows wider than 16384 (VPT 8) are compiled for 1024 threads and do not fit the registers that this leaves: 60 to 220 bytes per thread
+// go through local memory, with the residual add 820.  4096 x 28672: SiLU * mul 127 us (0.71 of the copy rate), plain rows 76 (0.71), add +
+// norm 415 (0.30).
 #include "quant_common.cuh"
 #include "sm100_ptx.cuh"
 

@@ -1,7 +1,8 @@
 // Product of 8-bit integer matrices with a scale for every token and every output channel:
 //   out[m, n] = (sum_k a[m, k] * w[n, k]) * a_scale[m] * w_scale[n]
 // a [M, K] int8 rows of tokens, w [N, K] int8 rows of output channels (both with K contiguous), 32-bit integer sums in tensor
-// memory (tcgen05.mma kind::i8), two fp32 products and one rounding to the output type in the epilogue.  K <= 131071 keeps every
+// memory (tcgen05.mma kind::i8); in the epilogue the sum becomes fp32 (rounded where it has more than 24 bits), is multiplied twice and
+// rounded to the output type.  K <= 131071 keeps every
 // sum inside 32 bits (128 * 128 * K < 2^31).  Integer sums do not depend on their order, so every split below gives the same bits.
 //
 // Operand tiles are 128 bytes of K wide, 128-byte swizzle, fetched by TMA (rows and bytes behind the matrix arrive as zeros).
@@ -534,7 +535,8 @@ static int launch_mm(const int8_t* a, int64_t lda, const int8_t* w, int64_t ldw,
     // The variant with the least estimated time (us).  A skinny CTA costs about 6 us around its stages; a stage costs less while
     // every SM has one CTA than with two (which then share the SM's intake).  A pair costs 5.4 or 6.5 us and 0.29 or 0.31 us per
     // stage and wave of tiles.  Measured against these estimates (B200, tokens x channels x K, us,
-    // each call by itself; with its start under the kernel before it a skinny one takes 1 to 2 us less):
+    // each call by itself; with its start under the kernel before it a skinny one takes 1 to 2 us less, which the estimates leave out: near
+    // a border pairs are taken somewhat too often):
     //   64 x 4096 x 11008: TN 64 in 8 splits 13.8, 4 splits 15.2, 1 split 29.2, pairs 31.0      256 x 4096 x 11008: TN 128 in 4 splits 20.1, pairs 31.0
     //   256 x 22016 x 4096: TN 64 50.8, TN 128 54.3, pairs of 256 29.7                          512 x 4096 x 1280: TN 64 12.9, pairs of 128 8.3, of 256 9.6
     //   600 x 600 x 8000: TN 64 in 4 splits 12.4, TN 128 in 8 splits 12.5, pairs of 128 24.6    400 x 8000 x 2992: pairs of 256 17.2, of 128 21.0, TN 128 36.7

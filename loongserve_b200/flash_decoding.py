@@ -86,8 +86,8 @@ Q8_MAX_EVEN = 384          # requests whose tokens one call divides evenly
 
 def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -> int:
     """Tokens per split, where splits have a fixed length: eight times as many (split, heads) items as the GPU holds CTAs, within 128
-    and 512 tokens.  Shorter splits cost partials, longer ones leave a tail: 32 requests x 1K-16K tokens x 32 heads take 409 / 357 /
-    347 / 353 / 369 us with 128 / 256 / 512 / 1024 / 2048."""
+    and 512 tokens.  Shorter splits cost partials, longer ones leave a tail: 32 requests x 32 heads, 287567 tokens, take 467 / 410 / 389 /
+    399 / 420 us with 128 / 256 / 512 / 1024 / 2048."""
     tiles = batch * kv_heads * ((group + 7) // 8)
     splits = max(1, -(-148 * 3 * 8 * 4 // max(1, tiles)))
     return min(512, max(128, -(-max(int(max_len_in_batch), 1) // splits // 128) * 128))
@@ -96,8 +96,8 @@ def q8_block_seq(batch: int, kv_heads: int, group: int, max_len_in_batch: int) -
 def token_decode_attention_q8(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len,
                               max_len_in_batch: int, block_seq=None, out=None, out_logexpsum=None, sm_scale: float = 0.0):
     """Decode attention over a pool held in 8 bits, splits and merge in one call: (o like q unless ``out`` is given, lse fp32).
-    ``block_seq``: tokens per split; by default the tokens of up to 384 requests are divided evenly over the GPU (338 us for 32 requests
-    x 1K-16K tokens x 32 heads, 180 us for 2 x 200K-262K x 8; with the best fixed length 347 and 186).  A request of length zero gets
+    ``block_seq``: tokens per split; by default the tokens of up to 384 requests are divided evenly over the GPU (392 us for 32 requests
+    x 32 heads, 287567 tokens, 185 us for 2 x 8, 501702 tokens; with the best fixed length 389 and 195).  A request of length zero gets
     o = 0, lse = -inf."""
     dev = need_here(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len, out, out_logexpsum)
     args, slots = _q8_args(q, cache_k, k_scale, cache_v, v_scale, req_to_token_indexs, b_req_idx, b_seq_len)

@@ -162,7 +162,7 @@ def dequantize_rows(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.bfloat
 
 def mm_w8a8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype=torch.bfloat16, out=None):
     """(a @ w.T) * a_scale[:, None] * w_scale[None]: int8 rows of tokens [M, K] and of output channels [N, K], exact integer sums,
-    one rounding to the output type.  K a multiple of 16, at most 131071."""
+    then fp32 (the sum, two products) and the rounding to the output type.  K a multiple of 16, at most 131071."""
     dev = need_here(a, a_scale, w, w_scale, out)
     sa, sw = a.shape, w.shape
     assert len(sa) == 2 and len(sw) == 2 and sa[1] == sw[1]
