@@ -95,7 +95,8 @@ def build_short_waits(force: bool = False) -> str:
     deps = [SHORT_WAITS_SRC] + [os.path.join(CSRC, f) for f in ("esp_common.cuh", "sm100_ptx.cuh", "quant_common.cuh", "w8a8_gemm.cu", "decode_q8.cu")] + \
         [os.path.join(ROOT, "include", "esp_attention.h")]
     if force or _newer(SHORT_WAITS_LIB, deps):
-        _run([_nvcc()] + NVCC_FLAGS + ["-shared", SHORT_WAITS_SRC, "-o", SHORT_WAITS_LIB])
+        # bound to its own kernels also where the product library is in the process for all to see
+        _run([_nvcc()] + NVCC_FLAGS + ["-Xlinker", "-Bsymbolic", "-shared", SHORT_WAITS_SRC, "-o", SHORT_WAITS_LIB])
     return SHORT_WAITS_LIB
 
 
